@@ -1,3 +1,4 @@
 """Torch-facing operators built on the fused sm_100a kernels."""
 from .fused_gemm import (FusedGemmError, gemm, GemmReduceScatter, AllGatherGemm, fused_lib)  # noqa: F401
 from .moe import MoeDispatchCombine, MoeError  # noqa: F401
+from .norms import rms_norm, block_norms, NormError  # noqa: F401
