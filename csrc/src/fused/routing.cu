@@ -1,0 +1,513 @@
+// Expert router (choice and weights of K experts per token) and balance loss, forward and backward.
+//
+// A warp takes a token: lane l holds the logits of experts l, l + 32, ... in registers, so a row is read once in whole lines and
+// everything after that is shuffles.  The choice is K rounds of a maximum over the warp of keys that order like the floats
+// (redux.sync), the lowest expert among equal keys.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include "../../include/bshmem/routing.h"
+
+namespace bshmem {
+namespace routing {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+
+// Unsigned keys in the order of the floats; 0 for -inf and NaN, which are never chosen.  -0 and 0 are equal.
+__device__ __forceinline__ uint32_t key32(float v) {
+  if (!(v > -CUDART_INF_F)) return 0u;
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key64(double v) {
+  if (!(v > -CUDART_INF)) return 0ull;
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+  return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Largest value of the warp, NaN ignored; -inf if there is none.
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Logits of this lane's experts; -inf past the last.
+template <typename T, int VPL>
+__device__ __forceinline__ void load_row(float (&l)[VPL], const T* row, int E, int lane) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = lane + 32 * i;
+    l[i] = e < E ? to_f(row[e]) : -CUDART_INF_F;
+  }
+}
+
+// Numerator of a score whose sum over a set of experts is divided out.  `top` is the largest logit of the set:
+//   softmax  exp(l - top)
+//   sigmoid  1 / (1 + exp(-l)), times exp(-top) where top < 0, so that a set of very negative logits does not underflow
+__device__ __forceinline__ float numerator(float l, float top, int score) {
+  if (score == BSHMEM_ROUTE_SOFTMAX) return expf(l - top);
+  return expf(fminf(l, 0.f) - fminf(top, 0.f)) / (1.f + expf(-fabsf(l)));
+}
+__device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
+
+struct Params {
+  bshmem_route_args_t a;
+};
+
+template <typename T, int VPL, bool BIAS>
+__global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ Params p) {
+  const bshmem_route_args_t& a = p.a;
+  const int lane = threadIdx.x & 31, K = a.K, E = a.E;
+  const long t = (long)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  if (a.valid && !a.valid[t]) {
+    if (lane < K) {
+      a.idx[t * K + lane] = -1;
+      a.weight[t * K + lane] = 0.f;
+    }
+    return;
+  }
+  const T* row = (const T*)a.logits + t * a.stride;
+  float l[VPL];
+  load_row(l, row, E, lane);
+  bool nan = false;
+  float top = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    nan |= l[i] != l[i];
+    top = fmaxf(top, l[i]);
+  }
+  nan = __any_sync(0xffffffffu, nan);
+  int mine = -1;  // lane k: the k-th chosen expert
+  if constexpr (!BIAS) {
+    uint32_t key[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) key[i] = key32(l[i]);
+    for (int k = 0; k < K; ++k) {
+      uint32_t best = 0;
+      int e = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          e = lane + 32 * i;
+        }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+      if (most == 0) break;
+      const int chosen = (int)__reduce_min_sync(0xffffffffu, best == most ? (unsigned)e : 0xffffffffu);
+      if (lane == k) mine = chosen;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (lane + 32 * i == chosen) key[i] = 0;
+    }
+    top = warp_max(top);
+  } else {
+    top = warp_max(top);
+    uint64_t key[VPL];
+    double s[VPL], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      if (a.score == BSHMEM_ROUTE_SOFTMAX) s[i] = l[i] > -CUDART_INF_F ? exp((double)l[i] - (double)top) : 0.0;
+      else s[i] = 1.0 / (1.0 + exp(-(double)l[i]));
+      sum += s[i];
+    }
+    if (a.score == BSHMEM_ROUTE_SOFTMAX) {
+      sum = warp_sum(sum);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) s[i] /= sum;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      key[i] = e < E && l[i] > -CUDART_INF_F ? key64(s[i] + (double)a.bias[e]) : 0ull;
+    }
+    for (int k = 0; k < K; ++k) {
+      uint64_t best = 0;
+      int e = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          e = lane + 32 * i;
+        }
+      const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
+      const uint32_t most = __reduce_max_sync(0xffffffffu, hi);
+      if (most == 0) break;  // the high half of a key of a finite number is never 0
+      const uint32_t most_lo = __reduce_max_sync(0xffffffffu, hi == most ? lo : 0u);
+      const int chosen = (int)__reduce_min_sync(0xffffffffu, hi == most && lo == most_lo ? (unsigned)e : 0xffffffffu);
+      if (lane == k) mine = chosen;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (lane + 32 * i == chosen) key[i] = 0;
+    }
+  }
+  float w = 0.f;
+  if (a.renormalize) {
+    // the largest chosen logit is the row's unless a bias chose otherwise
+    const float lm = mine >= 0 ? to_f(row[mine]) : -CUDART_INF_F;
+    const float set_top = warp_max(lm);
+    const float num = mine >= 0 ? numerator(lm, set_top, a.score) : 0.f;
+    const float sum = warp_sum(num);
+    w = mine >= 0 ? num / sum : 0.f;
+  } else if (a.score == BSHMEM_ROUTE_SOFTMAX) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) sum += l[i] > -CUDART_INF_F ? expf(l[i] - top) : 0.f;
+    sum = warp_sum(sum);
+    if (mine >= 0) w = expf(to_f(row[mine]) - top) / sum;
+  } else if (mine >= 0) {
+    w = sigmoid(to_f(row[mine]));
+  }
+  if (nan && a.score == BSHMEM_ROUTE_SOFTMAX && mine >= 0) w = CUDART_NAN_F;  // the sum over all experts is NaN
+  if (lane < K) {
+    a.idx[t * K + lane] = mine;
+    a.weight[t * K + lane] = w * a.scale;
+  }
+}
+
+// Gradient of the weights.  With w the weights before `scale`, over the chosen experts k:
+//   renormalised    dl_k = scale w_k (dw_k - sum_j dw_j w_j), for sigmoids times (1 - s_k); zero elsewhere
+//   softmax         dl_e = scale p_e ([e chosen] dw_e - sum_j dw_j p_j)
+//   sigmoid         dl_k = scale dw_k s_k (1 - s_k); zero elsewhere
+template <typename T, int VPL>
+__global__ void __launch_bounds__(THREADS) route_backward_kernel(const __grid_constant__ Params p) {
+  const bshmem_route_args_t& a = p.a;
+  const int lane = threadIdx.x & 31, K = a.K, E = a.E;
+  const long t = (long)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  T* out = (T*)a.dlogits + t * E;
+  const T* row = (const T*)a.logits + t * a.stride;
+  const int mine = lane < K ? a.idx[t * K + lane] : -1;
+  const float dw = mine >= 0 ? a.dweight[t * K + lane] : 0.f;
+  const float lm = mine >= 0 ? to_f(row[mine]) : -CUDART_INF_F;
+  const float poison = mine >= 0 ? 0.f * a.weight[t * K + lane] : 0.f;  // NaN where the forward's weight was
+  float d = 0.f;
+  if (!a.renormalize && a.score == BSHMEM_ROUTE_SOFTMAX) {
+    float l[VPL], top = -CUDART_INF_F, sum = 0.f;
+    load_row(l, row, E, lane);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
+    top = warp_max(top);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      l[i] = l[i] > -CUDART_INF_F ? expf(l[i] - top) : 0.f;
+      sum += l[i];
+    }
+    sum = warp_sum(sum);
+    const float pm = mine >= 0 ? expf(lm - top) / sum + poison : 0.f;
+    const float g = warp_sum(dw * pm);
+    const bool any = __any_sync(0xffffffffu, mine >= 0);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (lane + 32 * i < E) put(out + lane + 32 * i, any ? -a.scale * (l[i] / sum) * g : 0.f);
+    d = a.scale * pm * (dw - g);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (lane + 32 * i < E) put(out + lane + 32 * i, 0.f);
+    if (a.renormalize) {
+      const float set_top = warp_max(lm);
+      const float num = mine >= 0 ? numerator(lm, set_top, a.score) : 0.f;
+      const float sum = warp_sum(num);
+      const float w = mine >= 0 ? num / sum + poison : 0.f;
+      d = a.scale * w * (dw - warp_sum(dw * w));
+      if (a.score == BSHMEM_ROUTE_SIGMOID) d *= sigmoid(-lm);
+    } else {
+      d = a.scale * dw * sigmoid(lm) * sigmoid(-lm);
+    }
+  }
+  __syncwarp();  // the row's other values are written; the chosen ones replace theirs
+  if (mine >= 0) put(out + mine, d);
+}
+
+// Probabilities of the balance loss for this lane's experts, in place of the logits; all zero for a row of -inf.  s1[i] is the
+// derivative's factor 1 - sigmoid(l).
+template <int VPL, bool SLOPE>
+__device__ __forceinline__ void probabilities(float (&l)[VPL], float (&slope)[SLOPE ? VPL : 1], int score) {
+  float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) top = fmaxf(top, l[i]);
+  top = warp_max(top);
+  if (top == -CUDART_INF_F) top = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    if constexpr (SLOPE) slope[i] = score == BSHMEM_ROUTE_SIGMOID ? sigmoid(-l[i]) : 1.f;
+    l[i] = numerator(l[i], top, score);
+    sum += l[i];
+  }
+  sum = warp_sum(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) l[i] *= inv;
+}
+
+// Each CTA's sums of the probabilities and counts over its tokens: [grid][E] floats, [grid][E] counts, [grid] valid tokens.
+struct Workspace {
+  float* p;
+  int* counts;
+  int* n;
+};
+__host__ __device__ __forceinline__ Workspace workspace(void* base, int grid, int E) {
+  Workspace w;
+  w.p = (float*)base;
+  w.counts = (int*)(w.p + (size_t)grid * E);
+  w.n = w.counts + (size_t)grid * E;
+  return w;
+}
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(THREADS) balance_kernel(const __grid_constant__ Params p) {
+  const bshmem_route_args_t& a = p.a;
+  __shared__ int s_count[32 * VPL];
+  __shared__ float s_p[WARPS][32 * VPL];
+  __shared__ int s_n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K, E = a.E;
+  for (int e = threadIdx.x; e < 32 * VPL; e += THREADS) s_count[e] = 0;
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  float acc[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+  int n = 0;
+  for (long t = (long)blockIdx.x * WARPS + warp; t < a.T; t += (long)gridDim.x * WARPS) {
+    if (a.valid && !a.valid[t]) continue;
+    ++n;
+    float l[VPL], unused[1];
+    load_row(l, (const T*)a.logits + t * a.stride, E, lane);
+    if (lane < K) {
+      const int e = a.idx[t * K + lane];
+      if (e >= 0 && e < E) atomicAdd(&s_count[e], 1);
+    }
+    probabilities<VPL, false>(l, unused, a.score);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) acc[i] += l[i];
+  }
+  if (lane == 0 && n) atomicAdd(&s_n, n);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) s_p[warp][lane + 32 * i] = acc[i];
+  __syncthreads();
+  const Workspace w = workspace(a.workspace, gridDim.x, E);
+  for (int e = threadIdx.x; e < E; e += THREADS) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) s += s_p[k][e];
+    w.p[(size_t)blockIdx.x * E + e] = s;
+    w.counts[(size_t)blockIdx.x * E + e] = s_count[e];
+  }
+  if (threadIdx.x == 0) w.n[blockIdx.x] = s_n;
+}
+
+// Adds the CTAs' sums in order and forms the loss.  One CTA of 1024 threads.
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const __grid_constant__ Params p, int parts) {
+  const bshmem_route_args_t& a = p.a;
+  __shared__ int s_n;
+  __shared__ float s_loss[32];
+  __shared__ float s_p[1024];
+  __shared__ int s_c[1024];
+  const Workspace w = workspace(a.workspace, parts, a.E);
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  int n = 0;
+  for (int k = threadIdx.x; k < parts; k += blockDim.x) n += w.n[k];
+  if (n) atomicAdd(&s_n, n);
+  // `lanes` threads of a column each add a part of the CTAs
+  int cols = 32;
+  while (cols < a.E) cols *= 2;
+  const int slices = 1024 / cols, e = threadIdx.x % cols, slice = threadIdx.x / cols;
+  float ps = 0.f;
+  int cs = 0;
+  if (e < a.E)
+    for (int k = slice; k < parts; k += slices) {
+      ps += w.p[(size_t)k * a.E + e];
+      cs += w.counts[(size_t)k * a.E + e];
+    }
+  s_p[threadIdx.x] = ps;
+  s_c[threadIdx.x] = cs;
+  __syncthreads();
+  float term = 0.f;
+  if (slice == 0 && e < a.E) {
+    for (int k = 1; k < slices; ++k) {
+      ps += s_p[k * cols + e];
+      cs += s_c[k * cols + e];
+    }
+    const double nn = s_n > 0 ? (double)s_n : 1.0;
+    const float coef = (float)((double)a.E * cs / (a.K * nn * nn));
+    a.counts[e] = cs;
+    if (a.coef) a.coef[e] = coef;
+    term = coef * ps;
+  }
+  term = warp_sum(term);
+  if ((threadIdx.x & 31) == 0) s_loss[threadIdx.x >> 5] = term;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    term = warp_sum(s_loss[threadIdx.x]);
+    if (threadIdx.x == 0) *a.loss = term;
+  }
+}
+
+// dl_e = dloss p_e (coef_e - sum_j p_j coef_j), for sigmoids times (1 - s_e).
+template <typename T, int VPL>
+__global__ void __launch_bounds__(THREADS) balance_backward_kernel(const __grid_constant__ Params p) {
+  const bshmem_route_args_t& a = p.a;
+  const int lane = threadIdx.x & 31, E = a.E;
+  const long t = (long)blockIdx.x * WARPS + (threadIdx.x >> 5);
+  if (t >= a.T) return;
+  T* out = (T*)a.dlogits + t * E;
+  if (a.valid && !a.valid[t]) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (lane + 32 * i < E) put(out + lane + 32 * i, 0.f);
+    return;
+  }
+  float l[VPL], slope[VPL], c[VPL];
+  load_row(l, (const T*)a.logits + t * a.stride, E, lane);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) c[i] = lane + 32 * i < E ? a.coef[lane + 32 * i] : 0.f;
+  const float dloss = *a.dloss;
+  probabilities<VPL, true>(l, slope, a.score);
+  float mean = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) mean += l[i] * c[i];
+  mean = warp_sum(mean);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+    if (lane + 32 * i < E) put(out + lane + 32 * i, dloss * (l[i] * (c[i] - mean)) * slope[i]);
+}
+
+static int check(const bshmem_route_args_t* a) {
+  if (!a) return BSHMEM_ROUTE_ERR_ARGS;
+  if (a->T < 0 || a->E < 1 || a->E > BSHMEM_ROUTE_MAX_EXPERTS || a->K < 1 || a->K > BSHMEM_ROUTE_MAX_TOPK || a->K > a->E) return BSHMEM_ROUTE_ERR_SHAPE;
+  if ((long)a->T * a->K > INT_MAX) return BSHMEM_ROUTE_ERR_SHAPE;
+  if (a->type < 0 || a->type > 2 || a->score < 0 || a->score > 1) return BSHMEM_ROUTE_ERR_ARGS;
+  return BSHMEM_ROUTE_OK;
+}
+
+static int balance_ctas(int T) {
+  int device = 0, sms = 0;
+  cudaGetDevice(&device);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  const int want = (T + WARPS - 1) / WARPS, most = sms > 0 ? sms : 1;
+  return want < 1 ? 1 : want < most ? want : most;
+}
+
+// Calls f<T, VPL> for the type and the number of experts.
+template <typename T, typename F>
+static int by_experts(int E, F&& f) {
+  if (E <= 32) return f.template operator()<T, 1>();
+  if (E <= 64) return f.template operator()<T, 2>();
+  if (E <= 128) return f.template operator()<T, 4>();
+  if (E <= 256) return f.template operator()<T, 8>();
+  if (E <= 512) return f.template operator()<T, 16>();
+  return f.template operator()<T, 32>();
+}
+template <typename F>
+static int dispatch(const bshmem_route_args_t* a, F&& f) {
+  if (a->type == BSHMEM_ROUTE_F32) return by_experts<float>(a->E, f);
+  if (a->type == BSHMEM_ROUTE_BF16) return by_experts<__nv_bfloat16>(a->E, f);
+  return by_experts<__half>(a->E, f);
+}
+static int launched() { return cudaGetLastError() == cudaSuccess ? BSHMEM_ROUTE_OK : BSHMEM_ROUTE_ERR_DRIVER; }
+
+struct Route {
+  const Params& p;
+  cudaStream_t stream;
+  template <typename T, int VPL>
+  int operator()() const {
+    const unsigned grid = ((unsigned)p.a.T + WARPS - 1) / WARPS;
+    if (p.a.bias) route_kernel<T, VPL, true><<<grid, THREADS, 0, stream>>>(p);
+    else route_kernel<T, VPL, false><<<grid, THREADS, 0, stream>>>(p);
+    return launched();
+  }
+};
+struct RouteBackward {
+  const Params& p;
+  cudaStream_t stream;
+  template <typename T, int VPL>
+  int operator()() const {
+    route_backward_kernel<T, VPL><<<((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, 0, stream>>>(p);
+    return launched();
+  }
+};
+struct Balance {
+  const Params& p;
+  cudaStream_t stream;
+  template <typename T, int VPL>
+  int operator()() const {
+    const int grid = balance_ctas(p.a.T);
+    balance_kernel<T, VPL><<<grid, THREADS, 0, stream>>>(p);
+    balance_finish_kernel<<<1, 1024, 0, stream>>>(p, grid);
+    return launched();
+  }
+};
+struct BalanceBackward {
+  const Params& p;
+  cudaStream_t stream;
+  template <typename T, int VPL>
+  int operator()() const {
+    balance_backward_kernel<T, VPL><<<((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, 0, stream>>>(p);
+    return launched();
+  }
+};
+
+}  // namespace routing
+}  // namespace bshmem
+
+using namespace bshmem::routing;
+
+extern "C" size_t bshmem_balance_workspace(int T, int E) {
+  const size_t grid = (size_t)balance_ctas(T);
+  return (grid * E * 2 + grid) * 4;
+}
+
+extern "C" int bshmem_route(const bshmem_route_args_t* a, cudaStream_t stream) {
+  const int st = check(a);
+  if (st || a->T == 0) return st;
+  if (!a->logits || !a->idx || !a->weight) return BSHMEM_ROUTE_ERR_ARGS;
+  const Params p = {*a};
+  return dispatch(a, Route{p, stream});
+}
+
+extern "C" int bshmem_route_backward(const bshmem_route_args_t* a, cudaStream_t stream) {
+  const int st = check(a);
+  if (st || a->T == 0) return st;
+  if (!a->logits || !a->idx || !a->weight || !a->dweight || !a->dlogits) return BSHMEM_ROUTE_ERR_ARGS;
+  const Params p = {*a};
+  return dispatch(a, RouteBackward{p, stream});
+}
+
+extern "C" int bshmem_balance(const bshmem_route_args_t* a, cudaStream_t stream) {
+  const int st = check(a);
+  if (st) return st;
+  if ((a->T && (!a->logits || !a->idx)) || !a->loss || !a->counts || !a->workspace) return BSHMEM_ROUTE_ERR_ARGS;
+  const Params p = {*a};
+  return dispatch(a, Balance{p, stream});
+}
+
+extern "C" int bshmem_balance_backward(const bshmem_route_args_t* a, cudaStream_t stream) {
+  const int st = check(a);
+  if (st || a->T == 0) return st;
+  if (!a->logits || !a->coef || !a->dloss || !a->dlogits) return BSHMEM_ROUTE_ERR_ARGS;
+  const Params p = {*a};
+  return dispatch(a, BalanceBackward{p, stream});
+}
