@@ -224,6 +224,33 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(mask) : "memory");
 }
 
+// ---------------------------------------------------------------- block-scaled 4-bit floats
+// Instruction descriptor, kind::mxf4: D fp32, A and B E2M1, both K-major, scales E8M0.
+// Bits: [4,6) which scale of a word B uses, [7,10) A format (1 = E2M1), [10,12) B format, [17,23) N>>3, 23 scale format
+// (1 = E8M0), [27,29) M>>7, [29,31) which scale of a word A uses.  An MMA takes 64 values of K and so two scales per row:
+// bytes 0 and 1 of the row's word in tensor memory (`which` = 0) or bytes 2 and 3 (2).
+__host__ __device__ constexpr uint32_t umma_idesc_mxf4(int m, int n, int which) {
+  return ((uint32_t)which << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)which << 29);
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+      : "memory");
+}
+// Source of a 32 x 16 byte copy into tensor memory: no swizzle, rows of 16 bytes, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_scales(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  return d;
+}
+// 512 bytes of shared memory -> 32 lanes x 4 columns, the same in each of the four lane quarters.  Later MMAs of the thread see it.
+__device__ __forceinline__ void umma_copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+
 // 32 lanes x 32 consecutive fp32 columns: thread i of the warp receives row
 // (lane quarter base + i), v[j] = column (col + j).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t* v) {

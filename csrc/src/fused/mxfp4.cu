@@ -1,0 +1,377 @@
+// Microscaled 4-bit floating point: quantisation, reading back, and the block-scaled product on tcgen05.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <atomic>
+
+#include "../../include/bshmem/mxfp4.h"
+#include "../../include/bshmem/tcgen05.cuh"
+#include "tensor_map.cuh"
+
+namespace bshmem {
+namespace mx {
+using namespace sm100;
+
+constexpr int BLOCK = 32;              // values per scale
+constexpr int SCALE_BLOCK = 512;       // bytes: 128 rows x 4 scales
+
+__host__ __device__ __forceinline__ int64_t k_blocks(int64_t K) { return (K + 255) / 256 * 2; }      // of 128 values, even
+__host__ __device__ __forceinline__ int64_t row_blocks(int64_t R) { return (R + 127) / 128; }
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float from_f(float, float v) { return v; }
+__device__ __forceinline__ __nv_bfloat16 from_f(__nv_bfloat16, float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ __half from_f(__half, float v) { return __float2half_rn(v); }
+
+// ------------------------------------------------------------------ quantisation
+// Sixteen lanes take 128 values of a row (one word of four scales), eight values per lane; the largest exponent of a block of 32 comes from
+// two shuffles over its four lanes.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
+// Bound by memory: 2 or 4 bytes read and 17/32 written per value.
+constexpr int Q_THREADS = 256;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t stride, uint8_t* __restrict__ data,
+                                                             uint8_t* __restrict__ scales) {
+  const int64_t KB = k_blocks(K), tasks = row_blocks(R) * 128 * KB;
+  const int part = threadIdx.x & 15;
+  const int64_t step = (int64_t)gridDim.x * (Q_THREADS / 16);
+  // the bound is that of the warp's first half, so that both halves take part in the shuffles
+  for (int64_t first = (int64_t)blockIdx.x * (Q_THREADS / 16) + (threadIdx.x >> 5) * 2; first < tasks; first += step) {
+    const int64_t task = first + ((threadIdx.x >> 4) & 1);
+    const int64_t row = task / KB, kb = task % KB, col = kb * 128 + part * 8;
+    const bool live = task < tasks && row < R && col < K;
+    float f[8];
+    if (live) {
+      const T* src = x + row * stride + col;
+      if constexpr (VEC) {
+        alignas(16) T raw[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(raw) / 16; ++i) ((uint4*)raw)[i] = ((const uint4*)src)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(raw[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(src[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    }
+    uint32_t amax = 0;  // of the magnitudes' bits, which order like the magnitudes; a NaN is above infinity
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7fffffffu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
+    const uint32_t code = biased == 255 ? 255 : biased > 2 ? biased - 2 : 0;
+    const float inv = __uint_as_float((254u - (code == 255 ? 254u : code)) << 23);  // 2^(127 - code)
+    uint32_t packed = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      packed |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * i);
+    // the four scales of the sixteen lanes as one word
+    uint32_t word = code << (8 * (part >> 2));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if (live) *(uint32_t*)(data + row * (K / 2) + col / 2) = packed;
+    if (part == 0 && task < tasks) *(uint32_t*)(scales + ((row / 128) * KB + kb) * SCALE_BLOCK + (row % 32) * 16 + (row % 128 / 32) * 4) = word;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, int64_t R, int64_t K, T* __restrict__ out) {
+  const int64_t KB = k_blocks(K), per_row = K / 8, n = R * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * Q_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * Q_THREADS) {
+    const int64_t row = i / per_row, col = i % per_row * 8;
+    const uint32_t packed = *(const uint32_t*)(data + row * (K / 2) + col / 2);
+    const uint32_t code = scales[((row / 128) * KB + col / 128) * SCALE_BLOCK + (row % 32) * 16 + (row % 128 / 32) * 4 + col % 128 / BLOCK];
+    const float scale = __uint_as_float(code == 255 ? 0x7fffffffu : code ? code << 23 : 0x00400000u);
+    alignas(16) T raw[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t q = packed >> (4 * j) & 15, m = q & 7;
+      // E2M1: 0, 0.5, then 1 + m/2 times a power of two
+      const float mag = m < 2 ? 0.5f * (float)m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1) << 22);
+      raw[j] = from_f(T(), (q & 8 ? -mag : mag) * scale);
+    }
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(raw) / 16; ++j) ((uint4*)(out + row * K + col))[j] = ((uint4*)raw)[j];
+  }
+}
+
+// ------------------------------------------------------------------ product
+// One tile of 128 rows of the first operand by COLS rows of the second per CTA, over all of K in steps of 256 values (128 bytes).  The
+// scales of a step (1 KB per 128 rows) come with the operands' bytes into the same stage and are copied from there to tensor memory
+// by the thread that issues the MMAs, each stage to columns of its own: they are written again only after the stage's MMAs are done.
+// SWAP: the first operand is the weights (few rows of x).
+//   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
+constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128, G_RING = 208 * 1024;
+constexpr int G_SMEM = G_RING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+
+struct alignas(64) GemmParams {
+  CUtensorMap tmA, tmB;
+  const uint8_t *sa, *sb;   // scales of the two operands
+  __nv_bfloat16* out;
+  int* error_flag;
+  uint64_t wait_limit_ns;
+  int64_t rows_a, rows_b;   // rows of the operands
+  int64_t ld;               // of the output
+  int K, kb;                // kb: blocks of scales per row block
+  int tiles_a;
+};
+
+template <int COLS, bool SWAP>
+__global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  constexpr int B_BYTES = COLS * 128, SB_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + SB_BLOCKS * 1024;
+  constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, STAGES = G_RING / STAGE < 6 ? G_RING / STAGE : 6;
+  constexpr int S_COLS = 2 * 4 + 2 * 4 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
+  constexpr int TMEM = COLS + STAGES * S_COLS <= 128 ? 128 : COLS + STAGES * S_COLS <= 256 ? 256 : 512;
+  static_assert(COLS + STAGES * S_COLS <= 512, "tensor memory");
+  constexpr int PITCH = SWAP ? COLS + 1 : COLS + 4;
+  static_assert(128 * PITCH * 4 <= G_RING, "the finished tile reuses the ring");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * G_STAGE_A;
+  uint8_t* sS = sB + STAGES * B_BYTES;               // per stage: 1 KB of A's scales, then B's
+  uint64_t* full = (uint64_t*)(smem + G_RING);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t ta = blockIdx.x % p.tiles_a, tb = blockIdx.x / p.tiles_a;
+  const int64_t row_a = ta * 128, row_b = tb * COLS;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const int steps = (p.K + 255) / 256;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&p.tmA);
+      tma_prefetch_desc(&p.tmB);
+      const uint8_t* sa = p.sa + (row_a / 128) * p.kb * SCALE_BLOCK;
+      const uint8_t* sb = p.sb + (row_b / 128) * p.kb * SCALE_BLOCK;
+      // the second half of a 256-row tile may lie past the scales' last row block
+      const int sb_blocks = SB_BLOCKS == 2 && row_b + 128 < p.rows_b ? 2 : 1;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int k = 0; k < steps; ++k) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
+        uint8_t* s = sS + stage * S_BYTES;
+        mbar_expect_tx(&full[stage], G_STAGE_A + B_BYTES + 1024 + sb_blocks * 1024);
+        tma_load_2d(sA + stage * G_STAGE_A, &p.tmA, &full[stage], k * 64, (int)row_a);
+        tma_load_2d(sB + stage * B_BYTES, &p.tmB, &full[stage], k * 64, (int)row_b);
+        bulk_load(s, sa + (size_t)k * 1024, 1024, &full[stage]);
+        for (int b = 0; b < sb_blocks; ++b) bulk_load(s + 1024 + b * 1024, sb + ((size_t)b * p.kb + 2 * k) * SCALE_BLOCK, 1024, &full[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc[2] = {umma_idesc_mxf4(128, COLS, 0), umma_idesc_mxf4(128, COLS, 2)};
+      const uint32_t sfb_first = (uint32_t)(row_b % 128 / 32);  // rows of a narrow tile start inside a row block
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int k = 0; k < steps; ++k) {
+        if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) break;
+        tc_fence_after_sync();
+        const uint32_t sf = tmem + COLS + stage * S_COLS;  // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows
+        const uint32_t s = smem_u32(sS + stage * S_BYTES);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          umma_copy_scales(sf + h * 4, umma_desc_scales(s + h * SCALE_BLOCK));
+#pragma unroll
+          for (int b = 0; b < SB_BLOCKS; ++b) umma_copy_scales(sf + 8 + (h * SB_BLOCKS + b) * 4, umma_desc_scales(s + 1024 + b * 1024 + h * SCALE_BLOCK));
+        }
+        const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * G_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * B_BYTES));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
+          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, (k | i) != 0);
+        umma_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(acc_full);
+    }
+  }
+  __syncwarp();
+  // Every MMA of this CTA is complete, so every load has been consumed and the ring is free for the finished tile.
+  const bool ok = mbar_wait(acc_full, 0, p.wait_limit_ns, abort_flag) && !*abort_flag;
+  if (!ok) {
+    const uint64_t t0 = timer_ns();  // copies still in flight land before the shared memory is reused or goes away
+    while (timer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  tc_fence_after_sync();
+  float* tile = (float*)smem;  // [128][PITCH]
+  {
+    constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
+    const int c0 = (warp >> 2) * HALF;
+    float* mine = tile + ((warp & 3) * 32 + lane) * PITCH;
+    if (c0 < COLS) {
+#pragma unroll
+      for (int c = c0; c < c0 + HALF; c += 32) {
+        float f[32];
+        tmem_ld_32x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, (uint32_t*)f);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mine[c + j] = f[j];
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, TMEM);
+  if (SWAP) {
+    // row r of the tile is output column row_a + r, column c output row row_b + c
+    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
+      const int r = i & 127, c = i >> 7;
+      if (row_b + c < p.rows_b && row_a + r < p.rows_a) p.out[(row_b + c) * p.ld + row_a + r] = __float2bfloat16_rn(tile[r * PITCH + c]);
+    }
+  } else {
+    const bool vec = p.ld % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
+    for (int i = threadIdx.x; i < 128 * (COLS / 4); i += G_THREADS) {
+      const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+      if (row_a + r >= p.rows_a || row_b + c >= p.rows_b) continue;
+      const float* f = tile + r * PITCH + c;
+      __nv_bfloat16* dst = p.out + (row_a + r) * p.ld + row_b + c;
+      if (vec) {
+        uint2 o;
+        ((__nv_bfloat162*)&o)[0] = __floats2bfloat162_rn(f[0], f[1]);
+        ((__nv_bfloat162*)&o)[1] = __floats2bfloat162_rn(f[2], f[3]);
+        *(uint2*)dst = o;
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (row_b + c + j < p.rows_b) dst[j] = __float2bfloat16_rn(f[j]);
+      }
+    }
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
+}
+
+static int sm_count() {
+  int device = 0, sms = 0;
+  cudaGetDevice(&device);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  return sms > 0 ? sms : 1;
+}
+static int launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return BSHMEM_MX_OK;
+  fprintf(stderr, "%s: launch failed: %s\n", what, cudaGetErrorString(e));
+  return BSHMEM_MX_ERR_DRIVER;
+}
+
+template <typename T>
+static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
+  const int64_t tasks = row_blocks(R) * 128 * k_blocks(K), want = (tasks + Q_THREADS / 16 - 1) / (Q_THREADS / 16), most = (int64_t)sm_count() * 16;
+  const int grid = (int)(want < most ? want : most);
+  const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
+  if (vec) quantize_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
+  else quantize_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
+  return launched("bshmem_mxfp4_quantize");
+}
+template <typename T>
+static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
+  const int64_t want = (R * (K / 8) + Q_THREADS - 1) / Q_THREADS, most = (int64_t)sm_count() * 16;
+  dequantize_kernel<T><<<(int)(want < most ? want : most), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, K, (T*)out);
+  return launched("bshmem_mxfp4_dequantize");
+}
+
+template <int COLS, bool SWAP>
+static int launch_gemm(GemmParams& p, const void* a, const void* b, cudaStream_t stream) {
+  int st = make_map(&p.tmA, a, (uint64_t)p.rows_a, (uint64_t)p.K / 4, 128);  // bytes, in pairs: the box is 128 rows by 128 bytes
+  if (!st) st = make_map(&p.tmB, b, (uint64_t)p.rows_b, (uint64_t)p.K / 4, COLS);
+  if (st) return st == BSHMEM_FUSED_ERR_ALIGNMENT ? BSHMEM_MX_ERR_ALIGNMENT : BSHMEM_MX_ERR_DRIVER;
+  p.tiles_a = (int)((p.rows_a + 127) / 128);
+  const int64_t tiles = (int64_t)p.tiles_a * ((p.rows_b + COLS - 1) / COLS);
+  if (tiles > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
+  static std::atomic<uint64_t> ready;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return BSHMEM_MX_ERR_DRIVER;
+  if (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1)) {
+    if (cudaFuncSetAttribute((const void*)gemm_kernel<COLS, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, G_SMEM) != cudaSuccess) return BSHMEM_MX_ERR_DRIVER;
+    if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
+  }
+  gemm_kernel<COLS, SWAP><<<(int)tiles, G_THREADS, G_SMEM, stream>>>(p);
+  return launched("bshmem_mxfp4_gemm");
+}
+
+}  // namespace mx
+}  // namespace bshmem
+
+using namespace bshmem;
+using namespace bshmem::mx;
+
+extern "C" size_t bshmem_mxfp4_scale_bytes(int64_t R, int64_t K) { return R > 0 && K > 0 ? (size_t)(row_blocks(R) * k_blocks(K)) * SCALE_BLOCK : 0; }
+
+static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 0x7fffff00ll ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
+
+extern "C" int bshmem_mxfp4_quantize(const void* x, int type, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
+  const int st = check_matrix(R, K);
+  if (st || R == 0) return st;
+  if (!x || !data || !scales) return BSHMEM_MX_ERR_ARGS;
+  if (((uintptr_t)data | (uintptr_t)scales) & 15) return BSHMEM_MX_ERR_ALIGNMENT;
+  if (type == BSHMEM_MX_BF16) return launch_quantize<__nv_bfloat16>(x, R, K, stride, data, scales, stream);
+  if (type == BSHMEM_MX_F16) return launch_quantize<__half>(x, R, K, stride, data, scales, stream);
+  if (type == BSHMEM_MX_F32) return launch_quantize<float>(x, R, K, stride, data, scales, stream);
+  return BSHMEM_MX_ERR_ARGS;
+}
+
+extern "C" int bshmem_mxfp4_dequantize(const void* data, const void* scales, int64_t R, int64_t K, int type, void* out, cudaStream_t stream) {
+  const int st = check_matrix(R, K);
+  if (st || R == 0) return st;
+  if (!data || !scales || !out) return BSHMEM_MX_ERR_ARGS;
+  if (((uintptr_t)data | (uintptr_t)scales | (uintptr_t)out) & 15) return BSHMEM_MX_ERR_ALIGNMENT;
+  if (type == BSHMEM_MX_BF16) return launch_dequantize<__nv_bfloat16>(data, scales, R, K, out, stream);
+  if (type == BSHMEM_MX_F16) return launch_dequantize<__half>(data, scales, R, K, out, stream);
+  if (type == BSHMEM_MX_F32) return launch_dequantize<float>(data, scales, R, K, out, stream);
+  return BSHMEM_MX_ERR_ARGS;
+}
+
+extern "C" int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* a, cudaStream_t stream) {
+  if (!a) return BSHMEM_MX_ERR_ARGS;
+  const int st = check_matrix(a->M, a->K) | check_matrix(a->N, a->K);
+  if (st || a->M == 0 || a->N == 0) return st ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK;
+  if (!a->x || !a->x_scales || !a->w || !a->w_scales || !a->out || !a->error_flag) return BSHMEM_MX_ERR_ARGS;
+  if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales) & 15) return BSHMEM_MX_ERR_ALIGNMENT;
+  GemmParams p;
+  memset(&p, 0, sizeof(p));
+  const bool swap = a->M <= 128;
+  p.sa = (const uint8_t*)(swap ? a->w_scales : a->x_scales);
+  p.sb = (const uint8_t*)(swap ? a->x_scales : a->w_scales);
+  p.out = (__nv_bfloat16*)a->out;
+  p.error_flag = a->error_flag;
+  p.wait_limit_ns = a->wait_limit_ms ? (uint64_t)a->wait_limit_ms * 1000000ull : 10000000000ull;
+  p.rows_a = swap ? a->N : a->M;
+  p.rows_b = swap ? a->M : a->N;
+  p.ld = a->N;
+  p.K = (int)a->K;
+  p.kb = (int)k_blocks(a->K);
+  if (!swap) return launch_gemm<256, false>(p, a->x, a->w, stream);
+  if (a->M <= 32) return launch_gemm<32, true>(p, a->w, a->x, stream);
+  if (a->M <= 64) return launch_gemm<64, true>(p, a->w, a->x, stream);
+  return launch_gemm<128, true>(p, a->w, a->x, stream);
+}

@@ -1,0 +1,152 @@
+"""Microscaled 4-bit floating point, on the framework's own kernels (``libbshmem_fused.so``).
+
+* :func:`quantize_mxfp4` – a matrix ``[R, K]`` as E2M1 values with one power-of-two scale per 32 of them along K (17/32 of a byte a value).
+* :meth:`MxFp4.dequantize` – the values back.
+* :func:`gemm_mxfp4` – ``x @ w.T`` of two such matrices on the tensor cores' block-scaled form, accumulated in fp32; a bf16,
+  fp16 or fp32 ``x`` is quantised in the call.
+
+For serving: weights are quantised once, activations in every call.  K is a multiple of 32; rows and columns of the product may be
+any number.  Work is issued on the current stream; all tensors lie on the current device.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ..bindings import host as H
+from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
+
+BLOCK = 32
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
+
+
+class _GemmArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("w", C.c_void_p), ("w_scales", C.c_void_p), ("out", C.c_void_p), ("M", C.c_int64), ("N", C.c_int64),
+                ("K", C.c_int64), ("wait_limit_ms", C.c_uint32), ("error_flag", C.c_void_p)]
+
+
+def _lib():
+    lib = fused_lib()
+    if not hasattr(lib, "_mxfp4_ready"):
+        lib.bshmem_mxfp4_scale_bytes.restype, lib.bshmem_mxfp4_scale_bytes.argtypes = C.c_size_t, [C.c_int64, C.c_int64]
+        lib.bshmem_mxfp4_quantize.restype = C.c_int
+        lib.bshmem_mxfp4_quantize.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]
+        lib.bshmem_mxfp4_dequantize.restype = C.c_int
+        lib.bshmem_mxfp4_dequantize.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_void_p]
+        lib.bshmem_mxfp4_gemm.restype, lib.bshmem_mxfp4_gemm.argtypes = C.c_int, [C.POINTER(_GemmArgs), C.c_void_p]
+        lib._mxfp4_ready = True
+    return lib
+
+
+def _raise(st: int, name: str) -> None:
+    if st != 0:
+        raise FusedGemmError(f"{name}: {_ERRORS.get(st, st)}")
+
+
+def _check_device(*tensors) -> None:
+    for t in tensors:
+        if not t.is_cuda:
+            raise FusedGemmError("tensors must be on the GPU")
+        if t.get_device() != torch.cuda.current_device():
+            raise FusedGemmError("tensors must be on the current device")
+
+
+def _scale_shape(R: int, K: int) -> tuple[int, int, int]:
+    return (R + 127) // 128, (K + 255) // 256 * 2, 512
+
+
+class MxFp4:
+    """A matrix ``[R, K]`` in microscaled 4-bit floats.
+
+    ``data``: uint8 ``[R, K / 2]``, two values a byte, the lower K in the low four bits.  ``scales``: uint8 ``[R / 128, K / 128, 512]`` (both
+    rounded up, the second to an even number): E8M0 scales in the order of the tensor core's scale operand, row r and scale s of a block
+    at ``(r % 32) * 16 + (r / 32) * 4 + s``; zero for rows and columns past the end.
+    """
+    __slots__ = ("data", "scales", "shape")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int]):
+        R, K = shape
+        if K < BLOCK or K % BLOCK:
+            raise FusedGemmError(f"K must be a multiple of {BLOCK}, not {K}")
+        for name, t, want in (("data", data, (R, K // 2)), ("scales", scales, _scale_shape(R, K))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+                raise FusedGemmError(f"{name} must be a contiguous uint8 tensor of shape {want}")
+        self.data, self.scales, self.shape = data, scales, (R, K)
+
+    @classmethod
+    def from_codes(cls, data: torch.Tensor, codes: torch.Tensor) -> "MxFp4":
+        """From packed values ``[R, K / 2]`` and E8M0 scales ``[R, K / 32]`` (both uint8), the order that checkpoints use."""
+        if codes.dim() != 2 or data.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[0] != data.shape[0] or codes.shape[1] * 16 != data.shape[1]:
+            raise FusedGemmError(f"data {tuple(data.shape)} and codes {tuple(codes.shape)} {codes.dtype} do not belong together")
+        R, S = codes.shape
+        rb, kb, _ = _scale_shape(R, S * BLOCK)
+        padded = torch.zeros(rb * 128, kb * 4, dtype=torch.uint8, device=codes.device)
+        padded[:R, :S] = codes
+        scales = padded.view(rb, 4, 32, kb, 4).permute(0, 3, 2, 1, 4).reshape(rb, kb, 512).contiguous()
+        return cls(data.contiguous(), scales, (R, S * BLOCK))
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """E8M0 scales by row and block, uint8 ``[R, K / 32]``: scale ``2 ** (code - 127)``, 255 for NaN."""
+        R, K = self.shape
+        rb, kb, _ = self.scales.shape
+        return self.scales.view(rb, kb, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rb * 128, kb * 4)[:R, :K // BLOCK].contiguous()
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values, ``[R, K]``.  Exact in bf16 and fp32; fp16 rounds where its range ends."""
+        if dtype not in _TYPES:
+            raise FusedGemmError("dtype must be bfloat16, float16 or float32")
+        _check_device(self.data, self.scales)
+        R, K = self.shape
+        out = torch.empty(R, K, dtype=dtype, device=self.data.device)
+        _raise(_lib().bshmem_mxfp4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), R, K, _TYPES[dtype], out.data_ptr(), H.current_stream_handle()),
+               "bshmem_mxfp4_dequantize")
+        return out
+
+
+def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
+    """``x [R, K]`` (bf16, fp16 or fp32; rows may lie apart) in microscaled 4-bit floats.
+
+    A block of 32 values along K gets the scale ``2 ** (floor(log2(max|x|)) - 2)``, at least ``2 ** -127``; its values are ``x / scale``
+    rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to even) and saturated at 6.  A block with an infinity or a
+    NaN gets the scale NaN, and so do all its values."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _TYPES:
+        raise FusedGemmError("x must be a [R, K] tensor of bfloat16, float16 or float32")
+    R, K = x.shape
+    if K < BLOCK or K % BLOCK:
+        raise FusedGemmError(f"K must be a multiple of {BLOCK}, not {K}")
+    _check_device(x)
+    x = x.detach()
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    data = torch.empty(R, K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_shape(R, K), dtype=torch.uint8, device=x.device)
+    _raise(_lib().bshmem_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], R, K, x.stride(0), data.data_ptr(), scales.data_ptr(), H.current_stream_handle()),
+           "bshmem_mxfp4_quantize")
+    return MxFp4(data, scales, (R, K))
+
+
+def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x[M, K] @ w[N, K].T`` -> bf16 ``[M, N]`` on the block-scaled tensor-core path, accumulated in fp32 and rounded once.  An
+    ``x`` that is not quantised yet is quantised in the call (:func:`quantize_mxfp4`).  M and N may be any number."""
+    if not isinstance(w, MxFp4):
+        raise FusedGemmError("w must be quantised (quantize_mxfp4)")
+    if not isinstance(x, MxFp4):
+        x = quantize_mxfp4(x)
+    if x.shape[1] != w.shape[1]:
+        raise FusedGemmError(f"shape mismatch: x {x.shape} w {w.shape}")
+    _check_device(x.data, x.scales, w.data, w.scales)
+    M, N = x.shape[0], w.shape[0]
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=w.data.device)
+    else:
+        _check_device(out)
+        _check_out(out, M, N)
+    a = _GemmArgs()
+    a.x, a.x_scales, a.w, a.w_scales, a.out = x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr()
+    a.M, a.N, a.K = M, N, w.shape[1]
+    a.error_flag = _error_flag(out.device).data_ptr()
+    _raise(_lib().bshmem_mxfp4_gemm(C.byref(a), H.current_stream_handle()), "bshmem_mxfp4_gemm")
+    return out
