@@ -37,6 +37,7 @@ typedef struct {
   /* backward */
   const void *dr, *dy;
   void *dh, *dresidual, *dpost, *dpre, *dgate;
+  int* error_flag;  /* device int; set to 1 if a copy inside a kernel did not arrive in time */
   float* partials;  /* bshmem_block_norms_partials(T, H) floats, needed for dpost, dpre and the channel gate's gradient */
 } bshmem_norm_args_t;
 

@@ -16,7 +16,7 @@ import ctypes as C
 import torch
 
 from ..bindings import host as H
-from .fused_gemm import fused_lib
+from .fused_gemm import _error_flag, fused_lib
 
 MAX_H = 16384
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -34,7 +34,7 @@ class _Args(C.Structure):
                 ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("eps", C.c_float), ("weight_offset", C.c_float),
                 ("h", C.c_void_p), ("residual", C.c_void_p), ("post", C.c_void_p), ("pre", C.c_void_p), ("gate", C.c_void_p),
                 ("r", C.c_void_p), ("y", C.c_void_p), ("stat", C.c_void_p), ("dr", C.c_void_p), ("dy", C.c_void_p),
-                ("dh", C.c_void_p), ("dresidual", C.c_void_p), ("dpost", C.c_void_p), ("dpre", C.c_void_p), ("dgate", C.c_void_p), ("partials", C.c_void_p)]
+                ("dh", C.c_void_p), ("dresidual", C.c_void_p), ("dpost", C.c_void_p), ("dpre", C.c_void_p), ("dgate", C.c_void_p), ("error_flag", C.c_void_p), ("partials", C.c_void_p)]
 
 
 def _lib():
@@ -68,6 +68,7 @@ class _Plan:
         a.wt_type = a.type if wt is None else _TYPES[wt.dtype]
         a.residual_scale, a.branch_scale, a.eps, a.weight_offset = self.residual_scale, self.branch_scale, self.eps, self.weight_offset
         a.h, a.residual, a.post, a.pre, a.gate = _ptr(h), residual.data_ptr(), _ptr(post), _ptr(pre), _ptr(gate)
+        a.error_flag = _error_flag(residual.device).data_ptr()
         a.res_stride = residual.stride(0)
         if h is not None:
             a.h_stride = h.stride(0)
