@@ -313,21 +313,24 @@ __global__ void __launch_bounds__(MAX_THREADS) backward_kernel(const __grid_cons
 }
 
 // Sums of the CTAs' parts, in order: S (dpost and the channel gate's gradient) and dpre.
+constexpr int SLICES = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ Params p, int parts) {
+__global__ void __launch_bounds__(32 * SLICES) column_sum_kernel(const __grid_constant__ Params p, int parts) {
   const bshmem_norm_args_t& a = p.a;
   const int i = blockIdx.x * 32 + threadIdx.x;
   const bool pre = blockIdx.y != 0, channel = a.gate_mode == BSHMEM_NORM_GATE_CHANNEL, wide = a.wt_type == BSHMEM_NORM_F32 && sizeof(T) < 4;
   if (pre ? !a.dpre : !a.dpost && !(a.dgate && channel)) return;
-  __shared__ float s[8][32];
+  __shared__ float s[SLICES][33];
   float v = 0.f;
-  if (i < a.H)
-    for (int k = threadIdx.y; k < parts; k += 8) v += a.partials[((size_t)k * 2 + pre) * a.H + i];
+  if (i < a.H) {
+#pragma unroll 4
+    for (int k = threadIdx.y; k < parts; k += SLICES) v += a.partials[((size_t)k * 2 + pre) * a.H + i];
+  }
   s[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   if (threadIdx.y || i >= a.H) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) v += s[k][threadIdx.x];
+  for (int k = 1; k < SLICES; ++k) v += s[k][threadIdx.x];
   if (pre) {
     store1_wt<T>(a.dpre, wide, i, v);
     return;
@@ -336,26 +339,33 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
   if (a.dgate && channel) store1_wt<T>(a.dgate, wide, i, a.branch_scale * v * (a.post ? load1_wt<T>(a.post, wide, i) + a.weight_offset : 1.f));
 }
 
-// ------------------------------------------------------------------ many rows
-// The kernels above keep only the rows in flight that fit the registers.  With more rows than the SMs take at once, each CTA walks
-// rows instead: one warp copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of the other warps, each thread of
-// which owns sixteen columns for the whole run, with their parameters and their sums over rows in registers.
-constexpr int RING_CH = 4, RING_COLS = 4 * RING_CH, RING_MAX_H = 8192, RING_THREADS = RING_MAX_H / RING_COLS + 32, RING_MAX_STAGES = 8;
-constexpr int RING_SMEM = 216 * 1024;  // of an SM, shared by its CTAs
+// ------------------------------------------------------------------ rows of up to 8192
+// Every thread owns sixteen columns for the whole run, with their parameters and their sums over rows in registers; its CTA (or, up to 512
+// columns, its warp) walks rows with the stride of the grid.  512 threads of 128 registers take rows of 8192.
+//   STAGED  one thread copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that the bytes in
+//           flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which spill:
+//           backward at 4096 x 8192 took 269 us with it, 128 without.)
+//   VECTOR  rows are read where they lie, 8 or 16 bytes at a time: few rows, or rows too large for two stages
+//   SCALAR  the same one value at a time, for odd sizes and addresses
+enum Mode { STAGED, VECTOR, SCALAR };
+constexpr int ROW_CH = 4, ROW_COLS = 4 * ROW_CH, ROW_MAX_H = 8192, ROW_THREADS = ROW_MAX_H / ROW_COLS, MAX_STAGES = 8;
+constexpr int WARP_MAX_H = 32 * ROW_COLS, WARP_GROUPS = 8;   // rows of a warp each
+constexpr int STAGE_SMEM = 216 * 1024;  // of an SM, shared by its CTAs
 
-struct RingParams {
+struct RowParams {
   bshmem_norm_args_t a;
-  int stages, stage_bytes;
+  int threads;              // per row
+  int stages, stage_bytes;  // STAGED
 };
 
 // The rows that are copied, in the order of their places in a stage.
-struct RingRows {
+struct StageRows {
   int h, residual, dr, dy, gate;  // offsets; -1: absent
   int bytes;
 };
 __host__ __device__ __forceinline__ int type_bytes(int t) { return t == BSHMEM_NORM_F32 ? 4 : 2; }
-__host__ __device__ __forceinline__ RingRows ring_rows(const bshmem_norm_args_t& a, bool backward) {
-  RingRows r;
+__host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_t& a, bool backward) {
+  StageRows r;
   const int t = a.H * type_bytes(a.type), rt = a.H * type_bytes(a.res_type), wt = a.H * type_bytes(a.wt_type);
   int at = 0;
   auto place = [&](bool present, int bytes) {
@@ -372,342 +382,403 @@ __host__ __device__ __forceinline__ RingRows ring_rows(const bshmem_norm_args_t&
   return r;
 }
 
-struct Ring {
-  uint8_t* data;
-  uint64_t *full, *empty;
-  volatile int* abort_flag;
-  int stage;
-  uint32_t phase;
+// A row's inputs, wherever they are.
+struct RowSource {
+  const uint8_t *h, *residual, *dr, *dy, *gate;
 };
-constexpr uint64_t RING_WAIT_NS = 10000000000ull;  // the waits are for this CTA's own copies and threads
 
-__device__ __forceinline__ Ring ring_setup(const RingParams& p, uint8_t* smem, int consumer_warps) {
-  Ring r;
-  r.data = smem;
-  r.full = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
-  r.empty = r.full + RING_MAX_STAGES;
-  r.abort_flag = (volatile int*)(r.empty + RING_MAX_STAGES);
-  r.stage = 0;
-  r.phase = 0;
-  if (threadIdx.x == 0) {
-    *r.abort_flag = 0;
-    for (int i = 0; i < p.stages; ++i) {
-      sm100::mbar_init(&r.full[i], 1);
-      sm100::mbar_init(&r.empty[i], consumer_warps);
-    }
-    sm100::mbar_fence_init();
-    sm100::fence_proxy_async_smem();
+template <Mode MODE>
+struct Rows {
+  const RowParams& p;
+  uint8_t* data = nullptr;
+  uint64_t* full = nullptr;
+  volatile int* abort_flag = nullptr;
+  StageRows at;
+  int tid, threads, stage = 0;
+  uint32_t phase = 0;
+  size_t first, step;
+
+  static constexpr uint64_t WAIT_NS = 10000000000ull;  // the waits are for this CTA's own copies
+
+  // Starts the copy of a row into a stage that nobody reads any more.  One thread.
+  __device__ __forceinline__ void load(size_t row, int to) const {
+    const RowSource g = global(row);
+    const int ts = type_bytes(p.a.type), rs = type_bytes(p.a.res_type), ws = type_bytes(p.a.wt_type), H = p.a.H;
+    uint8_t* dst = data + (size_t)to * p.stage_bytes;
+    uint64_t* bar = &full[to];
+    sm100::mbar_expect_tx(bar, at.bytes);
+    sm100::bulk_load(dst + at.residual, g.residual, H * rs, bar);
+    if (at.h >= 0) sm100::bulk_load(dst + at.h, g.h, H * ts, bar);
+    if (at.dr >= 0) sm100::bulk_load(dst + at.dr, g.dr, H * rs, bar);
+    if (at.dy >= 0) sm100::bulk_load(dst + at.dy, g.dy, H * ts, bar);
+    if (at.gate >= 0) sm100::bulk_load(dst + at.gate, g.gate, H * ws, bar);
   }
-  __syncthreads();
-  return r;
-}
-__device__ __forceinline__ void ring_next(Ring& r, int stages) {
-  if (++r.stage == stages) {
-    r.stage = 0;
-    r.phase ^= 1;
-  }
-}
-// The copying warp: every row of this CTA, as stages become free.
-__device__ __forceinline__ void ring_fill(const RingParams& p, Ring& r, bool backward) {
-  const bshmem_norm_args_t& a = p.a;
-  if (sm100::elect_one()) {
-    const RingRows rows = ring_rows(a, backward);
+  __device__ __forceinline__ RowSource global(size_t row) const {
+    const bshmem_norm_args_t& a = p.a;
     const size_t ts = type_bytes(a.type), rs = type_bytes(a.res_type), ws = type_bytes(a.wt_type);
-    for (size_t row = blockIdx.x; row < (size_t)a.T; row += gridDim.x) {
-      if (!sm100::mbar_wait(&r.empty[r.stage], r.phase ^ 1, RING_WAIT_NS, r.abort_flag)) break;
-      uint8_t* dst = r.data + (size_t)r.stage * p.stage_bytes;
-      uint64_t* bar = &r.full[r.stage];
-      sm100::mbar_expect_tx(bar, rows.bytes);
-      sm100::bulk_load(dst + rows.residual, (const uint8_t*)a.residual + row * a.res_stride * rs, a.H * rs, bar);
-      if (rows.h >= 0) sm100::bulk_load(dst + rows.h, (const uint8_t*)a.h + row * a.h_stride * ts, a.H * ts, bar);
-      if (rows.dr >= 0) sm100::bulk_load(dst + rows.dr, (const uint8_t*)a.dr + row * a.dr_stride * rs, a.H * rs, bar);
-      if (rows.dy >= 0) sm100::bulk_load(dst + rows.dy, (const uint8_t*)a.dy + row * a.dy_stride * ts, a.H * ts, bar);
-      if (rows.gate >= 0) sm100::bulk_load(dst + rows.gate, (const uint8_t*)a.gate + row * a.gate_stride * ws, a.H * ws, bar);
-      ring_next(r, p.stages);
+    RowSource g;
+    g.residual = (const uint8_t*)a.residual + row * a.res_stride * rs;
+    g.h = (const uint8_t*)a.h + row * a.h_stride * ts;
+    g.dr = (const uint8_t*)a.dr + row * a.dr_stride * rs;
+    g.dy = (const uint8_t*)a.dy + row * a.dy_stride * ts;
+    g.gate = (const uint8_t*)a.gate + row * a.gate_stride * ws;
+    return g;
+  }
+  __device__ __forceinline__ Rows(const RowParams& params, uint8_t* smem, bool backward) : p(params), at(stage_rows(params.a, backward)) {
+    threads = p.threads;
+    const int groups = blockDim.x / threads;
+    tid = threadIdx.x % threads;
+    first = (size_t)blockIdx.x * groups + threadIdx.x / threads;
+    step = (size_t)gridDim.x * groups;
+    if constexpr (MODE == STAGED) {
+      data = smem;
+      full = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
+      abort_flag = (volatile int*)(full + MAX_STAGES);
+      if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int i = 0; i < p.stages; ++i) sm100::mbar_init(&full[i], 1);
+        sm100::mbar_fence_init();
+        sm100::fence_proxy_async_smem();
+        for (int i = 0; i < p.stages; ++i)
+          if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
+      }
+      __syncthreads();
     }
   }
-  __syncwarp();
-}
-__device__ __forceinline__ void ring_end(const RingParams& p, const Ring& r) {
-  __syncthreads();
-  if (!*r.abort_flag) return;
-  const uint64_t t0 = sm100::timer_ns();  // copies still in flight land before the shared memory goes away
-  while (sm100::timer_ns() - t0 < 200000) __nanosleep(1000);
-  if (threadIdx.x == 0) atomicOr(p.a.error_flag, 1);
-}
-
-// Sum over the consumer warps (at most 16), the same value in every thread.  `s` alternates between two buffers, so that one
-// barrier per sum is enough.
-template <int N>
-__device__ __forceinline__ void ring_sum(float (&v)[N], float (*s)[N], int warps) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  if (warps == 1) return;
-  if (lane == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[warp][i] = v[i];
-  sm100::named_bar_sync(1, warps * 32);
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lane < warps ? s[lane][i] : 0.f;
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
-}
-
-// Four neighbouring values: 8 or 16 bytes a thread, so that a warp's accesses to shared memory are free of bank conflicts for
-// both sizes of type, and few values are live at a time.
-template <typename T>
-__device__ __forceinline__ void load4(float* f, const T* row, int col, int H) {
-  alignas(16) T raw[4];
-  if constexpr (sizeof(T) == 4) *(uint4*)raw = col < H ? *(const uint4*)(row + col) : make_uint4(0u, 0u, 0u, 0u);
-  else *(uint2*)raw = col < H ? *(const uint2*)(row + col) : make_uint2(0u, 0u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = to_f<T>(raw[i]);
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* row, int col, int H, const float* f) {
-  if (col >= H) return;
-  alignas(16) T raw[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(f[i]);
-  if constexpr (sizeof(T) == 4) *(uint4*)(row + col) = *(uint4*)raw;
-  else *(uint2*)(row + col) = *(uint2*)raw;
-}
-template <typename T>
-__device__ __forceinline__ void load4_wt(float* f, const void* row, bool wide, int col, int H) {
-  if (wide) load4<float>(f, (const float*)row, col, H);
-  else load4<T>(f, (const T*)row, col, H);
-}
-
-// u = branch_scale (post + offset) gate, without the gate where it differs from row to row.
-template <typename T>
-__device__ __forceinline__ void load_u(float* u, const bshmem_norm_args_t& a, bool wide, int col) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = 1.f;
-  if (a.post) {
-    load4_wt<T>(u, a.post, wide, col, a.H);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] += a.weight_offset;
+  __device__ __forceinline__ RowSource wait(size_t row) const {
+    if constexpr (MODE == STAGED) {
+      sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
+      const uint8_t* s = data + (size_t)stage * p.stage_bytes;
+      return {s + at.h, s + at.residual, s + at.dr, s + at.dy, s + at.gate};
+    } else {
+      return global(row);
+    }
   }
-  if (a.gate_mode == BSHMEM_NORM_GATE_CHANNEL) {
-    float g[4];
-    load4_wt<T>(g, a.gate, wide, col, a.H);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] *= g[i];
+  // All threads are past their last look at the stage of `row` (`behind` = 0) or of the row before it (1): it takes the next row that
+  // falls to it.
+  __device__ __forceinline__ void refill(size_t row, int behind) const {
+    if constexpr (MODE == STAGED) {
+      const size_t next = row + (size_t)(p.stages - behind) * step;
+      if (threadIdx.x == 0 && row >= first + behind * step && next < (size_t)p.a.T) load(next, stage >= behind ? stage - behind : p.stages - 1);
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] *= a.branch_scale;
-}
-__device__ __forceinline__ int ring_col(int c, int threads) { return (c * threads + (int)threadIdx.x) * 4; }
+  __device__ __forceinline__ void next() {
+    if constexpr (MODE == STAGED) {
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  __device__ __forceinline__ void end() const {
+    if constexpr (MODE == STAGED) {
+      __syncthreads();
+      if (!*abort_flag) return;
+      const uint64_t t0 = sm100::timer_ns();  // copies still in flight land before the shared memory goes away
+      while (sm100::timer_ns() - t0 < 200000) __nanosleep(1000);
+      if (threadIdx.x == 0) atomicOr(p.a.error_flag, 1);
+    }
+  }
 
-// FULL: the gate is [T][H].
-template <typename T, typename R, bool FULL>
-__global__ void __launch_bounds__(RING_THREADS, 1) forward_ring_kernel(const __grid_constant__ RingParams p) {
+  // This thread's four columns of chunk c.  With vectors they are neighbours (8 or 16 bytes a thread: a warp's accesses to shared memory
+  // are free of bank conflicts for both sizes of type); without, they are a row's threads apart.
+  template <typename T>
+  __device__ __forceinline__ void load4(float* f, const void* row, int c) const {
+    if constexpr (MODE == SCALAR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = (c * 4 + i) * threads + tid;
+        f[i] = col < p.a.H ? to_f<T>(((const T*)row)[col]) : 0.f;
+      }
+    } else {
+      const int col = (c * threads + tid) * 4;
+      alignas(16) T raw[4];
+      if constexpr (sizeof(T) == 4) *(uint4*)raw = col < p.a.H ? *(const uint4*)((const T*)row + col) : make_uint4(0u, 0u, 0u, 0u);
+      else *(uint2*)raw = col < p.a.H ? *(const uint2*)((const T*)row + col) : make_uint2(0u, 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = to_f<T>(raw[i]);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store4(void* row, int c, const float* f) const {
+    if constexpr (MODE == SCALAR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int col = (c * 4 + i) * threads + tid;
+        if (col < p.a.H) ((T*)row)[col] = from_f<T>(f[i]);
+      }
+    } else {
+      const int col = (c * threads + tid) * 4;
+      if (col >= p.a.H) return;
+      alignas(16) T raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(f[i]);
+      if constexpr (sizeof(T) == 4) *(uint4*)((T*)row + col) = *(uint4*)raw;
+      else *(uint2*)((T*)row + col) = *(uint2*)raw;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void load4_wt(float* f, const void* row, bool wide, int c) const {
+    if (wide) load4<float>(f, row, c);
+    else load4<T>(f, row, c);
+  }
+  // u = branch_scale (post + offset) gate, without the gate where it differs from row to row.
+  template <typename T>
+  __device__ __forceinline__ void load_u(float* u, bool wide, int c) const {
+    const bshmem_norm_args_t& a = p.a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = 1.f;
+    if (a.post) {
+      load4_wt<T>(u, a.post, wide, c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] += a.weight_offset;
+    }
+    if (a.gate_mode == BSHMEM_NORM_GATE_CHANNEL) {
+      float g[4];
+      load4_wt<T>(g, a.gate, wide, c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] *= g[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] *= a.branch_scale;
+  }
+  // Sum over a row's threads, the same value in every one of them.  One barrier per sum: consecutive sums of a CTA use two
+  // buffers in turn.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N], float (*s)[N]) const {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (blockDim.x != threads) return;  // a warp's row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[warp][i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane < warps ? s[lane][i] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+  }
+  __device__ __forceinline__ void barrier() const {
+    if (blockDim.x == threads) __syncthreads();
+  }
+};
+
+// ALL: h, both norms, and a gate per channel or none, as compile-time facts; without it each part is looked up.
+template <typename T, typename R, Mode MODE, bool ALL>
+__global__ void __launch_bounds__(ROW_THREADS, 1) forward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][16][1];
-  const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5;
-  Ring ring = ring_setup(p, smem, warps);
-  if (warp == warps) {
-    ring_fill(p, ring, false);
-  } else {
-    const RingRows rows = ring_rows(a, false);
-    const bool wide = a.wt_type == BSHMEM_NORM_F32 && sizeof(T) < 4, token = a.gate_mode == BSHMEM_NORM_GATE_TOKEN;
-    float u[RING_CH][4], wp[RING_CH][4];
-    if (a.h) {
+  Rows<MODE> rows(p, smem, false);
+  const bool wide = a.wt_type == BSHMEM_NORM_F32 && sizeof(T) < 4;
+  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_y = ALL || a.y;
+  const float inv_h = 1.f / (float)a.H;
+  float u[ROW_CH][4], wp[ROW_CH][4];
 #pragma unroll
-      for (int c = 0; c < RING_CH; ++c) load_u<T>(u[c], a, wide, ring_col(c, threads));
-    }
-    if (a.y) {
+  for (int c = 0; c < ROW_CH; ++c) {
+    if (has_h) rows.template load_u<T>(u[c], wide, c);
+    if (has_y) {
+      rows.template load4_wt<T>(wp[c], a.pre, wide, c);
 #pragma unroll
-      for (int c = 0; c < RING_CH; ++c) {
-        load4_wt<T>(wp[c], a.pre, wide, ring_col(c, threads), a.H);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) wp[c][i] += a.weight_offset;
-      }
-    }
-    for (size_t row = blockIdx.x; row < (size_t)a.T; row += gridDim.x) {
-      const float tg = token ? load1_wt<T>(a.gate, wide, row) : 1.f;
-      sm100::mbar_wait(&ring.full[ring.stage], ring.phase, RING_WAIT_NS, ring.abort_flag);
-      const uint8_t* src = ring.data + (size_t)ring.stage * p.stage_bytes;
-      float r[RING_CH][4], ss[1];
-      if (a.h) {
-        float inv = 1.f;
-        ss[0] = 0.f;
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c) {
-          load4<T>(r[c], (const T*)(src + rows.h), ring_col(c, threads), a.H);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
-        }
-        if (a.post) {
-          ring_sum<1>(ss, sums[0], warps);
-          inv = rsqrtf(ss[0] / (float)a.H + a.eps);
-          if (threadIdx.x == 0 && a.stat) a.stat[row] = inv;
-        }
-        inv *= tg;
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c) {
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[c][i] *= inv * u[c][i];
-          if constexpr (FULL) {
-            load4_wt<T>(x, src + rows.gate, wide, ring_col(c, threads), a.H);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[c][i] *= x[i];
-          }
-          load4<R>(x, (const R*)(src + rows.residual), ring_col(c, threads), a.H);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[c][i] += a.residual_scale * x[i];
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c) {
-          load4<R>(r[c], (const R*)(src + rows.residual), ring_col(c, threads), a.H);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[c][i] *= a.residual_scale;
-        }
-      }
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) sm100::mbar_arrive(&ring.empty[ring.stage]);
-      ring_next(ring, p.stages);
-      if (a.r) {
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c) store4<R>((R*)a.r + row * a.H, ring_col(c, threads), a.H, r[c]);
-      }
-      if (a.y) {
-        ss[0] = 0.f;
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
-        ring_sum<1>(ss, sums[1], warps);
-        const float inv = rsqrtf(ss[0] / (float)a.H + a.eps);
-        if (threadIdx.x == 0 && a.stat) a.stat[a.T + row] = inv;
-#pragma unroll
-        for (int c = 0; c < RING_CH; ++c) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) r[c][i] *= inv * wp[c][i];
-          store4<T>((T*)a.y + row * a.H, ring_col(c, threads), a.H, r[c]);
-        }
-      }
-      // one of the two sums alone would write its buffer again before all have read it
-      if (!(a.h && a.post && a.y)) sm100::named_bar_sync(1, threads);
+      for (int i = 0; i < 4; ++i) wp[c][i] += a.weight_offset;
     }
   }
-  ring_end(p, ring);
+  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+    const float tg = token ? load1_wt<T>(a.gate, wide, row) : 1.f;
+    const RowSource src = rows.wait(row);
+    float r[ROW_CH][4], ss[1];
+    if (has_h) {
+      float inv = 1.f;
+      ss[0] = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template load4<T>(r[c], src.h, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
+      }
+      if (has_post) {
+        rows.sum(ss, sums[0]);
+        inv = rsqrtf(ss[0] * inv_h + a.eps);
+        if (rows.tid == 0 && a.stat) a.stat[row] = inv;
+      }
+      inv *= tg;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= inv * u[c][i];
+        if (full) {
+          rows.template load4_wt<T>(x, src.gate, wide, c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[c][i] *= x[i];
+        }
+        rows.template load4<R>(x, src.residual, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] += a.residual_scale * x[i];
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template load4<R>(r[c], src.residual, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= a.residual_scale;
+      }
+    }
+    if (a.r) {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) rows.template store4<R>((R*)a.r + row * a.H, c, r[c]);
+    }
+    float inv = 0.f;
+    if (has_y) {
+      ss[0] = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
+      rows.sum(ss, sums[1]);
+      inv = rsqrtf(ss[0] * inv_h + a.eps);
+      if (rows.tid == 0 && a.stat) a.stat[a.T + row] = inv;
+    } else {
+      rows.barrier();
+    }
+    rows.refill(row, 0);  // the barrier of the sum: every thread has taken the row out of its stage
+    rows.next();
+    if (has_y) {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= inv * wp[c][i];
+        rows.template store4<T>((T*)a.y + row * a.H, c, r[c]);
+      }
+      if (!(has_h && has_post)) rows.barrier();  // the one buffer of this sum has been read by all
+    }
+  }
+  rows.end();
 }
 
-// The values are taken from the stage twice, before and after the row's sums, instead of being held in registers.
-template <typename T, typename R, bool FULL>
-__global__ void __launch_bounds__(RING_THREADS, 1) backward_ring_kernel(const __grid_constant__ RingParams p) {
+// The values are taken from the source twice, before and after the row's sums, instead of being held in registers.
+// ALL: h, dr, dy, post and a gate per channel or none, as compile-time facts; without it each part is looked up.
+template <typename T, typename R, Mode MODE, bool ALL>
+__global__ void __launch_bounds__(ROW_THREADS, 1) backward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][16][3];
-  const int threads = blockDim.x - 32, warps = threads >> 5, warp = threadIdx.x >> 5;
-  Ring ring = ring_setup(p, smem, warps);
-  if (warp == warps) {
-    ring_fill(p, ring, true);
-  } else {
-    const RingRows rows = ring_rows(a, true);
-    const bool wide = a.wt_type == BSHMEM_NORM_F32 && sizeof(T) < 4, token = a.gate_mode == BSHMEM_NORM_GATE_TOKEN;
-    float u[RING_CH][4], wp[RING_CH][4], acc_s[RING_CH][4], acc_p[RING_CH][4];
+  Rows<MODE> rows(p, smem, true);
+  const bool wide = a.wt_type == BSHMEM_NORM_F32 && sizeof(T) < 4;
+  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_dr = ALL || a.dr, has_dy = ALL || a.dy;
+  const float inv_h = 1.f / (float)a.H;
+  float u[ROW_CH][4], wp[ROW_CH][4], acc_s[ROW_CH][4], acc_p[ROW_CH][4];
 #pragma unroll
-    for (int c = 0; c < RING_CH; ++c) {
-      if (a.h) load_u<T>(u[c], a, wide, ring_col(c, threads));
-      if (a.dy) load4_wt<T>(wp[c], a.pre, wide, ring_col(c, threads), a.H);
+  for (int c = 0; c < ROW_CH; ++c) {
+    if (has_h) rows.template load_u<T>(u[c], wide, c);
+    if (has_dy) rows.template load4_wt<T>(wp[c], a.pre, wide, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      wp[c][i] = has_dy ? wp[c][i] + a.weight_offset : 0.f;
+      if (!has_h) u[c][i] = 0.f;
+      acc_s[c][i] = acc_p[c][i] = 0.f;
+    }
+  }
+  int buf = 0;
+  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+    const float tg = token ? load1_wt<T>(a.gate, wide, row) : 1.f;
+    const float s1 = has_h && has_post ? a.stat[row] : 1.f, s2 = has_dy ? a.stat[a.T + row] : 0.f;
+    const RowSource src = rows.wait(row);
+    // hh = hhat, ge = the row's gate, rh = rhat, dy, g = dr + s2 dy pre of four columns
+    auto values = [&](int c, float* hh, float* ge, float* rh, float* dy, float* g) {
+      rows.template load4<R>(rh, src.residual, c);
+      if (has_h) rows.template load4<T>(hh, src.h, c);
+      if (full) rows.template load4_wt<T>(ge, src.gate, wide, c);
+      if (has_dr) rows.template load4<R>(g, src.dr, c);
+      if (has_dy) rows.template load4<T>(dy, src.dy, c);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        wp[c][i] = a.dy ? wp[c][i] + a.weight_offset : 0.f;
-        if (!a.h) u[c][i] = 0.f;
-        acc_s[c][i] = acc_p[c][i] = 0.f;
+        if (!full) ge[i] = tg;
+        hh[i] = has_h ? hh[i] * s1 : 0.f;
+        if (!has_dr) g[i] = 0.f;
+        if (!has_dy) dy[i] = 0.f;
+        rh[i] = s2 * (a.residual_scale * rh[i] + ge[i] * u[c][i] * hh[i]);
+        g[i] += s2 * (dy[i] * wp[c][i]);
+      }
+    };
+    float v[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < ROW_CH; ++c) {
+      float hh[4], ge[4], rh[4], dy[4], g[4];
+      values(c, hh, ge, rh, dy, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float q = u[c][i] * hh[i] * (full ? ge[i] : 1.f);   // without a gate per token: see c2
+        v[0] += dy[i] * wp[c][i] * rh[i];
+        v[1] += q * g[i];
+        v[2] += q * rh[i];
       }
     }
-    int buf = 0;
-    for (size_t row = blockIdx.x; row < (size_t)a.T; row += gridDim.x) {
-      const float tg = token ? load1_wt<T>(a.gate, wide, row) : 1.f;
-      const float s1 = a.h && a.post ? a.stat[row] : 1.f, s2 = a.dy ? a.stat[a.T + row] : 0.f;
-      sm100::mbar_wait(&ring.full[ring.stage], ring.phase, RING_WAIT_NS, ring.abort_flag);
-      const uint8_t* src = ring.data + (size_t)ring.stage * p.stage_bytes;
-      // hh = hhat, ge = the row's gate, rh = rhat, dy, g = dr + s2 dy pre of four columns
-      auto values = [&](int c, float* hh, float* ge, float* rh, float* dy, float* g) {
-        const int col = ring_col(c, threads);
-        load4<R>(rh, (const R*)(src + rows.residual), col, a.H);
-        if (a.h) load4<T>(hh, (const T*)(src + rows.h), col, a.H);
-        if constexpr (FULL) load4_wt<T>(ge, src + rows.gate, wide, col, a.H);
-        if (a.dr) load4<R>(g, (const R*)(src + rows.dr), col, a.H);
-        if (a.dy) load4<T>(dy, (const T*)(src + rows.dy), col, a.H);
+    rows.sum(v, sums[buf]);
+    buf ^= 1;
+    rows.refill(row, 1);  // the barrier of the sum: every thread is done with the row before
+    const float c1 = s2 * v[0] * inv_h, qg = v[1] - c1 * v[2], c2 = has_post ? qg * tg * inv_h : 0.f;
+    if (token && a.dgate && rows.tid == 0) store1_wt<T>(a.dgate, wide, row, qg);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (!FULL) ge[i] = tg;
-          hh[i] = a.h ? hh[i] * s1 : 0.f;
-          if (!a.dr) g[i] = 0.f;
-          if (!a.dy) dy[i] = 0.f;
-          rh[i] = s2 * (a.residual_scale * rh[i] + ge[i] * u[c][i] * hh[i]);
-          g[i] += s2 * (dy[i] * wp[c][i]);
-        }
-      };
-      float v[3] = {0.f, 0.f, 0.f};
+    for (int c = 0; c < ROW_CH; ++c) {
+      float hh[4], ge[4], rh[4], dy[4], g[4];
+      values(c, hh, ge, rh, dy, g);
 #pragma unroll
-      for (int c = 0; c < RING_CH; ++c) {
-        float hh[4], ge[4], rh[4], dy[4], g[4];
-        values(c, hh, ge, rh, dy, g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float q = u[c][i] * hh[i] * (FULL ? ge[i] : 1.f);   // without a gate per token: see c2
-          v[0] += dy[i] * wp[c][i] * rh[i];
-          v[1] += q * g[i];
-          v[2] += q * rh[i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        g[i] -= c1 * rh[i];
+        acc_p[c][i] += dy[i] * rh[i];
+        acc_s[c][i] += ge[i] * g[i] * hh[i];
+        dy[i] = a.residual_scale * g[i];
       }
-      ring_sum<3>(v, sums[buf], warps);
-      buf ^= 1;
-      const float c1 = s2 * v[0] / (float)a.H, qg = v[1] - c1 * v[2], c2 = a.post ? qg * tg / (float)a.H : 0.f;
-      if (token && a.dgate && threadIdx.x == 0) store1_wt<T>(a.dgate, wide, row, qg);
+      if (a.dresidual) rows.template store4<R>((R*)a.dresidual + row * a.H, c, dy);
+      if (a.dh) {
 #pragma unroll
-      for (int c = 0; c < RING_CH; ++c) {
-        const int col = ring_col(c, threads);
-        float hh[4], ge[4], rh[4], dy[4], g[4];
-        values(c, hh, ge, rh, dy, g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[i] -= c1 * rh[i];
-          acc_p[c][i] += dy[i] * rh[i];
-          acc_s[c][i] += ge[i] * g[i] * hh[i];
-          dy[i] = a.residual_scale * g[i];
-        }
-        if (a.dresidual) store4<R>((R*)a.dresidual + row * a.H, col, a.H, dy);
-        if (a.dh) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dy[i] = s1 * (ge[i] * u[c][i] * g[i] - hh[i] * c2);
-          store4<T>((T*)a.dh + row * a.H, col, a.H, dy);
-        }
-        if (FULL && a.dgate) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dy[i] = g[i] * u[c][i] * hh[i];
-          if (wide) store4<float>((float*)a.dgate + row * a.H, col, a.H, dy);
-          else store4<T>((T*)a.dgate + row * a.H, col, a.H, dy);
-        }
+        for (int i = 0; i < 4; ++i) dy[i] = s1 * (ge[i] * u[c][i] * g[i] - hh[i] * c2);
+        rows.template store4<T>((T*)a.dh + row * a.H, c, dy);
       }
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) sm100::mbar_arrive(&ring.empty[ring.stage]);
-      ring_next(ring, p.stages);
+      if (full && a.dgate) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dy[i] = g[i] * u[c][i] * hh[i];
+        if (wide) rows.template store4<float>((float*)a.dgate + row * a.H, c, dy);
+        else rows.template store4<T>((T*)a.dgate + row * a.H, c, dy);
+      }
     }
-    if (a.partials) {
+    rows.next();
+  }
+  if (a.partials) {
+    float* part = a.partials + (size_t)blockIdx.x * 2 * a.H;
+    if (MODE == STAGED || blockDim.x == rows.threads) {
 #pragma unroll
-      for (int c = 0; c < RING_CH; ++c) {
-        store4<float>(a.partials + (size_t)blockIdx.x * 2 * a.H, ring_col(c, threads), a.H, acc_s[c]);
-        store4<float>(a.partials + ((size_t)blockIdx.x * 2 + 1) * a.H, ring_col(c, threads), a.H, acc_p[c]);
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template store4<float>(part, c, acc_s[c]);
+        rows.template store4<float>(part + a.H, c, acc_p[c]);
+      }
+    } else {  // the warps' sums, in order
+      float* s = (float*)smem;  // [warps][2][H]
+      const int warps = blockDim.x >> 5;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template store4<float>(s + (threadIdx.x >> 5) * 2 * a.H, c, acc_s[c]);
+        rows.template store4<float>(s + ((threadIdx.x >> 5) * 2 + 1) * a.H, c, acc_p[c]);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * a.H; i += blockDim.x) {
+        float v = 0.f;
+        for (int k = 0; k < warps; ++k) v += s[k * 2 * a.H + i];
+        part[i] = v;
       }
     }
   }
-  ring_end(p, ring);
+  rows.end();
 }
 
 static bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -734,12 +805,6 @@ static int check(const bshmem_norm_args_t* a) {
   return BSHMEM_NORM_OK;
 }
 
-static int group_threads(int H, int chunks) {
-  int g = 32;
-  while (g * CHUNK * chunks < H && g < MAX_THREADS) g *= 2;
-  return g;
-}
-
 static int sm_count() {
   int device = 0, sms = 0;
   cudaGetDevice(&device);
@@ -747,72 +812,90 @@ static int sm_count() {
   return sms > 0 ? sms : 1;
 }
 
-static int backward_ctas(int T, int H) {
-  const int group = group_threads(H, 1), groups = group < 128 ? 128 / group : 1;
-  const int want = (T + groups - 1) / groups, most = sm_count() * (H <= 4096 ? 4 : 1);
-  return want < most ? want : most;
-}
-
-// How the ring kernels run a call; `ctas` 0: they do not take it.
-struct RingPlan {
-  int ctas, threads, stages, stage_bytes, smem;
+// How the kernels for rows of up to 8192 run a call; `ctas` 0: they do not take it.
+struct RowPlan {
+  Mode mode;
+  int ctas, block, threads, stages, stage_bytes, smem;
 };
-static RingPlan ring_plan(const bshmem_norm_args_t* a, bool backward, bool vec) {
-  RingPlan r = {0, 0, 0, 0, 0};
-  if (!vec || a->H < 1024 || a->H > RING_MAX_H) return r;
-  r.threads = (a->H + RING_COLS * 32 - 1) / (RING_COLS * 32) * 32;
-  const int per_sm = r.threads >= 320 ? 1 : 512 / r.threads < 6 ? 512 / r.threads : 6, sms = sm_count();
-  r.stage_bytes = ring_rows(*a, backward).bytes;
-  const int budget = RING_SMEM / per_sm - 2048;
-  r.stages = budget / r.stage_bytes < RING_MAX_STAGES ? budget / r.stage_bytes : RING_MAX_STAGES;
-  if (r.stages < 2 || a->T <= 2 * sms) return r;
-  r.smem = r.stages * r.stage_bytes + RING_MAX_STAGES * 16 + 16;
-  r.threads += 32;
-  r.ctas = a->T < sms * per_sm ? a->T : sms * per_sm;
+static RowPlan row_plan(const bshmem_norm_args_t* a, bool backward, bool vec) {
+  RowPlan r = {vec ? VECTOR : SCALAR, 0, 0, 0, 0, 0, 0};
+  if (a->H > ROW_MAX_H) return r;
+  const int sms = sm_count();
+  r.threads = (a->H + ROW_COLS * 32 - 1) / (ROW_COLS * 32) * 32;
+  if (a->H <= WARP_MAX_H) {
+    r.block = 32 * WARP_GROUPS;
+    r.smem = backward && a->partials ? WARP_GROUPS * 2 * a->H * 4 : 0;
+  } else {
+    r.block = r.threads;
+  }
+  int per_sm = ROW_THREADS / r.block;
+  if (vec && a->H > WARP_MAX_H && a->T > sms * per_sm) {
+    // Two stages at least; rather fewer CTAs of an SM than none.
+    r.stage_bytes = stage_rows(*a, backward).bytes;
+    for (int n = per_sm < 6 ? per_sm : 6; n > 0; --n) {
+      const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
+      if (fit < 2) continue;
+      r.mode = STAGED;
+      r.stages = fit < MAX_STAGES ? fit : MAX_STAGES;
+      r.smem = r.stages * r.stage_bytes + MAX_STAGES * 8 + 16;
+      per_sm = n;
+      break;
+    }
+  }
+  const int groups = r.block / r.threads, want = (int)(((int64_t)a->T + groups - 1) / groups);
+  r.ctas = want < sms * per_sm ? want : sms * per_sm;
   return r;
 }
-// Raises a kernel's shared-memory limit to what a ring may take.
+static bool plain_gate(const bshmem_norm_args_t& a) { return a.gate_mode == BSHMEM_NORM_GATE_NONE || a.gate_mode == BSHMEM_NORM_GATE_CHANNEL; }
+// Raises a kernel's shared-memory limit to what it may take.
 static bool reserve_smem(const void* kernel, int bytes) {
   return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
+static int long_row_ctas(int T) {
+  const int sms = sm_count();
+  return T < sms ? T : sms;
+}
 
 template <typename T, typename R>
-static int launch_forward(const Params& p, int chunks, bool vec, cudaStream_t stream) {
-  const RingPlan ring = ring_plan(&p.a, false, vec);
-  if (ring.ctas) {
-    const RingParams rp = {p.a, ring.stages, ring.stage_bytes};
-    void (*const kernel)(RingParams) = p.a.gate_mode == BSHMEM_NORM_GATE_FULL ? forward_ring_kernel<T, R, true> : forward_ring_kernel<T, R, false>;
-    if (!reserve_smem((const void*)kernel, ring.smem)) return BSHMEM_NORM_ERR_DRIVER;
-    kernel<<<ring.ctas, ring.threads, ring.smem, stream>>>(rp);
-    return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+static int launch_forward(const bshmem_norm_args_t* a, cudaStream_t stream) {
+  const bool vec = vectors(a);
+  const RowPlan plan = row_plan(a, false, vec);
+  if (plan.ctas) {
+    const RowParams p = {*a, plan.threads, plan.stages, plan.stage_bytes};
+    const bool all = plan.mode == STAGED && plain_gate(*a) && a->post && a->y;
+    void (*const kernel)(RowParams) = all ? forward_rows_kernel<T, R, STAGED, true> : plan.mode == STAGED ? forward_rows_kernel<T, R, STAGED, false>
+                                      : plan.mode == VECTOR ? forward_rows_kernel<T, R, VECTOR, false> : forward_rows_kernel<T, R, SCALAR, false>;
+    if (!reserve_smem((const void*)kernel, plan.smem)) return BSHMEM_NORM_ERR_DRIVER;
+    kernel<<<plan.ctas, plan.block, plan.smem, stream>>>(p);
+  } else {
+    const Params p = {*a, MAX_THREADS};
+    if (vec) forward_kernel<T, R, 2, true><<<a->T, MAX_THREADS, 0, stream>>>(p);
+    else forward_kernel<T, R, 2, false><<<a->T, MAX_THREADS, 0, stream>>>(p);
   }
-  const int threads = p.group < 128 ? 128 : p.group, rows = threads / p.group;
-  const unsigned grid = (unsigned)(((size_t)p.a.T + rows - 1) / rows);
-  if (chunks == 1 && vec) forward_kernel<T, R, 1, true><<<grid, threads, 0, stream>>>(p);
-  else if (chunks == 1) forward_kernel<T, R, 1, false><<<grid, threads, 0, stream>>>(p);
-  else if (vec) forward_kernel<T, R, 2, true><<<grid, threads, 0, stream>>>(p);
-  else forward_kernel<T, R, 2, false><<<grid, threads, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
 }
 
 template <typename T, typename R>
-static int launch_backward(const Params& p, int chunks, bool vec, cudaStream_t stream) {
-  const RingPlan ring = ring_plan(&p.a, true, vec);
-  int grid = ring.ctas;
-  if (grid) {
-    const RingParams rp = {p.a, ring.stages, ring.stage_bytes};
-    void (*const kernel)(RingParams) = p.a.gate_mode == BSHMEM_NORM_GATE_FULL ? backward_ring_kernel<T, R, true> : backward_ring_kernel<T, R, false>;
-    if (!reserve_smem((const void*)kernel, ring.smem)) return BSHMEM_NORM_ERR_DRIVER;
-    kernel<<<grid, ring.threads, ring.smem, stream>>>(rp);
+static int launch_backward(const bshmem_norm_args_t* a, cudaStream_t stream) {
+  const bool vec = vectors(a);
+  const RowPlan plan = row_plan(a, true, vec);
+  const Params long_row = {*a, MAX_THREADS};
+  int parts = plan.ctas;
+  if (plan.ctas) {
+    const RowParams p = {*a, plan.threads, plan.stages, plan.stage_bytes};
+    const bool all = plan.mode == STAGED && plain_gate(*a) && a->post && a->dr && a->dy;
+    void (*const kernel)(RowParams) = all ? backward_rows_kernel<T, R, STAGED, true> : plan.mode == STAGED ? backward_rows_kernel<T, R, STAGED, false>
+                                      : plan.mode == VECTOR ? backward_rows_kernel<T, R, VECTOR, false> : backward_rows_kernel<T, R, SCALAR, false>;
+    if (!reserve_smem((const void*)kernel, plan.smem)) return BSHMEM_NORM_ERR_DRIVER;
+    kernel<<<plan.ctas, plan.block, plan.smem, stream>>>(p);
   } else {
-    const int threads = p.group < 128 ? 128 : p.group, groups = threads / p.group, smem = p.a.partials ? groups * 2 * p.a.H * 4 : 0;
-    grid = backward_ctas(p.a.T, p.a.H);
-    void (*const kernel)(Params) = chunks == 1 ? (vec ? backward_kernel<T, R, 1, true> : backward_kernel<T, R, 1, false>)
-                                               : (vec ? backward_kernel<T, R, 2, true> : backward_kernel<T, R, 2, false>);
+    parts = long_row_ctas(a->T);
+    const int smem = a->partials ? 2 * a->H * 4 : 0;
+    void (*const kernel)(Params) = vec ? backward_kernel<T, R, 2, true> : backward_kernel<T, R, 2, false>;
     if (!reserve_smem((const void*)kernel, smem)) return BSHMEM_NORM_ERR_DRIVER;
-    kernel<<<grid, threads, smem, stream>>>(p);
+    kernel<<<parts, MAX_THREADS, smem, stream>>>(long_row);
   }
-  if (p.a.partials) column_sum_kernel<T><<<dim3((p.a.H + 31) / 32, 2), dim3(32, 8), 0, stream>>>(p, grid);
+  if (a->partials) column_sum_kernel<T><<<dim3((a->H + 31) / 32, 2), dim3(32, SLICES), 0, stream>>>(long_row, parts);
   return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
 }
 
@@ -829,11 +912,11 @@ static int by_type(const bshmem_norm_args_t* a, F&& f) {
 
 using namespace bshmem::norms;
 
-// Parts of at most the CTAs of either backward kernel.
+// One part per CTA, of whichever kernel takes the call.
 extern "C" size_t bshmem_block_norms_partials(int T, int H) {
   if (T <= 0 || H <= 0) return 0;
-  const int most = sm_count() * 6, ctas = backward_ctas(T, H);
-  return (size_t)(T < most ? (T > ctas ? T : ctas) : most) * 2 * H;
+  const int most = sm_count() * (ROW_THREADS / 64);
+  return (size_t)(T < most ? T : most) * 2 * H;
 }
 
 extern "C" int bshmem_block_norms(const bshmem_norm_args_t* a, cudaStream_t stream) {
@@ -841,12 +924,7 @@ extern "C" int bshmem_block_norms(const bshmem_norm_args_t* a, cudaStream_t stre
   const int st = check(a);
   if (st) return st;
   if ((!a->r && !a->y) || !a->error_flag) return BSHMEM_NORM_ERR_ARGS;
-  const int group = group_threads(a->H, 1), chunks = a->H > group * CHUNK ? 2 : 1;
-  const Params p = {*a, group};
-  const bool vec = vectors(a);
-  return by_type(a, [&](auto* t, auto* r) {
-    return launch_forward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(p, chunks, vec, stream);
-  });
+  return by_type(a, [&](auto* t, auto* r) { return launch_forward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(a, stream); });
 }
 
 extern "C" int bshmem_block_norms_backward(const bshmem_norm_args_t* a, cudaStream_t stream) {
@@ -857,11 +935,7 @@ extern "C" int bshmem_block_norms_backward(const bshmem_norm_args_t* a, cudaStre
   const bool sums = a->dpost || a->dpre || (a->dgate && a->gate_mode == BSHMEM_NORM_GATE_CHANNEL);
   if ((!a->dr && !a->dy) || (a->dpre && !a->dy) || (a->dpost && !a->post) || ((a->dh || a->dgate) && !a->h) || (a->dgate && !a->gate_mode)) return BSHMEM_NORM_ERR_ARGS;
   if ((sums && !a->partials) || ((a->post || a->dy) && !a->stat)) return BSHMEM_NORM_ERR_ARGS;
-  const int group = group_threads(a->H, 1), chunks = a->H > group * CHUNK ? 2 : 1;
-  Params p = {*a, group};
-  if (!sums) p.a.partials = nullptr;
-  const bool vec = vectors(a);
-  return by_type(a, [&](auto* t, auto* r) {
-    return launch_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(p, chunks, vec, stream);
-  });
+  bshmem_norm_args_t args = *a;
+  if (!sums) args.partials = nullptr;
+  return by_type(a, [&](auto* t, auto* r) { return launch_backward<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(r)>>(&args, stream); });
 }
