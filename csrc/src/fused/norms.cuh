@@ -1,0 +1,656 @@
+// Kernels of the norms around a block; norms_{bf16,f16,f32}.cu instantiate them, norms.cu checks calls and picks a type.
+//
+// Every thread owns sixteen columns for the whole run, with their parameters and their sums over rows in registers; its CTA (up to 512
+// columns its warp, above 8192 its pair of CTAs, half a row each) walks rows with the stride of the grid.  512 threads of 128 registers
+// take 8192 columns.  Each input is read once from memory and each output written once.
+//   STAGED  one thread copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that the bytes in
+//           flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which spill:
+//           backward at 4096 x 8192 took 269 us with it, 119 without.)
+//   VECTOR  rows are read where they lie, 8 or 16 bytes at a time: few rows, or rows too large for two stages
+//   SCALAR  the same one value at a time, for odd sizes and addresses
+//
+// Backward.  With hhat = h s1, rhat = r s2 (s1, s2 from forward), u = branch_scale post, q = gate u hhat:
+//   c1 = mean(dy pre rhat)     G = dr + s2 (dy pre - rhat c1)          gradient of r
+//   dresidual = residual_scale G      dgate = G u hhat
+//   dh = s1 (gate u G - hhat c2),  c2 = mean(q G) = mean(q (dr + s2 dy pre)) - c1 s2 mean(q rhat)
+//   dpost = branch_scale sum over rows of gate G hhat     dpre = sum of dy rhat
+// c2 is linear in G, so one reduction of three sums serves a row.  (For a gate per token the sums are taken without the gate:
+// they are its gradient.)  Where the gate is per channel it is the same for every row, and one sum S = sum of G hhat gives both
+// dpost = branch_scale gate S and dgate = u S.  A CTA keeps its part of the two
+// sums over rows; a second kernel adds the CTAs' parts in order.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/bshmem/norms.h"
+#include "../../include/bshmem/tcgen05.cuh"
+
+namespace bshmem {
+namespace norms {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// Element i of a parameter of type W.
+template <typename W>
+__device__ __forceinline__ float load1(const void* p, size_t i) {
+  return to_f<W>(((const W*)p)[i]);
+}
+template <typename W>
+__device__ __forceinline__ void store1(void* p, size_t i, float v) {
+  ((W*)p)[i] = from_f<W>(v);
+}
+
+enum Mode { STAGED, VECTOR, SCALAR };
+constexpr int ROW_CH = 4, ROW_COLS = 4 * ROW_CH, CTA_COLS = 8192, ROW_THREADS = CTA_COLS / ROW_COLS, MAX_STAGES = 8;
+constexpr int WARP_COLS = 32 * ROW_COLS, WARP_GROUPS = 8;   // rows of a warp each
+constexpr int STAGE_SMEM = 216 * 1024;  // of an SM, shared by its CTAs
+constexpr int SUM_ROWS = 17;            // 16 warps, and the other CTA of a pair
+static_assert(BSHMEM_NORM_MAX_H == 2 * CTA_COLS, "a pair of CTAs takes the longest row");
+
+struct RowParams {
+  bshmem_norm_args_t a;
+  int threads;              // per row and CTA
+  int half;                 // columns of the first CTA of a pair; 0: no pairs
+  int stages, stage_bytes;  // STAGED
+};
+
+// The parts of a row that are copied, in the order of their places in a stage.
+struct StageRows {
+  int h, residual, dr, dy, gate;  // offsets; -1: absent
+  int bytes;
+};
+__host__ __device__ __forceinline__ int type_bytes(int t) { return t == BSHMEM_NORM_F32 ? 4 : 2; }
+__host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_t& a, int cols, bool backward) {
+  StageRows r;
+  const int t = cols * type_bytes(a.type), rt = cols * type_bytes(a.res_type), wt = cols * type_bytes(a.wt_type);
+  int at = 0;
+  auto place = [&](bool present, int bytes) {
+    const int here = present ? at : -1;
+    if (present) at += bytes;
+    return here;
+  };
+  r.residual = place(true, rt);
+  r.h = place(a.h != nullptr, t);
+  r.dr = place(backward && a.dr, rt);
+  r.dy = place(backward && a.dy, t);
+  r.gate = place(a.gate_mode == BSHMEM_NORM_GATE_FULL, wt);
+  r.bytes = at;
+  return r;
+}
+
+// This CTA's columns of a row's inputs, wherever they are.
+struct RowSource {
+  const uint8_t *h, *residual, *dr, *dy, *gate;
+};
+
+template <Mode MODE>
+struct Rows {
+  const RowParams& p;
+  uint8_t* data = nullptr;
+  uint64_t* full = nullptr;
+  volatile int* abort_flag = nullptr;
+  StageRows at;
+  int tid, threads, base, cols, stage = 0;  // base, cols: this CTA's columns
+  uint32_t phase = 0;
+  size_t first, step;
+
+  static constexpr uint64_t WAIT_NS = 10000000000ull;  // the waits are for this CTA's own copies
+
+  __device__ __forceinline__ RowSource global(size_t row) const {
+    const bshmem_norm_args_t& a = p.a;
+    const size_t ts = type_bytes(a.type), rs = type_bytes(a.res_type), ws = type_bytes(a.wt_type);
+    RowSource g;
+    g.residual = (const uint8_t*)a.residual + (row * a.res_stride + base) * rs;
+    g.h = (const uint8_t*)a.h + (row * a.h_stride + base) * ts;
+    g.dr = (const uint8_t*)a.dr + (row * a.dr_stride + base) * rs;
+    g.dy = (const uint8_t*)a.dy + (row * a.dy_stride + base) * ts;
+    g.gate = (const uint8_t*)a.gate + (row * a.gate_stride + base) * ws;
+    return g;
+  }
+  // Starts the copy of a row into a stage that nobody reads any more.  One thread.
+  __device__ __forceinline__ void load(size_t row, int to) const {
+    const RowSource g = global(row);
+    const int ts = type_bytes(p.a.type), rs = type_bytes(p.a.res_type), ws = type_bytes(p.a.wt_type);
+    uint8_t* dst = data + (size_t)to * p.stage_bytes;
+    uint64_t* bar = &full[to];
+    sm100::mbar_expect_tx(bar, at.bytes);
+    sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
+    if (at.h >= 0) sm100::bulk_load(dst + at.h, g.h, cols * ts, bar);
+    if (at.dr >= 0) sm100::bulk_load(dst + at.dr, g.dr, cols * rs, bar);
+    if (at.dy >= 0) sm100::bulk_load(dst + at.dy, g.dy, cols * ts, bar);
+    if (at.gate >= 0) sm100::bulk_load(dst + at.gate, g.gate, cols * ws, bar);
+  }
+  __device__ __forceinline__ Rows(const RowParams& params, uint8_t* smem, bool backward) : p(params) {
+    const int pair = p.half ? 2 : 1, rank = p.half ? blockIdx.x & 1 : 0, groups = blockDim.x / p.threads;
+    threads = p.threads;
+    base = rank ? p.half : 0;
+    cols = !p.half ? p.a.H : rank ? p.a.H - p.half : p.half;
+    at = stage_rows(p.a, cols, backward);
+    tid = threadIdx.x % threads;
+    first = (size_t)(blockIdx.x / pair) * groups + threadIdx.x / threads;
+    step = (size_t)(gridDim.x / pair) * groups;
+    if constexpr (MODE == STAGED) {
+      data = smem;
+      full = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
+      abort_flag = (volatile int*)(full + MAX_STAGES);
+      if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int i = 0; i < p.stages; ++i) sm100::mbar_init(&full[i], 1);
+        sm100::mbar_fence_init();
+        sm100::fence_proxy_async_smem();
+        for (int i = 0; i < p.stages; ++i)
+          if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
+      }
+      __syncthreads();
+    }
+    if (p.half) sm100::cluster_sync_all();  // the other CTA runs: its shared memory may be written
+  }
+  __device__ __forceinline__ RowSource wait(size_t row) const {
+    if constexpr (MODE == STAGED) {
+      sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
+      const uint8_t* s = data + (size_t)stage * p.stage_bytes;
+      return {s + at.h, s + at.residual, s + at.dr, s + at.dy, s + at.gate};
+    } else {
+      return global(row);
+    }
+  }
+  // All threads are past their last look at the stage of `row` (`behind` = 0) or of the row before it (1): it takes the next row that
+  // falls to it.
+  __device__ __forceinline__ void refill(size_t row, int behind) const {
+    if constexpr (MODE == STAGED) {
+      const size_t next = row + (size_t)(p.stages - behind) * step;
+      if (threadIdx.x == 0 && row >= first + behind * step && next < (size_t)p.a.T) load(next, stage >= behind ? stage - behind : p.stages - 1);
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if constexpr (MODE == STAGED) {
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  __device__ __forceinline__ void end() const {
+    if constexpr (MODE == STAGED) {
+      __syncthreads();
+      if (!*abort_flag) return;
+      const uint64_t t0 = sm100::timer_ns();  // copies still in flight land before the shared memory goes away
+      while (sm100::timer_ns() - t0 < 200000) __nanosleep(1000);
+      if (threadIdx.x == 0) atomicOr(p.a.error_flag, 1);
+    }
+  }
+
+  // This thread's four columns of chunk c, of the 512 neighbouring ones of its warp.  With vectors they are neighbours (8 or 16 bytes a
+  // thread: a warp's accesses to shared memory are free of bank conflicts for both sizes of type); without, they are 32 apart.
+  __device__ __forceinline__ int col(int c, int i) const {
+    const int lane = tid & 31, warp_first = (tid >> 5) * WARP_COLS;
+    return MODE == SCALAR ? warp_first + lane + (c * 4 + i) * 32 : warp_first + lane * 4 + c * 128 + i;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load4(float* f, const void* row, int c) const {
+    if constexpr (MODE == SCALAR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = col(c, i) < cols ? to_f<T>(((const T*)row)[col(c, i)]) : 0.f;
+      }
+    } else {
+      const int at = col(c, 0);
+      alignas(16) T raw[4];
+      if constexpr (sizeof(T) == 4) *(uint4*)raw = at < cols ? *(const uint4*)((const T*)row + at) : make_uint4(0u, 0u, 0u, 0u);
+      else *(uint2*)raw = at < cols ? *(const uint2*)((const T*)row + at) : make_uint2(0u, 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = to_f<T>(raw[i]);
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store4(T* row, int c, const float* f) const {
+    if constexpr (MODE == SCALAR) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (col(c, i) < cols) row[col(c, i)] = from_f<T>(f[i]);
+      }
+    } else {
+      const int at = col(c, 0);
+      if (at >= cols) return;
+      alignas(16) T raw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(f[i]);
+      if constexpr (sizeof(T) == 4) *(uint4*)(row + at) = *(uint4*)raw;
+      else *(uint2*)(row + at) = *(uint2*)raw;
+    }
+  }
+  // This CTA's part of a parameter, and of a row of a dense output.
+  template <typename W>
+  __device__ __forceinline__ const W* mine(const void* parameter) const { return (const W*)parameter + base; }
+  template <typename T>
+  __device__ __forceinline__ T* out(void* rows, size_t row) const { return (T*)rows + row * p.a.H + base; }
+
+  // u = branch_scale (post + offset) gate, without the gate where it differs from row to row.  The loads do not hang on one another.
+  template <typename W>
+  __device__ __forceinline__ void load_u(float* u, int c, bool has_post) const {
+    const bshmem_norm_args_t& a = p.a;
+    const bool channel = a.gate_mode == BSHMEM_NORM_GATE_CHANNEL;
+    float g[4];
+    if (has_post) {
+      load4<W>(u, mine<W>(a.post), c);
+      load4<W>(g, mine<W>(channel ? a.gate : a.post), c);
+    } else if (channel) {
+      load4<W>(g, mine<W>(a.gate), c);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = (has_post ? u[i] + a.weight_offset : 1.f) * (channel ? g[i] : 1.f) * a.branch_scale;
+  }
+  // Sum over a row's threads, the same value in every one of them.  One barrier per sum: consecutive sums use two buffers in turn.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N], float (*s)[N]) const {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (blockDim.x != threads) return;  // a warp's row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[warp][i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane < warps ? s[lane][i] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+    if (!p.half) return;
+    if (threadIdx.x == 0) {  // to the other CTA
+      const uint32_t other = sm100::mapa_u32(sm100::smem_u32(&s[SUM_ROWS - 1][0]), (sm100::cluster_ctarank() ^ 1));
+#pragma unroll
+      for (int i = 0; i < N; ++i) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(other + 4 * i), "f"(v[i]) : "memory");
+    }
+    sm100::cluster_sync_all();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += s[SUM_ROWS - 1][i];
+  }
+};
+
+// ALL: h, both norms, and a gate per channel or none, as compile-time facts; without it each part is looked up.
+template <typename T, typename R, typename W, Mode MODE, bool ALL>
+__global__ void __launch_bounds__(ROW_THREADS, 1) forward_rows_kernel(const __grid_constant__ RowParams p) {
+  const bshmem_norm_args_t& a = p.a;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sums[2][SUM_ROWS][1];
+  Rows<MODE> rows(p, smem, false);
+  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_y = ALL || a.y;
+  const float inv_h = 1.f / (float)a.H;
+  float u[ROW_CH][4], wp[ROW_CH][4];
+#pragma unroll
+  for (int c = 0; c < ROW_CH; ++c) {
+    if (has_h) rows.template load_u<W>(u[c], c, has_post);
+    if (has_y) {
+      rows.template load4<W>(wp[c], rows.template mine<W>(a.pre), c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wp[c][i] += a.weight_offset;
+    }
+  }
+  int buf = 0;
+  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+    const float tg = token ? load1<W>(a.gate, row) : 1.f;
+    const RowSource src = rows.wait(row);
+    float r[ROW_CH][4], ss[1];
+    if (has_h) {
+      float inv = 1.f, res[MODE == STAGED ? 1 : ROW_CH][4];
+      ss[0] = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template load4<T>(r[c], src.h, c);
+        if constexpr (MODE != STAGED) rows.template load4<R>(res[c], src.residual, c);  // on the way during the sum
+      }
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
+      if (has_post) {
+        rows.sum(ss, sums[buf]);
+        buf ^= 1;
+        inv = rsqrtf(ss[0] * inv_h + a.eps);
+        if (rows.tid == 0 && a.stat) a.stat[row] = inv;
+      }
+      inv *= tg;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= inv * u[c][i];
+        if (full) {
+          rows.template load4<W>(x, src.gate, c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[c][i] *= x[i];
+        }
+        if constexpr (MODE == STAGED) rows.template load4<R>(x, src.residual, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] += a.residual_scale * (MODE == STAGED ? x[i] : res[MODE == STAGED ? 0 : c][i]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.template load4<R>(r[c], src.residual, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= a.residual_scale;
+      }
+    }
+    if (a.r) {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) rows.store4(rows.template out<R>(a.r, row), c, r[c]);
+    }
+    float inv = 0.f;
+    if (has_y) {
+      ss[0] = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss[0] += r[c][i] * r[c][i];
+      rows.sum(ss, sums[buf]);
+      buf ^= 1;
+      inv = rsqrtf(ss[0] * inv_h + a.eps);
+      if (rows.tid == 0 && a.stat) a.stat[a.T + row] = inv;
+    } else if (MODE == STAGED) {
+      __syncthreads();
+    }
+    rows.refill(row, 0);  // after a barrier: every thread has taken the row out of its stage
+    rows.next();
+    if (has_y) {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= inv * wp[c][i];
+        rows.store4(rows.template out<T>(a.y, row), c, r[c]);
+      }
+    }
+  }
+  rows.end();
+}
+
+// The values are taken from the source twice, before and after the row's sums, instead of being held in registers.
+// ALL: h, dr, dy, post and a gate per channel or none, as compile-time facts; without it each part is looked up.
+template <typename T, typename R, typename W, Mode MODE, bool ALL>
+__global__ void __launch_bounds__(ROW_THREADS, 1) backward_rows_kernel(const __grid_constant__ RowParams p) {
+  const bshmem_norm_args_t& a = p.a;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float sums[2][SUM_ROWS][3];
+  Rows<MODE> rows(p, smem, true);
+  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_dr = ALL || a.dr, has_dy = ALL || a.dy;
+  const float inv_h = 1.f / (float)a.H;
+  float u[ROW_CH][4], wp[ROW_CH][4], acc_s[ROW_CH][4], acc_p[ROW_CH][4];
+#pragma unroll
+  for (int c = 0; c < ROW_CH; ++c) {
+    if (has_h) rows.template load_u<W>(u[c], c, has_post);
+    if (has_dy) rows.template load4<W>(wp[c], rows.template mine<W>(a.pre), c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      wp[c][i] = has_dy ? wp[c][i] + a.weight_offset : 0.f;
+      if (!has_h) u[c][i] = 0.f;
+      acc_s[c][i] = acc_p[c][i] = 0.f;
+    }
+  }
+  int buf = 0;
+  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+    const float tg = token ? load1<W>(a.gate, row) : 1.f;
+    const float s1 = has_h && has_post ? a.stat[row] : 1.f, s2 = has_dy ? a.stat[a.T + row] : 0.f;
+    const RowSource src = rows.wait(row);
+    // hh = hhat, ge = the row's gate, rh = rhat, dy, g = dr + s2 dy pre of four columns
+    auto values = [&](int c, float* hh, float* ge, float* rh, float* dy, float* g) {
+      rows.template load4<R>(rh, src.residual, c);
+      if (has_h) rows.template load4<T>(hh, src.h, c);
+      if (full) rows.template load4<W>(ge, src.gate, c);
+      if (has_dr) rows.template load4<R>(g, src.dr, c);
+      if (has_dy) rows.template load4<T>(dy, src.dy, c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!full) ge[i] = tg;
+        hh[i] = has_h ? hh[i] * s1 : 0.f;
+        if (!has_dr) g[i] = 0.f;
+        if (!has_dy) dy[i] = 0.f;
+        rh[i] = s2 * (a.residual_scale * rh[i] + ge[i] * u[c][i] * hh[i]);
+        g[i] += s2 * (dy[i] * wp[c][i]);
+      }
+    };
+    float v[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < ROW_CH; ++c) {
+      float hh[4], ge[4], rh[4], dy[4], g[4];
+      values(c, hh, ge, rh, dy, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float q = u[c][i] * hh[i] * (full ? ge[i] : 1.f);   // without a gate per token: see c2
+        v[0] += dy[i] * wp[c][i] * rh[i];
+        v[1] += q * g[i];
+        v[2] += q * rh[i];
+      }
+    }
+    rows.sum(v, sums[buf]);
+    buf ^= 1;
+    rows.refill(row, 1);  // the barrier of the sum: every thread is done with the row before
+    const float c1 = s2 * v[0] * inv_h, qg = v[1] - c1 * v[2], c2 = has_post ? qg * tg * inv_h : 0.f;
+    if (token && a.dgate && rows.tid == 0) store1<W>(a.dgate, row, qg);
+#pragma unroll
+    for (int c = 0; c < ROW_CH; ++c) {
+      float hh[4], ge[4], rh[4], dy[4], g[4];
+      values(c, hh, ge, rh, dy, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        g[i] -= c1 * rh[i];
+        acc_p[c][i] += dy[i] * rh[i];
+        acc_s[c][i] += ge[i] * g[i] * hh[i];
+        dy[i] = a.residual_scale * g[i];
+      }
+      if (a.dresidual) rows.store4(rows.template out<R>(a.dresidual, row), c, dy);
+      if (a.dh) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dy[i] = s1 * (ge[i] * u[c][i] * g[i] - hh[i] * c2);
+        rows.store4(rows.template out<T>(a.dh, row), c, dy);
+      }
+      if (full && a.dgate) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dy[i] = g[i] * u[c][i] * hh[i];
+        rows.store4(rows.template out<W>(a.dgate, row), c, dy);
+      }
+    }
+    rows.next();
+  }
+  if (a.partials) {
+    float* part = a.partials + (size_t)(p.half ? blockIdx.x / 2 : blockIdx.x) * 2 * a.H;
+    if (MODE == STAGED || blockDim.x == rows.threads) {
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.store4(part + rows.base, c, acc_s[c]);
+        rows.store4(part + a.H + rows.base, c, acc_p[c]);
+      }
+    } else {  // the warps' sums, in order
+      float* s = (float*)smem;  // [warps][2][H]
+      const int warps = blockDim.x >> 5;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        rows.store4(s + (threadIdx.x >> 5) * 2 * a.H, c, acc_s[c]);
+        rows.store4(s + ((threadIdx.x >> 5) * 2 + 1) * a.H, c, acc_p[c]);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * a.H; i += blockDim.x) {
+        float v = 0.f;
+        for (int k = 0; k < warps; ++k) v += s[k * 2 * a.H + i];
+        part[i] = v;
+      }
+    }
+  }
+  rows.end();
+}
+
+// Sums of the CTAs' parts, in order: S (dpost and the channel gate's gradient) and dpre.
+constexpr int SLICES = 32;
+template <typename W>
+static __global__ void __launch_bounds__(32 * SLICES) column_sum_kernel(const __grid_constant__ bshmem_norm_args_t a, int parts) {
+  const int i = blockIdx.x * 32 + threadIdx.x;
+  const bool pre = blockIdx.y != 0, channel = a.gate_mode == BSHMEM_NORM_GATE_CHANNEL;
+  if (pre ? !a.dpre : !a.dpost && !(a.dgate && channel)) return;
+  __shared__ float s[SLICES][33];
+  float v = 0.f;
+  if (i < a.H) {
+#pragma unroll 4
+    for (int k = threadIdx.y; k < parts; k += SLICES) v += a.partials[((size_t)k * 2 + pre) * a.H + i];
+  }
+  s[threadIdx.y][threadIdx.x] = v;
+  __syncthreads();
+  if (threadIdx.y || i >= a.H) return;
+#pragma unroll
+  for (int k = 1; k < SLICES; ++k) v += s[k][threadIdx.x];
+  if (pre) {
+    store1<W>(a.dpre, i, v);
+    return;
+  }
+  if (a.dpost) store1<W>(a.dpost, i, a.branch_scale * v * (channel ? load1<W>(a.gate, i) : 1.f));
+  if (a.dgate && channel) store1<W>(a.dgate, i, a.branch_scale * v * (a.post ? load1<W>(a.post, i) + a.weight_offset : 1.f));
+}
+
+// ------------------------------------------------------------------ host
+static inline bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Rows and parameters may be read and written 16 bytes at a time.
+static inline bool vectors(const bshmem_norm_args_t* a) {
+  if (a->H % 8) return false;
+  const void* ptrs[] = {a->h, a->residual, a->post, a->pre, a->gate, a->r, a->y, a->dr, a->dy, a->dh, a->dresidual, a->dgate};
+  for (const void* q : ptrs)
+    if (!aligned(q)) {
+      if (q == a->gate || q == a->dgate) {
+        if (a->gate_mode == BSHMEM_NORM_GATE_TOKEN) continue;
+      }
+      return false;
+    }
+  return !((a->h_stride | a->res_stride | a->dr_stride | a->dy_stride) & 7) && (a->gate_mode != BSHMEM_NORM_GATE_FULL || !(a->gate_stride & 7));
+}
+
+static inline int sm_count() {
+  int device = 0, sms = 0;
+  cudaGetDevice(&device);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  return sms > 0 ? sms : 1;
+}
+
+// How a call runs.
+struct RowPlan {
+  Mode mode;
+  int ctas, block, threads, half, stages, stage_bytes, smem, parts;
+};
+static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward, bool vec) {
+  RowPlan r = {vec ? VECTOR : SCALAR, 0, 0, 0, 0, 0, 0, 0, 0};
+  if (a->H > CTA_COLS) r.half = ((a->H + 1) / 2 + 7) / 8 * 8;
+  const int sms = sm_count();
+  const int cols = r.half ? r.half : a->H;
+  r.threads = (cols + ROW_COLS * 32 - 1) / (ROW_COLS * 32) * 32;
+  if (a->H <= WARP_COLS) {
+    r.block = 32 * WARP_GROUPS;
+    r.smem = backward && a->partials ? WARP_GROUPS * 2 * a->H * 4 : 0;
+  } else {
+    r.block = r.threads;
+  }
+  int per_sm = ROW_THREADS / r.block;
+  if (vec && a->H > WARP_COLS && a->T > sms * per_sm / (r.half ? 2 : 1)) {
+    // Two stages at least; rather fewer CTAs of an SM than none.
+    r.stage_bytes = stage_rows(*a, cols, backward).bytes;
+    for (int n = per_sm < 6 ? per_sm : 6; n > 0; --n) {
+      const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
+      if (fit < 2) continue;
+      r.mode = STAGED;
+      r.stages = fit < MAX_STAGES ? fit : MAX_STAGES;
+      r.smem = r.stages * r.stage_bytes + MAX_STAGES * 8 + 16;
+      per_sm = n;
+      break;
+    }
+  }
+  const int groups = r.block / r.threads, want = (int)(((int64_t)a->T + groups - 1) / groups), most = sms * per_sm / (r.half ? 2 : 1);
+  r.parts = want < most ? want : most;
+  r.ctas = r.parts * (r.half ? 2 : 1);
+  return r;
+}
+static inline bool plain_gate(const bshmem_norm_args_t& a) { return a.gate_mode == BSHMEM_NORM_GATE_NONE || a.gate_mode == BSHMEM_NORM_GATE_CHANNEL; }
+// Raises a kernel's shared-memory limit to what it may take.
+static inline bool reserve_smem(const void* kernel, int bytes) {
+  return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+template <typename P>
+static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, cudaStream_t stream) {
+  if (!reserve_smem((const void*)kernel, plan.smem)) return BSHMEM_NORM_ERR_DRIVER;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(plan.block);
+  cfg.dynamicSmemBytes = plan.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = plan.half ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+}
+
+template <typename T, typename R, typename W>
+static int launch_forward(const bshmem_norm_args_t* a, cudaStream_t stream) {
+  const RowPlan plan = row_plan(a, false, vectors(a));
+  const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
+  const bool all = plain_gate(*a) && a->post && a->y;
+  void (*const kernel)(RowParams) = plan.mode == STAGED ? (all ? forward_rows_kernel<T, R, W, STAGED, true> : forward_rows_kernel<T, R, W, STAGED, false>)
+                                    : plan.mode == VECTOR ? (all ? forward_rows_kernel<T, R, W, VECTOR, true> : forward_rows_kernel<T, R, W, VECTOR, false>)
+                                                          : forward_rows_kernel<T, R, W, SCALAR, false>;
+  return launch(kernel, plan, p, stream);
+}
+
+template <typename T, typename R, typename W>
+static int launch_backward(const bshmem_norm_args_t* a, cudaStream_t stream) {
+  const RowPlan plan = row_plan(a, true, vectors(a));
+  const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
+  const bool all = plain_gate(*a) && a->post && a->dr && a->dy;
+  void (*const kernel)(RowParams) = plan.mode == STAGED ? (all ? backward_rows_kernel<T, R, W, STAGED, true> : backward_rows_kernel<T, R, W, STAGED, false>)
+                                    : plan.mode == VECTOR ? (all ? backward_rows_kernel<T, R, W, VECTOR, true> : backward_rows_kernel<T, R, W, VECTOR, false>)
+                                                          : backward_rows_kernel<T, R, W, SCALAR, false>;
+  const int st = launch(kernel, plan, p, stream);
+  if (st || !a->partials) return st;
+  column_sum_kernel<W><<<dim3((a->H + 31) / 32, 2), dim3(32, SLICES), 0, stream>>>(*a, plan.parts);
+  return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+}
+
+// A call whose rows are of type T: by the types of the residual and of the parameters.
+template <typename T>
+static int run(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream) {
+  const bool r = a->res_type == a->type, w = a->wt_type == a->type;
+  if constexpr (sizeof(T) == 4) {
+    return backward ? launch_backward<T, T, T>(a, stream) : launch_forward<T, T, T>(a, stream);
+  } else if (backward) {
+    return r ? (w ? launch_backward<T, T, T>(a, stream) : launch_backward<T, T, float>(a, stream)) : w ? launch_backward<T, float, T>(a, stream) : launch_backward<T, float, float>(a, stream);
+  } else {
+    return r ? (w ? launch_forward<T, T, T>(a, stream) : launch_forward<T, T, float>(a, stream)) : w ? launch_forward<T, float, T>(a, stream) : launch_forward<T, float, float>(a, stream);
+  }
+}
+int run_bf16(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream);
+int run_f16(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream);
+int run_f32(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream);
+
+}  // namespace norms
+}  // namespace bshmem
