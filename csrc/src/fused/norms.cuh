@@ -24,6 +24,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/bshmem/norms.h"
 #include "../../include/bshmem/tcgen05.cuh"
 
@@ -58,7 +60,15 @@ __device__ __forceinline__ void store1(void* p, size_t i, float v) {
 }
 
 enum Mode { STAGED, VECTOR, SCALAR };
+// What a kernel knows of its calls at compile time, besides a multiple of 512 columns (every warp has all of its own):
+//   BOTH  h, both norms, a gate per channel or none (backward: both gradients)
+//   IN    no h: the norm of a row alone      OUT  h, the norm after it, no norm that follows, any gate but [T][H]
+//   ANY   nothing; each part is looked up, and columns are guarded
+enum Kind { ANY, BOTH, IN, OUT };
+// CTAs of 512 threads an SM: two sums and two parameters a column need 128 registers a thread, one of each 64.
+constexpr int ctas_per_sm(Kind kind) { return kind == IN || kind == OUT ? 2 : 1; }
 constexpr int ROW_CH = 4, ROW_COLS = 4 * ROW_CH, CTA_COLS = 8192, ROW_THREADS = CTA_COLS / ROW_COLS, MAX_STAGES = 8;
+constexpr int MAX_CTAS_PER_SM = 8;
 constexpr int WARP_COLS = 32 * ROW_COLS, WARP_GROUPS = 8;   // rows of a warp each
 constexpr int STAGE_SMEM = 216 * 1024;  // of an SM, shared by its CTAs
 constexpr int SUM_ROWS = 17;            // 16 warps, and the other CTA of a pair
@@ -95,12 +105,14 @@ __host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_
   return r;
 }
 
+// Rows that are absent are read from the residual's place (it is at least as long) and their values dropped, which takes no branch.
 // This CTA's columns of a row's inputs, wherever they are.
 struct RowSource {
   const uint8_t *h, *residual, *dr, *dy, *gate;
 };
 
-template <Mode MODE>
+// EVEN: whole warps of columns, nothing to guard.
+template <Mode MODE, bool EVEN>
 struct Rows {
   const RowParams& p;
   uint8_t* data = nullptr;
@@ -118,24 +130,29 @@ struct Rows {
     const size_t ts = type_bytes(a.type), rs = type_bytes(a.res_type), ws = type_bytes(a.wt_type);
     RowSource g;
     g.residual = (const uint8_t*)a.residual + (row * a.res_stride + base) * rs;
-    g.h = (const uint8_t*)a.h + (row * a.h_stride + base) * ts;
-    g.dr = (const uint8_t*)a.dr + (row * a.dr_stride + base) * rs;
-    g.dy = (const uint8_t*)a.dy + (row * a.dy_stride + base) * ts;
+    g.h = a.h ? (const uint8_t*)a.h + (row * a.h_stride + base) * ts : g.residual;
+    g.dr = a.dr ? (const uint8_t*)a.dr + (row * a.dr_stride + base) * rs : g.residual;
+    g.dy = a.dy ? (const uint8_t*)a.dy + (row * a.dy_stride + base) * ts : g.residual;
     g.gate = (const uint8_t*)a.gate + (row * a.gate_stride + base) * ws;
     return g;
   }
-  // Starts the copy of a row into a stage that nobody reads any more.  One thread.
+  // Starts the copy of a row into a stage that nobody reads any more.  One thread of each of the first five warps (of all, if there are
+  // fewer), so that no warp is held up by all the copies.
   __device__ __forceinline__ void load(size_t row, int to) const {
     const RowSource g = global(row);
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    auto mine = [&](int copy) { return copy % warps == warp; };
     const int ts = type_bytes(p.a.type), rs = type_bytes(p.a.res_type), ws = type_bytes(p.a.wt_type);
     uint8_t* dst = data + (size_t)to * p.stage_bytes;
     uint64_t* bar = &full[to];
-    sm100::mbar_expect_tx(bar, at.bytes);
-    sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
-    if (at.h >= 0) sm100::bulk_load(dst + at.h, g.h, cols * ts, bar);
-    if (at.dr >= 0) sm100::bulk_load(dst + at.dr, g.dr, cols * rs, bar);
-    if (at.dy >= 0) sm100::bulk_load(dst + at.dy, g.dy, cols * ts, bar);
-    if (at.gate >= 0) sm100::bulk_load(dst + at.gate, g.gate, cols * ws, bar);
+    if (mine(0)) {
+      sm100::mbar_expect_tx(bar, at.bytes);  // the phase ends when this has arrived and the bytes of all copies are in
+      sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
+    }
+    if (at.h >= 0 && mine(1)) sm100::bulk_load(dst + at.h, g.h, cols * ts, bar);
+    if (at.dr >= 0 && mine(2)) sm100::bulk_load(dst + at.dr, g.dr, cols * rs, bar);
+    if (at.dy >= 0 && mine(3)) sm100::bulk_load(dst + at.dy, g.dy, cols * ts, bar);
+    if (at.gate >= 0 && mine(4)) sm100::bulk_load(dst + at.gate, g.gate, cols * ws, bar);
   }
   __device__ __forceinline__ Rows(const RowParams& params, uint8_t* smem, bool backward) : p(params) {
     const int pair = p.half ? 2 : 1, rank = p.half ? blockIdx.x & 1 : 0, groups = blockDim.x / p.threads;
@@ -155,10 +172,11 @@ struct Rows {
         for (int i = 0; i < p.stages; ++i) sm100::mbar_init(&full[i], 1);
         sm100::mbar_fence_init();
         sm100::fence_proxy_async_smem();
-        for (int i = 0; i < p.stages; ++i)
-          if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
       }
       __syncthreads();
+      if ((threadIdx.x & 31) == 0)
+        for (int i = 0; i < p.stages; ++i)
+          if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
     }
     if (p.half) sm100::cluster_sync_all();  // the other CTA runs: its shared memory may be written
   }
@@ -166,7 +184,7 @@ struct Rows {
     if constexpr (MODE == STAGED) {
       sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
       const uint8_t* s = data + (size_t)stage * p.stage_bytes;
-      return {s + at.h, s + at.residual, s + at.dr, s + at.dy, s + at.gate};
+      return {s + max(at.h, 0), s + at.residual, s + max(at.dr, 0), s + max(at.dy, 0), s + at.gate};
     } else {
       return global(row);
     }
@@ -176,7 +194,7 @@ struct Rows {
   __device__ __forceinline__ void refill(size_t row, int behind) const {
     if constexpr (MODE == STAGED) {
       const size_t next = row + (size_t)(p.stages - behind) * step;
-      if (threadIdx.x == 0 && row >= first + behind * step && next < (size_t)p.a.T) load(next, stage >= behind ? stage - behind : p.stages - 1);
+      if ((threadIdx.x & 31) == 0 && row >= first + behind * step && next < (size_t)p.a.T) load(next, stage >= behind ? stage - behind : p.stages - 1);
     }
   }
   __device__ __forceinline__ void next() {
@@ -208,13 +226,13 @@ struct Rows {
     if constexpr (MODE == SCALAR) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        f[i] = col(c, i) < cols ? to_f<T>(((const T*)row)[col(c, i)]) : 0.f;
+        f[i] = EVEN || col(c, i) < cols ? to_f<T>(((const T*)row)[col(c, i)]) : 0.f;
       }
     } else {
       const int at = col(c, 0);
       alignas(16) T raw[4];
-      if constexpr (sizeof(T) == 4) *(uint4*)raw = at < cols ? *(const uint4*)((const T*)row + at) : make_uint4(0u, 0u, 0u, 0u);
-      else *(uint2*)raw = at < cols ? *(const uint2*)((const T*)row + at) : make_uint2(0u, 0u);
+      if constexpr (sizeof(T) == 4) *(uint4*)raw = EVEN || at < cols ? *(const uint4*)((const T*)row + at) : make_uint4(0u, 0u, 0u, 0u);
+      else *(uint2*)raw = EVEN || at < cols ? *(const uint2*)((const T*)row + at) : make_uint2(0u, 0u);
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = to_f<T>(raw[i]);
     }
@@ -228,7 +246,7 @@ struct Rows {
       }
     } else {
       const int at = col(c, 0);
-      if (at >= cols) return;
+      if (!EVEN && at >= cols) return;
       alignas(16) T raw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[i] = from_f<T>(f[i]);
@@ -290,15 +308,14 @@ struct Rows {
   }
 };
 
-// ALL: h, both norms, and a gate per channel or none, as compile-time facts; without it each part is looked up.
-template <typename T, typename R, typename W, Mode MODE, bool ALL>
-__global__ void __launch_bounds__(ROW_THREADS, 1) forward_rows_kernel(const __grid_constant__ RowParams p) {
+template <typename T, typename R, typename W, Mode MODE, Kind KIND>
+__global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][1];
-  Rows<MODE> rows(p, smem, false);
-  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
-  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_y = ALL || a.y;
+  Rows<MODE, KIND != ANY> rows(p, smem, false);
+  const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN, has_y = KIND == ANY ? a.y != nullptr : KIND != OUT;
   const float inv_h = 1.f / (float)a.H;
   float u[ROW_CH][4], wp[ROW_CH][4];
 #pragma unroll
@@ -389,15 +406,15 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) forward_rows_kernel(const __gr
 }
 
 // The values are taken from the source twice, before and after the row's sums, instead of being held in registers.
-// ALL: h, dr, dy, post and a gate per channel or none, as compile-time facts; without it each part is looked up.
-template <typename T, typename R, typename W, Mode MODE, bool ALL>
-__global__ void __launch_bounds__(ROW_THREADS, 1) backward_rows_kernel(const __grid_constant__ RowParams p) {
+template <typename T, typename R, typename W, Mode MODE, Kind KIND>
+__global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][3];
-  Rows<MODE> rows(p, smem, true);
-  const bool token = !ALL && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = !ALL && a.gate_mode == BSHMEM_NORM_GATE_FULL;
-  const bool has_h = ALL || a.h, has_post = ALL || a.post, has_dr = ALL || a.dr, has_dy = ALL || a.dy;
+  Rows<MODE, KIND != ANY> rows(p, smem, true);
+  const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
+  const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN;
+  const bool has_dr = KIND == ANY ? a.dr != nullptr : KIND != IN, has_dy = KIND == ANY ? a.dy != nullptr : KIND != OUT;
   const float inv_h = 1.f / (float)a.H;
   float u[ROW_CH][4], wp[ROW_CH][4], acc_s[ROW_CH][4], acc_p[ROW_CH][4];
 #pragma unroll
@@ -411,68 +428,77 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) backward_rows_kernel(const __g
       acc_s[c][i] = acc_p[c][i] = 0.f;
     }
   }
+  // The row's scalars, read one row ahead.
+  float tg = 1.f, s1 = 1.f, s2 = 0.f, tg_next = 1.f, s1_next = 1.f, s2_next = 0.f;
+  auto scalars = [&](size_t row) {
+    if (row >= (size_t)a.T) return;
+    if (token) tg_next = load1<W>(a.gate, row);
+    if (has_h && has_post) s1_next = a.stat[row];
+    if (has_dy) s2_next = a.stat[a.T + row];
+  };
+  scalars(rows.first);
   int buf = 0;
   for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
-    const float tg = token ? load1<W>(a.gate, row) : 1.f;
-    const float s1 = has_h && has_post ? a.stat[row] : 1.f, s2 = has_dy ? a.stat[a.T + row] : 0.f;
+    tg = tg_next, s1 = s1_next, s2 = s2_next;
+    scalars(row + rows.step);
     const RowSource src = rows.wait(row);
-    // hh = hhat, ge = the row's gate, rh = rhat, dy, g = dr + s2 dy pre of four columns
-    auto values = [&](int c, float* hh, float* ge, float* rh, float* dy, float* g) {
-      rows.template load4<R>(rh, src.residual, c);
-      if (has_h) rows.template load4<T>(hh, src.h, c);
+    // h, ge = the row's gate, q = gate u hhat, r, dy, g = dr + s2 dy pre of four columns
+    auto values = [&](int c, float* h, float* ge, float* q, float* r, float* dy, float* g) {
+      rows.template load4<R>(r, src.residual, c);
+      if (KIND != IN) rows.template load4<T>(h, src.h, c);
+      if (KIND != IN) rows.template load4<R>(g, src.dr, c);
+      if (KIND != OUT) rows.template load4<T>(dy, src.dy, c);
       if (full) rows.template load4<W>(ge, src.gate, c);
-      if (has_dr) rows.template load4<R>(g, src.dr, c);
-      if (has_dy) rows.template load4<T>(dy, src.dy, c);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (!full) ge[i] = tg;
-        hh[i] = has_h ? hh[i] * s1 : 0.f;
+        if (!has_h) h[i] = 0.f;
         if (!has_dr) g[i] = 0.f;
         if (!has_dy) dy[i] = 0.f;
-        rh[i] = s2 * (a.residual_scale * rh[i] + ge[i] * u[c][i] * hh[i]);
+        q[i] = s1 * (u[c][i] * h[i]);
+        if (full || token) q[i] *= ge[i];
+        r[i] = a.residual_scale * r[i] + q[i];
         g[i] += s2 * (dy[i] * wp[c][i]);
       }
     };
     float v[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < ROW_CH; ++c) {
-      float hh[4], ge[4], rh[4], dy[4], g[4];
-      values(c, hh, ge, rh, dy, g);
+      float h[4], ge[4], q[4], r[4], dy[4], g[4];
+      values(c, h, ge, q, r, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float q = u[c][i] * hh[i] * (full ? ge[i] : 1.f);   // without a gate per token: see c2
-        v[0] += dy[i] * wp[c][i] * rh[i];
-        v[1] += q * g[i];
-        v[2] += q * rh[i];
+        if (token) q[i] = s1 * (u[c][i] * h[i]);   // without the gate: see c2
+        v[0] += dy[i] * wp[c][i] * r[i];
+        v[1] += q[i] * g[i];
+        v[2] += q[i] * r[i];
       }
     }
     rows.sum(v, sums[buf]);
     buf ^= 1;
     rows.refill(row, 1);  // the barrier of the sum: every thread is done with the row before
-    const float c1 = s2 * v[0] * inv_h, qg = v[1] - c1 * v[2], c2 = has_post ? qg * tg * inv_h : 0.f;
+    const float c1 = ((s2 * v[0]) * inv_h * s2) * s2;              // c1 s2^2, as rhat = s2 r; in this order it does not overflow
+    const float qg = v[1] - c1 * v[2], c2 = has_post ? s1 * qg * tg * inv_h : 0.f;
     if (token && a.dgate && rows.tid == 0) store1<W>(a.dgate, row, qg);
 #pragma unroll
     for (int c = 0; c < ROW_CH; ++c) {
-      float hh[4], ge[4], rh[4], dy[4], g[4];
-      values(c, hh, ge, rh, dy, g);
+      float h[4], ge[4], q[4], r[4], dy[4], g[4];
+      values(c, h, ge, q, r, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        g[i] -= c1 * rh[i];
-        acc_p[c][i] += dy[i] * rh[i];
-        acc_s[c][i] += ge[i] * g[i] * hh[i];
+        g[i] -= c1 * r[i];
+        acc_p[c][i] += (s2 * dy[i]) * r[i];
+        float gs = s1 * g[i];
+        if (full || token) gs *= ge[i];
+        acc_s[c][i] += gs * h[i];
         dy[i] = a.residual_scale * g[i];
+        q[i] = s1 * (g[i] * u[c][i]);
+        r[i] = (full || token ? ge[i] * q[i] : q[i]) - (s1 * c2) * h[i];
+        q[i] *= h[i];
       }
       if (a.dresidual) rows.store4(rows.template out<R>(a.dresidual, row), c, dy);
-      if (a.dh) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dy[i] = s1 * (ge[i] * u[c][i] * g[i] - hh[i] * c2);
-        rows.store4(rows.template out<T>(a.dh, row), c, dy);
-      }
-      if (full && a.dgate) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dy[i] = g[i] * u[c][i] * hh[i];
-        rows.store4(rows.template out<W>(a.dgate, row), c, dy);
-      }
+      if (a.dh) rows.store4(rows.template out<T>(a.dh, row), c, r);
+      if (full && a.dgate) rows.store4(rows.template out<W>(a.dgate, row), c, q);
     }
     rows.next();
   }
@@ -556,12 +582,20 @@ static inline int sm_count() {
 // How a call runs.
 struct RowPlan {
   Mode mode;
+  Kind kind;
   int ctas, block, threads, half, stages, stage_bytes, smem, parts;
 };
-static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward, bool vec) {
-  RowPlan r = {vec ? VECTOR : SCALAR, 0, 0, 0, 0, 0, 0, 0, 0};
+static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
+  const bool vec = vectors(a);
+  RowPlan r = {vec ? VECTOR : SCALAR, ANY, 0, 0, 0, 0, 0, 0, 0, 0};
   if (a->H > CTA_COLS) r.half = ((a->H + 1) / 2 + 7) / 8 * 8;
-  const int sms = sm_count();
+  const int sms = sm_count(), pair = r.half ? 2 : 1;
+  const bool after = backward ? a->dr != nullptr : a->r != nullptr, before = backward ? a->dy != nullptr : a->y != nullptr;
+  if (vec && a->H % (WARP_COLS * pair) == 0) {
+    if (!a->h && before && !(backward && a->dr)) r.kind = IN;
+    else if (a->h && a->post && after && !before && a->gate_mode != BSHMEM_NORM_GATE_FULL) r.kind = OUT;
+    else if (a->h && a->post && after && before && (a->gate_mode == BSHMEM_NORM_GATE_NONE || a->gate_mode == BSHMEM_NORM_GATE_CHANNEL)) r.kind = BOTH;
+  }
   const int cols = r.half ? r.half : a->H;
   r.threads = (cols + ROW_COLS * 32 - 1) / (ROW_COLS * 32) * 32;
   if (a->H <= WARP_COLS) {
@@ -570,11 +604,12 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward, bool 
   } else {
     r.block = r.threads;
   }
-  int per_sm = ROW_THREADS / r.block;
-  if (vec && a->H > WARP_COLS && a->T > sms * per_sm / (r.half ? 2 : 1)) {
+  int per_sm = ctas_per_sm(r.kind) * ROW_THREADS / r.block;
+  if (per_sm > MAX_CTAS_PER_SM) per_sm = MAX_CTAS_PER_SM;
+  if (vec && a->H > WARP_COLS && a->T > sms * per_sm / pair) {
     // Two stages at least; rather fewer CTAs of an SM than none.
     r.stage_bytes = stage_rows(*a, cols, backward).bytes;
-    for (int n = per_sm < 6 ? per_sm : 6; n > 0; --n) {
+    for (int n = per_sm; n > 0; --n) {
       const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
       if (fit < 2) continue;
       r.mode = STAGED;
@@ -584,12 +619,11 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward, bool 
       break;
     }
   }
-  const int groups = r.block / r.threads, want = (int)(((int64_t)a->T + groups - 1) / groups), most = sms * per_sm / (r.half ? 2 : 1);
+  const int groups = r.block / r.threads, want = (int)(((int64_t)a->T + groups - 1) / groups), most = sms * per_sm / pair;
   r.parts = want < most ? want : most;
-  r.ctas = r.parts * (r.half ? 2 : 1);
+  r.ctas = r.parts * pair;
   return r;
 }
-static inline bool plain_gate(const bshmem_norm_args_t& a) { return a.gate_mode == BSHMEM_NORM_GATE_NONE || a.gate_mode == BSHMEM_NORM_GATE_CHANNEL; }
 // Raises a kernel's shared-memory limit to what it may take.
 static inline bool reserve_smem(const void* kernel, int bytes) {
   return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
@@ -611,42 +645,41 @@ static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, cudaStream
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
 }
 
-template <typename T, typename R, typename W>
-static int launch_forward(const bshmem_norm_args_t* a, cudaStream_t stream) {
-  const RowPlan plan = row_plan(a, false, vectors(a));
-  const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
-  const bool all = plain_gate(*a) && a->post && a->y;
-  void (*const kernel)(RowParams) = plan.mode == STAGED ? (all ? forward_rows_kernel<T, R, W, STAGED, true> : forward_rows_kernel<T, R, W, STAGED, false>)
-                                    : plan.mode == VECTOR ? (all ? forward_rows_kernel<T, R, W, VECTOR, true> : forward_rows_kernel<T, R, W, VECTOR, false>)
-                                                          : forward_rows_kernel<T, R, W, SCALAR, false>;
-  return launch(kernel, plan, p, stream);
+// The kernel of a plan.  A row alone (IN) has one type.
+template <typename T, typename R, typename W, bool BACKWARD, Mode MODE, Kind KIND>
+constexpr auto kernel_of() {
+  if constexpr (BACKWARD) return backward_rows_kernel<T, R, W, MODE, KIND>;
+  else return forward_rows_kernel<T, R, W, MODE, KIND>;
 }
-
-template <typename T, typename R, typename W>
-static int launch_backward(const bshmem_norm_args_t* a, cudaStream_t stream) {
-  const RowPlan plan = row_plan(a, true, vectors(a));
+template <typename T, typename R, typename W, bool BACKWARD, Mode MODE>
+static void (*by_kind(Kind kind))(RowParams) {
+  if constexpr (std::is_same<T, R>::value)
+    if (kind == IN) return kernel_of<T, R, W, BACKWARD, MODE, IN>();
+  return kind == BOTH ? kernel_of<T, R, W, BACKWARD, MODE, BOTH>() : kind == OUT ? kernel_of<T, R, W, BACKWARD, MODE, OUT>() : kernel_of<T, R, W, BACKWARD, MODE, ANY>();
+}
+template <typename T, typename R, typename W, bool BACKWARD>
+static int launch_rows(const bshmem_norm_args_t* a, cudaStream_t stream) {
+  const RowPlan plan = row_plan(a, BACKWARD);
   const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
-  const bool all = plain_gate(*a) && a->post && a->dr && a->dy;
-  void (*const kernel)(RowParams) = plan.mode == STAGED ? (all ? backward_rows_kernel<T, R, W, STAGED, true> : backward_rows_kernel<T, R, W, STAGED, false>)
-                                    : plan.mode == VECTOR ? (all ? backward_rows_kernel<T, R, W, VECTOR, true> : backward_rows_kernel<T, R, W, VECTOR, false>)
-                                                          : backward_rows_kernel<T, R, W, SCALAR, false>;
+  void (*const kernel)(RowParams) = plan.mode == STAGED ? by_kind<T, R, W, BACKWARD, STAGED>(plan.kind) : plan.mode == VECTOR ? by_kind<T, R, W, BACKWARD, VECTOR>(plan.kind)
+                                                                                                        : kernel_of<T, R, W, BACKWARD, SCALAR, ANY>();
   const int st = launch(kernel, plan, p, stream);
-  if (st || !a->partials) return st;
+  if (st || !BACKWARD || !a->partials) return st;
   column_sum_kernel<W><<<dim3((a->H + 31) / 32, 2), dim3(32, SLICES), 0, stream>>>(*a, plan.parts);
   return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+}
+template <typename T, typename R, typename W>
+static int launch_either(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream) {
+  return backward ? launch_rows<T, R, W, true>(a, stream) : launch_rows<T, R, W, false>(a, stream);
 }
 
 // A call whose rows are of type T: by the types of the residual and of the parameters.
 template <typename T>
 static int run(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream) {
   const bool r = a->res_type == a->type, w = a->wt_type == a->type;
-  if constexpr (sizeof(T) == 4) {
-    return backward ? launch_backward<T, T, T>(a, stream) : launch_forward<T, T, T>(a, stream);
-  } else if (backward) {
-    return r ? (w ? launch_backward<T, T, T>(a, stream) : launch_backward<T, T, float>(a, stream)) : w ? launch_backward<T, float, T>(a, stream) : launch_backward<T, float, float>(a, stream);
-  } else {
-    return r ? (w ? launch_forward<T, T, T>(a, stream) : launch_forward<T, T, float>(a, stream)) : w ? launch_forward<T, float, T>(a, stream) : launch_forward<T, float, float>(a, stream);
-  }
+  if constexpr (sizeof(T) == 4) return launch_either<T, T, T>(a, backward, stream);
+  else if (r) return w ? launch_either<T, T, T>(a, backward, stream) : launch_either<T, T, float>(a, backward, stream);
+  else return w ? launch_either<T, float, T>(a, backward, stream) : launch_either<T, float, float>(a, backward, stream);
 }
 int run_bf16(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream);
 int run_f16(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream);
