@@ -87,7 +87,7 @@ struct StageRows {
   int bytes;
 };
 __host__ __device__ __forceinline__ int type_bytes(int t) { return t == BSHMEM_NORM_F32 ? 4 : 2; }
-__host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_t& a, int cols, bool backward) {
+__host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_t& a, int cols, bool backward, Kind kind) {
   StageRows r;
   const int t = cols * type_bytes(a.type), rt = cols * type_bytes(a.res_type), wt = cols * type_bytes(a.wt_type);
   int at = 0;
@@ -96,7 +96,7 @@ __host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_
     if (present) at += bytes;
     return here;
   };
-  r.residual = place(true, rt);
+  r.residual = place(!(backward && kind == OUT), rt);  // of no use to it
   r.h = place(a.h != nullptr, t);
   r.dr = place(backward && a.dr, rt);
   r.dy = place(backward && a.dy, t);
@@ -111,9 +111,9 @@ struct RowSource {
   const uint8_t *h, *residual, *dr, *dy, *gate;
 };
 
-// EVEN: whole warps of columns, nothing to guard.
-template <Mode MODE, bool EVEN>
+template <Mode MODE, Kind KIND>
 struct Rows {
+  static constexpr bool EVEN = KIND != ANY;  // whole warps of columns: nothing to guard
   const RowParams& p;
   uint8_t* data = nullptr;
   uint64_t* full = nullptr;
@@ -147,7 +147,7 @@ struct Rows {
     uint64_t* bar = &full[to];
     if (mine(0)) {
       sm100::mbar_expect_tx(bar, at.bytes);  // the phase ends when this has arrived and the bytes of all copies are in
-      sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
+      if (at.residual >= 0) sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
     }
     if (at.h >= 0 && mine(1)) sm100::bulk_load(dst + at.h, g.h, cols * ts, bar);
     if (at.dr >= 0 && mine(2)) sm100::bulk_load(dst + at.dr, g.dr, cols * rs, bar);
@@ -159,7 +159,7 @@ struct Rows {
     threads = p.threads;
     base = rank ? p.half : 0;
     cols = !p.half ? p.a.H : rank ? p.a.H - p.half : p.half;
-    at = stage_rows(p.a, cols, backward);
+    at = stage_rows(p.a, cols, backward, KIND);
     tid = threadIdx.x % threads;
     first = (size_t)(blockIdx.x / pair) * groups + threadIdx.x / threads;
     step = (size_t)(gridDim.x / pair) * groups;
@@ -184,7 +184,7 @@ struct Rows {
     if constexpr (MODE == STAGED) {
       sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
       const uint8_t* s = data + (size_t)stage * p.stage_bytes;
-      return {s + max(at.h, 0), s + at.residual, s + max(at.dr, 0), s + max(at.dy, 0), s + at.gate};
+      return {s + max(at.h, 0), s + max(at.residual, 0), s + max(at.dr, 0), s + max(at.dy, 0), s + at.gate};
     } else {
       return global(row);
     }
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][1];
-  Rows<MODE, KIND != ANY> rows(p, smem, false);
+  Rows<MODE, KIND> rows(p, smem, false);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
   const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN, has_y = KIND == ANY ? a.y != nullptr : KIND != OUT;
   const float inv_h = 1.f / (float)a.H;
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][3];
-  Rows<MODE, KIND != ANY> rows(p, smem, true);
+  Rows<MODE, KIND> rows(p, smem, true);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
   const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN;
   const bool has_dr = KIND == ANY ? a.dr != nullptr : KIND != IN, has_dy = KIND == ANY ? a.dy != nullptr : KIND != OUT;
@@ -443,8 +443,9 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
     scalars(row + rows.step);
     const RowSource src = rows.wait(row);
     // h, ge = the row's gate, q = gate u hhat, r, dy, g = dr + s2 dy pre of four columns
+    // (products with an absent part are left out where that is known: 0 * x is not 0 for every x)
     auto values = [&](int c, float* h, float* ge, float* q, float* r, float* dy, float* g) {
-      rows.template load4<R>(r, src.residual, c);
+      if (KIND != OUT) rows.template load4<R>(r, src.residual, c);
       if (KIND != IN) rows.template load4<T>(h, src.h, c);
       if (KIND != IN) rows.template load4<R>(g, src.dr, c);
       if (KIND != OUT) rows.template load4<T>(dy, src.dy, c);
@@ -455,10 +456,17 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
         if (!has_h) h[i] = 0.f;
         if (!has_dr) g[i] = 0.f;
         if (!has_dy) dy[i] = 0.f;
-        q[i] = s1 * (u[c][i] * h[i]);
-        if (full || token) q[i] *= ge[i];
-        r[i] = a.residual_scale * r[i] + q[i];
-        g[i] += s2 * (dy[i] * wp[c][i]);
+        if constexpr (KIND != IN) {
+          q[i] = s1 * (u[c][i] * h[i]);
+          if (full || token) q[i] *= ge[i];
+        }
+        if constexpr (KIND == IN) {
+          r[i] *= a.residual_scale;
+          g[i] = s2 * (dy[i] * wp[c][i]);
+        } else if constexpr (KIND != OUT) {
+          r[i] = a.residual_scale * r[i] + q[i];
+          g[i] += s2 * (dy[i] * wp[c][i]);
+        }
       }
     };
     float v[3] = {0.f, 0.f, 0.f};
@@ -468,10 +476,12 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
       values(c, h, ge, q, r, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (token) q[i] = s1 * (u[c][i] * h[i]);   // without the gate: see c2
-        v[0] += dy[i] * wp[c][i] * r[i];
-        v[1] += q[i] * g[i];
-        v[2] += q[i] * r[i];
+        if constexpr (KIND != OUT) v[0] += dy[i] * wp[c][i] * r[i];
+        if constexpr (KIND != IN) {
+          if (token) q[i] = s1 * (u[c][i] * h[i]);   // without the gate: see c2
+          v[1] += q[i] * g[i];
+          if constexpr (KIND != OUT) v[2] += q[i] * r[i];
+        }
       }
     }
     rows.sum(v, sums[buf]);
@@ -486,18 +496,22 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
       values(c, h, ge, q, r, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        g[i] -= c1 * r[i];
-        acc_p[c][i] += (s2 * dy[i]) * r[i];
-        float gs = s1 * g[i];
-        if (full || token) gs *= ge[i];
-        acc_s[c][i] += gs * h[i];
+        if constexpr (KIND != OUT) {
+          g[i] -= c1 * r[i];
+          acc_p[c][i] += (s2 * dy[i]) * r[i];
+        }
         dy[i] = a.residual_scale * g[i];
-        q[i] = s1 * (g[i] * u[c][i]);
-        r[i] = (full || token ? ge[i] * q[i] : q[i]) - (s1 * c2) * h[i];
-        q[i] *= h[i];
+        if constexpr (KIND != IN) {
+          float gs = s1 * g[i];
+          if (full || token) gs *= ge[i];
+          acc_s[c][i] += gs * h[i];
+          q[i] = s1 * (g[i] * u[c][i]);
+          r[i] = (full || token ? ge[i] * q[i] : q[i]) - (s1 * c2) * h[i];
+          q[i] *= h[i];
+        }
       }
       if (a.dresidual) rows.store4(rows.template out<R>(a.dresidual, row), c, dy);
-      if (a.dh) rows.store4(rows.template out<T>(a.dh, row), c, r);
+      if (KIND != IN && a.dh) rows.store4(rows.template out<T>(a.dh, row), c, r);
       if (full && a.dgate) rows.store4(rows.template out<W>(a.dgate, row), c, q);
     }
     rows.next();
@@ -608,7 +622,7 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
   if (per_sm > MAX_CTAS_PER_SM) per_sm = MAX_CTAS_PER_SM;
   if (vec && a->H > WARP_COLS && a->T > sms * per_sm / pair) {
     // Two stages at least; rather fewer CTAs of an SM than none.
-    r.stage_bytes = stage_rows(*a, cols, backward).bytes;
+    r.stage_bytes = stage_rows(*a, cols, backward, r.kind).bytes;
     for (int n = per_sm; n > 0; --n) {
       const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
       if (fit < 2) continue;
