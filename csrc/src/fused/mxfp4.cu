@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/bshmem/mxfp4.h"
 #include "../../include/bshmem/tcgen05.cuh"
@@ -31,78 +32,113 @@ __device__ __forceinline__ __nv_bfloat16 from_f(__nv_bfloat16, float v) { return
 __device__ __forceinline__ __half from_f(__half, float v) { return __float2half_rn(v); }
 
 // ------------------------------------------------------------------ quantisation
-// Sixteen lanes take 128 values of a row (one word of four scales), eight values per lane; the largest exponent of a block of 32 comes from
-// two shuffles over its four lanes.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
-// Bound by memory: 2 or 4 bytes read and 17/32 written per value.
-constexpr int Q_THREADS = 256;
+// Bound by memory: 2 or 4 bytes read and 17/32 written per value, and the reverse.  A warp takes 2048 values of a row, all its loads on
+// their way before the first is used.  The eight rows of a CTA are those whose scales share a 32-byte sector: r, r + 1 and the same
+// 32, 64 and 96 rows on.
+constexpr int Q_THREADS = 256, Q_CHUNK = 2048;
 
+struct RowSlot {
+  int64_t row;
+  int64_t scale;   // offset of the row's scales inside a block of 128 rows
+};
+__device__ __forceinline__ RowSlot row_slot() {
+  const int warp = threadIdx.x >> 5, in32 = (blockIdx.x & 15) * 2 + (warp & 1), quarter = warp >> 1;
+  return {(int64_t)(blockIdx.x >> 4) * 128 + quarter * 32 + in32, in32 * 16 + quarter * 4};
+}
+static dim3 row_grid(int64_t R, int64_t K) { return dim3((unsigned)(row_blocks(R) * 16), (unsigned)((k_blocks(K) * 128 + Q_CHUNK - 1) / Q_CHUNK)); }
+
+// Sixteen lanes take 128 values (one word of four scales), eight values per lane; the largest exponent of a block of 32 comes from two
+// shuffles over its four lanes.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t stride, uint8_t* __restrict__ data,
                                                              uint8_t* __restrict__ scales) {
-  const int64_t KB = k_blocks(K), tasks = row_blocks(R) * 128 * KB;
-  const int part = threadIdx.x & 15;
-  const int64_t step = (int64_t)gridDim.x * (Q_THREADS / 16);
-  // the bound is that of the warp's first half, so that both halves take part in the shuffles
-  for (int64_t first = (int64_t)blockIdx.x * (Q_THREADS / 16) + (threadIdx.x >> 5) * 2; first < tasks; first += step) {
-    const int64_t task = first + ((threadIdx.x >> 4) & 1);
-    const int64_t row = task / KB, kb = task % KB, col = kb * 128 + part * 8;
-    const bool live = task < tasks && row < R && col < K;
-    float f[8];
-    if (live) {
-      const T* src = x + row * stride + col;
+  constexpr int UNROLL = sizeof(T) == 4 ? 4 : 8, WORDS = sizeof(T) * 8 / 16;
+  const RowSlot slot = row_slot();
+  const int half = (threadIdx.x >> 4) & 1, part = threadIdx.x & 15;
+  const int64_t KB = k_blocks(K), first = (int64_t)blockIdx.y * (Q_CHUNK / 128);
+  const bool row_live = slot.row < R;
+  const T* src = x + slot.row * stride + part * 8;
+  uint8_t* dst = data + slot.row * (K / 2) + part * 4;
+  uint8_t* sdst = scales + (slot.row / 128) * KB * SCALE_BLOCK + slot.scale;
+#pragma unroll 1
+  for (int64_t base = first; base < first + Q_CHUNK / 128 && base < KB; base += 2 * UNROLL) {
+    uint4 raw[UNROLL][WORDS];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t kb = base + 2 * u + half;
+      const bool live = row_live && kb * 128 + part * 8 < K;
       if constexpr (VEC) {
-        alignas(16) T raw[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(raw) / 16; ++i) ((uint4*)raw)[i] = ((const uint4*)src)[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f(raw[i]);
+        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? ((const uint4*)(src + kb * 128))[i] : make_uint4(0u, 0u, 0u, 0u);
       } else {
+        T* v = (T*)raw[u];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f(src[i]);
+        for (int i = 0; i < 8; ++i) v[i] = live ? src[kb * 128 + i] : T(0.f);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f;
     }
-    uint32_t amax = 0;  // of the magnitudes' bits, which order like the magnitudes; a NaN is above infinity
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7fffffffu);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
-    const uint32_t code = biased == 255 ? 255 : biased > 2 ? biased - 2 : 0;
-    const float inv = __uint_as_float((254u - (code == 255 ? 254u : code)) << 23);  // 2^(127 - code)
-    uint32_t packed = 0;
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t kb = base + 2 * u + half;
+      float f[8];
+      const T* v = (const T*)raw[u];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      packed |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * i);
-    // the four scales of the sixteen lanes as one word
-    uint32_t word = code << (8 * (part >> 2));
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    if (live) *(uint32_t*)(data + row * (K / 2) + col / 2) = packed;
-    if (part == 0 && task < tasks) *(uint32_t*)(scales + ((row / 128) * KB + kb) * SCALE_BLOCK + (row % 32) * 16 + (row % 128 / 32) * 4) = word;
+      for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
+      uint32_t amax = 0;  // of the magnitudes' bits, which order like the magnitudes; a NaN is above infinity
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7fffffffu);
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
+      const uint32_t code = biased == 255 ? 255 : biased > 2 ? biased - 2 : 0;
+      const float inv = __uint_as_float((254u - (code == 255 ? 254u : code)) << 23);  // 2^(127 - code)
+      uint32_t packed = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        packed |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * i);
+      uint32_t word = code << (8 * (part >> 2));  // the four scales of the sixteen lanes as one word
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      word |= __shfl_xor_sync(0xffffffffu, word, 8);
+      if (row_live && kb * 128 + part * 8 < K) *(uint32_t*)(dst + kb * 64) = packed;
+      if (part == 0 && kb < KB) *(uint32_t*)(sdst + kb * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
+    }
   }
 }
 
+// The reverse; a lane's values fill one 16-byte store: four fp32 or eight 16-bit ones.
 template <typename T>
 __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, int64_t R, int64_t K, T* __restrict__ out) {
-  const int64_t KB = k_blocks(K), per_row = K / 8, n = R * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * Q_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * Q_THREADS) {
-    const int64_t row = i / per_row, col = i % per_row * 8;
-    const uint32_t packed = *(const uint32_t*)(data + row * (K / 2) + col / 2);
-    const uint32_t code = scales[((row / 128) * KB + col / 128) * SCALE_BLOCK + (row % 32) * 16 + (row % 128 / 32) * 4 + col % 128 / BLOCK];
-    const float scale = __uint_as_float(code == 255 ? 0x7fffffffu : code ? code << 23 : 0x00400000u);
-    alignas(16) T raw[8];
+  constexpr int PER_LANE = 16 / sizeof(T), STEP = 32 * PER_LANE, UNROLL = Q_CHUNK / STEP < 8 ? Q_CHUNK / STEP : 8;
+  typedef typename std::conditional<PER_LANE == 8, uint32_t, uint16_t>::type Packed;
+  const RowSlot slot = row_slot();
+  if (slot.row >= R) return;
+  const int lane = threadIdx.x & 31;
+  const uint8_t* ssrc = scales + (slot.row / 128) * k_blocks(K) * SCALE_BLOCK + slot.scale;
+  const int64_t first = (int64_t)blockIdx.y * Q_CHUNK, last = first + Q_CHUNK < K ? first + Q_CHUNK : K;
+#pragma unroll 1
+  for (int64_t base = first + lane * PER_LANE; base < last; base += UNROLL * STEP) {
+    uint32_t packed[UNROLL], code[UNROLL];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t q = packed >> (4 * j) & 15, m = q & 7;
-      // E2M1: 0, 0.5, then 1 + m/2 times a power of two
-      const float mag = m < 2 ? 0.5f * (float)m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1) << 22);
-      raw[j] = from_f(T(), (q & 8 ? -mag : mag) * scale);
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t col = base + u * STEP;
+      if (col >= last) continue;
+      packed[u] = *(const Packed*)(data + (slot.row * K + col) / 2);
+      code[u] = ssrc[col / 128 * SCALE_BLOCK + col % 128 / BLOCK];
     }
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(raw) / 16; ++j) ((uint4*)(out + row * K + col))[j] = ((uint4*)raw)[j];
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t col = base + u * STEP;
+      if (col >= last) continue;
+      const float scale = __uint_as_float(code[u] == 255 ? 0x7fffffffu : code[u] ? code[u] << 23 : 0x00400000u);
+      alignas(16) T raw[PER_LANE];
+#pragma unroll
+      for (int j = 0; j < PER_LANE; ++j) {
+        const uint32_t q = packed[u] >> (4 * j) & 15, m = q & 7;
+        // E2M1: 0, 0.5, then 1 + m/2 times a power of two
+        const float mag = m < 2 ? 0.5f * (float)m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1) << 22);
+        raw[j] = from_f(T(), (q & 8 ? -mag : mag) * scale);
+      }
+      *(uint4*)(out + slot.row * K + col) = *(uint4*)raw;
+    }
   }
 }
 
@@ -271,12 +307,6 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
 }
 
-static int sm_count() {
-  int device = 0, sms = 0;
-  cudaGetDevice(&device);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  return sms > 0 ? sms : 1;
-}
 static int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return BSHMEM_MX_OK;
@@ -286,17 +316,14 @@ static int launched(const char* what) {
 
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
-  const int64_t tasks = row_blocks(R) * 128 * k_blocks(K), want = (tasks + Q_THREADS / 16 - 1) / (Q_THREADS / 16), most = (int64_t)sm_count() * 16;
-  const int grid = (int)(want < most ? want : most);
   const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
-  if (vec) quantize_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
-  else quantize_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
+  if (vec) quantize_kernel<T, true><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
+  else quantize_kernel<T, false><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
   return launched("bshmem_mxfp4_quantize");
 }
 template <typename T>
 static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
-  const int64_t want = (R * (K / 8) + Q_THREADS - 1) / Q_THREADS, most = (int64_t)sm_count() * 16;
-  dequantize_kernel<T><<<(int)(want < most ? want : most), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, K, (T*)out);
+  dequantize_kernel<T><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, K, (T*)out);
   return launched("bshmem_mxfp4_dequantize");
 }
 
@@ -327,7 +354,7 @@ using namespace bshmem::mx;
 
 extern "C" size_t bshmem_mxfp4_scale_bytes(int64_t R, int64_t K) { return R > 0 && K > 0 ? (size_t)(row_blocks(R) * k_blocks(K)) * SCALE_BLOCK : 0; }
 
-static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 0x7fffff00ll ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
+static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 1 << 27 ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
 
 extern "C" int bshmem_mxfp4_quantize(const void* x, int type, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const int st = check_matrix(R, K);
