@@ -1,7 +1,6 @@
 // Microscaled 4-bit floating point: quantisation, reading back, and the block-scaled product on tcgen05.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp4.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -49,56 +48,74 @@ static dim3 row_grid(int64_t R, int64_t K) { return dim3((unsigned)(row_blocks(R
 
 // Sixteen lanes take 128 values (one word of four scales), eight values per lane; the largest exponent of a block of 32 comes from two
 // shuffles over its four lanes.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
+__device__ __forceinline__ uint32_t pack_e2m1(const float* f) {  // eight values, the first in the low four bits; nearest even, saturating
+  uint32_t out;
+  asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}\n"
+      : "=r"(out)
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return out;
+}
+// Largest magnitude of eight values, as the bits of a float (up to the lowest bits of 16-bit types, which do not reach the exponent).
+template <typename T>
+__device__ __forceinline__ uint32_t exponent_bits(const uint4* raw, const float* f) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of a float: the largest of each pair at once
+    const uint32_t m = __vmaxu2(__vmaxu2(raw->x & 0x7fff7fffu, raw->y & 0x7fff7fffu), __vmaxu2(raw->z & 0x7fff7fffu, raw->w & 0x7fff7fffu));
+    return max(m & 0xffff0000u, m << 16);
+  } else {
+    uint32_t m = 0;  // bits order like the magnitudes; a NaN is above infinity
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+    return m;
+  }
+}
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t stride, uint8_t* __restrict__ data,
+__global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int K, int64_t stride, uint8_t* __restrict__ data,
                                                              uint8_t* __restrict__ scales) {
   constexpr int UNROLL = sizeof(T) == 4 ? 4 : 8, WORDS = sizeof(T) * 8 / 16;
   const RowSlot slot = row_slot();
   const int half = (threadIdx.x >> 4) & 1, part = threadIdx.x & 15;
-  const int64_t KB = k_blocks(K), first = (int64_t)blockIdx.y * (Q_CHUNK / 128);
+  const int KB = (int)k_blocks(K), first = (int)blockIdx.y * (Q_CHUNK / 128), last = first + Q_CHUNK / 128 < KB ? first + Q_CHUNK / 128 : KB;
   const bool row_live = slot.row < R;
   const T* src = x + slot.row * stride + part * 8;
   uint8_t* dst = data + slot.row * (K / 2) + part * 4;
   uint8_t* sdst = scales + (slot.row / 128) * KB * SCALE_BLOCK + slot.scale;
 #pragma unroll 1
-  for (int64_t base = first; base < first + Q_CHUNK / 128 && base < KB; base += 2 * UNROLL) {
+  for (int base = first + half; base < last + half; base += 2 * UNROLL) {
+    const int left = row_live ? K - base * 128 - part * 8 : 0;  // values from this lane's first on
     uint4 raw[UNROLL][WORDS];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t kb = base + 2 * u + half;
-      const bool live = row_live && kb * 128 + part * 8 < K;
+      const T* from = src + base * 128 + u * 256;
       if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? ((const uint4*)(src + kb * 128))[i] : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < WORDS; ++i) raw[u][i] = left > u * 256 ? ((const uint4*)from)[i] : make_uint4(0u, 0u, 0u, 0u);
       } else {
         T* v = (T*)raw[u];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = live ? src[kb * 128 + i] : T(0.f);
+        for (int i = 0; i < 8; ++i) v[i] = left > u * 256 ? from[i] : T(0.f);
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t kb = base + 2 * u + half;
       float f[8];
       const T* v = (const T*)raw[u];
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
-      uint32_t amax = 0;  // of the magnitudes' bits, which order like the magnitudes; a NaN is above infinity
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7fffffffu);
+      uint32_t amax = exponent_bits<T>(raw[u], f);
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
-      const uint32_t code = biased == 255 ? 255 : biased > 2 ? biased - 2 : 0;
-      const float inv = __uint_as_float((254u - (code == 255 ? 254u : code)) << 23);  // 2^(127 - code)
-      uint32_t packed = 0;
+      const uint32_t code = biased == 255 ? 255 : max(biased, 2u) - 2;
+      const float inv = __uint_as_float((254u - min(code, 254u)) << 23);  // 2^(127 - code)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        packed |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(f[2 * i] * inv, f[2 * i + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * i);
+      for (int i = 0; i < 8; ++i) f[i] *= inv;
       uint32_t word = code << (8 * (part >> 2));  // the four scales of the sixteen lanes as one word
       word |= __shfl_xor_sync(0xffffffffu, word, 4);
       word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      if (row_live && kb * 128 + part * 8 < K) *(uint32_t*)(dst + kb * 64) = packed;
+      const int kb = base + 2 * u;
+      if (left > u * 256) *(uint32_t*)(dst + kb * 64) = pack_e2m1(f);
       if (part == 0 && kb < KB) *(uint32_t*)(sdst + kb * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
     }
   }
@@ -106,38 +123,40 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict
 
 // The reverse; a lane's values fill one 16-byte store: four fp32 or eight 16-bit ones.
 template <typename T>
-__global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, int64_t R, int64_t K, T* __restrict__ out) {
+__global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, int64_t R, int K, T* __restrict__ out) {
   constexpr int PER_LANE = 16 / sizeof(T), STEP = 32 * PER_LANE, UNROLL = Q_CHUNK / STEP < 8 ? Q_CHUNK / STEP : 8;
   typedef typename std::conditional<PER_LANE == 8, uint32_t, uint16_t>::type Packed;
   const RowSlot slot = row_slot();
   if (slot.row >= R) return;
   const int lane = threadIdx.x & 31;
   const uint8_t* ssrc = scales + (slot.row / 128) * k_blocks(K) * SCALE_BLOCK + slot.scale;
-  const int64_t first = (int64_t)blockIdx.y * Q_CHUNK, last = first + Q_CHUNK < K ? first + Q_CHUNK : K;
+  const uint8_t* src = data + slot.row * (K / 2);
+  T* dst = out + slot.row * K;
+  const int first = (int)blockIdx.y * Q_CHUNK, last = first + Q_CHUNK < K ? first + Q_CHUNK : K;
 #pragma unroll 1
-  for (int64_t base = first + lane * PER_LANE; base < last; base += UNROLL * STEP) {
+  for (int base = first + lane * PER_LANE; base < last; base += UNROLL * STEP) {
     uint32_t packed[UNROLL], code[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t col = base + u * STEP;
+      const int col = base + u * STEP;
       if (col >= last) continue;
-      packed[u] = *(const Packed*)(data + (slot.row * K + col) / 2);
+      packed[u] = *(const Packed*)(src + col / 2);
       code[u] = ssrc[col / 128 * SCALE_BLOCK + col % 128 / BLOCK];
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t col = base + u * STEP;
+      const int col = base + u * STEP;
       if (col >= last) continue;
       const float scale = __uint_as_float(code[u] == 255 ? 0x7fffffffu : code[u] ? code[u] << 23 : 0x00400000u);
       alignas(16) T raw[PER_LANE];
 #pragma unroll
       for (int j = 0; j < PER_LANE; ++j) {
-        const uint32_t q = packed[u] >> (4 * j) & 15, m = q & 7;
-        // E2M1: 0, 0.5, then 1 + m/2 times a power of two
-        const float mag = m < 2 ? 0.5f * (float)m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1) << 22);
-        raw[j] = from_f(T(), (q & 8 ? -mag : mag) * scale);
+        // E2M1's exponent and mantissa in a float's places stand for the value times 2^-126, its 0.5 included (a subnormal)
+        const uint32_t q = packed[u] << (28 - 4 * j);
+        const float v = __uint_as_float((q & 0x80000000u) | (q >> 28 & 7) << 22) * 0x1p126f;
+        raw[j] = from_f(T(), v * scale);
       }
-      *(uint4*)(out + slot.row * K + col) = *(uint4*)raw;
+      *(uint4*)(dst + col) = *(uint4*)raw;
     }
   }
 }
@@ -317,13 +336,13 @@ static int launched(const char* what) {
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
-  if (vec) quantize_kernel<T, true><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
-  else quantize_kernel<T, false><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, K, stride, (uint8_t*)data, (uint8_t*)scales);
+  if (vec) quantize_kernel<T, true><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
+  else quantize_kernel<T, false><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
   return launched("bshmem_mxfp4_quantize");
 }
 template <typename T>
 static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
-  dequantize_kernel<T><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, K, (T*)out);
+  dequantize_kernel<T><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out);
   return launched("bshmem_mxfp4_dequantize");
 }
 
