@@ -1,0 +1,382 @@
+// Block-scaled product of two matrices in microscaled 4-bit floats: out[M][N] = x[M][K] w[N][K]^T, on tcgen05.
+//
+// 256 values of K are 128 bytes of a row, one swizzle atom: a K step of 256 moves and multiplies the same bytes as one of 64 values of bf16,
+// four MMAs of 64 values each.  Its scales (1 KB per 128 rows) travel into the same stage and are copied to tensor memory by the thread that
+// issues the MMAs, a row's scales in the lane of its number modulo 32.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/bshmem/mxfp4.h"
+#include "../../include/bshmem/tcgen05.cuh"
+
+namespace bshmem {
+namespace mx {
+using namespace sm100;
+
+constexpr int BLOCK = 32;              // values per scale
+constexpr int SCALE_BLOCK = 512;       // bytes: 128 rows x 4 scales
+
+__host__ __device__ __forceinline__ int64_t k_blocks(int64_t K) { return (K + 255) / 256 * 2; }      // of 128 values, even
+__host__ __device__ __forceinline__ int64_t row_blocks(int64_t R) { return (R + 127) / 128; }
+
+// ------------------------------------------------------------------ CTA pairs
+// Pairs of CTAs walk tiles of 256 rows of x by COLS rows of w (persistent).  Each CTA loads its own 128 rows of x and half the rows of w, the
+// even one issues the MMAs for both, and each CTA's tensor memory gets its own 128 x COLS accumulator: half the traffic from L2 per
+// operation of a single CTA's tile, which at this rate is what bounds it (64 bytes a clock and SM instead of 96).
+// Tensor memory (COLS = 256): two accumulators, which overlap by the 48 columns that two steps' scales take:
+//   [0, 256) accumulator 0    [208, 464) accumulator 1    [464, 512) scales
+// The epilogue drains the shared columns of a tile first; from then on the other accumulator may be written.
+// The scales of a step replace those of two steps before; the MMAs that read them are known to be complete (their stage's barrier).
+//   warp 0  TMA producer   warp 1  MMA issuer (even CTA)   warp 2  tensor memory   warps 4 to 7  epilogue
+constexpr int P_THREADS = 256, P_EPI_WARP0 = 4, P_EPI_THREADS = 128, P_CHUNK = 64;
+constexpr int P_STAGE_A = 128 * 128, P_OUT = 128 * P_CHUNK * 2;
+template <int COLS>
+struct PairTile {
+  static constexpr int B_ROWS = COLS / 2, B_BYTES = B_ROWS * 128, S_BLOCKS = COLS / 128, S_BYTES = 1024 * (1 + S_BLOCKS);
+  static constexpr int STAGE = P_STAGE_A + B_BYTES + S_BYTES, STAGES = COLS == 256 ? 5 : 7;
+  static constexpr int S_COLS = 8 + 8 * S_BLOCKS, S_FIRST = 512 - 2 * S_COLS, ACC1 = COLS < S_FIRST - COLS ? COLS : S_FIRST - COLS;
+  static constexpr int TILES = STAGES * STAGE + 2 * P_OUT, SMEM = TILES + 1024 /*alignment slack*/ + 256 /*barriers*/;
+  static_assert(COLS - ACC1 <= P_CHUNK, "the first chunk that the epilogue drains holds all shared columns");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct alignas(64) PairParams {
+  CUtensorMap tmA, tmB, tmSA, tmSB, tmOut;
+  int* error_flag;
+  uint64_t wait_limit_ns;
+  int M, N, K;
+  int tiles_m, tiles;   // row tiles run fastest
+};
+
+template <int COLS>
+__global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_constant__ PairParams p) {
+  using Tile = PairTile<COLS>;
+  constexpr int STAGES = Tile::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + STAGES * P_STAGE_A;
+  uint8_t* sE = sB + STAGES * Tile::B_BYTES;     // two output chunks
+  uint8_t* sS = sE + 2 * P_OUT;                  // per stage: 1 KB of A's scales, then B's
+  uint64_t* full = (uint64_t*)(smem + Tile::TILES);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;           // [2]
+  uint64_t* acc_free = acc_full + 2;             // a tile's shared columns have been drained
+  uint32_t* tmem_slot = (uint32_t*)(acc_free + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_ctarank();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 2);   // one arrival, with its byte count, from each CTA's producer
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&acc_full[0], 1);
+    mbar_init(&acc_full[1], 1);
+    mbar_init(acc_free, 2 * P_EPI_THREADS / 32);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 2) {
+    tmem_alloc<2>(tmem_slot, 512);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // the other CTA's barriers are initialised before anything arrives on them
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the launch may overlap the end of the kernel before it
+  const int steps = (p.K + 255) / 256, first = (int)blockIdx.x >> 1, walkers = (int)gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&p.tmA);
+      tma_prefetch_desc(&p.tmB);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = first; t < p.tiles && !*abort_flag; t += walkers) {
+        const int tm = t % p.tiles_m, tn = t / p.tiles_m;
+        for (int k = 0; k < steps; ++k) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
+          const uint32_t lead = mapa_u32(smem_u32(&full[stage]), 0);
+          mbar_expect_tx_cluster(lead, Tile::STAGE);
+          tma_load_2d_pair(sA + stage * P_STAGE_A, &p.tmA, lead, k * 64, tm * 256 + rank * 128);
+          tma_load_2d_pair(sB + stage * Tile::B_BYTES, &p.tmB, lead, k * 64, tn * COLS + rank * Tile::B_ROWS);
+          tma_load_2d_pair(sS + stage * Tile::S_BYTES, &p.tmSA, lead, k * 256, tm * 2 + rank);
+          tma_load_2d_pair(sS + stage * Tile::S_BYTES + 1024, &p.tmSB, lead, k * 256, tn * Tile::S_BLOCKS);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // The last fills' stages are still handed back by the even CTA: this CTA stays until they are.
+      for (int i = 0; i < STAGES && !*abort_flag; ++i) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc[2] = {umma_idesc_mxf4(256, COLS, 0), umma_idesc_mxf4(256, COLS, 2)};
+      int stage = 0, acc = 0, n = 0;
+      uint32_t phase = 0, step = 0;
+      for (int t = first; t < p.tiles && !*abort_flag; t += walkers, ++n) {
+        if (n && !mbar_wait(acc_free, (n - 1) & 1, p.wait_limit_ns, abort_flag)) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem + (acc ? Tile::ACC1 : 0);
+        bool ok = true;
+        for (int k = 0; k < steps; ++k, ++step) {
+          if (step >= 2) {  // the MMAs of two steps before are complete: their scales may be replaced
+            const uint32_t s2 = step - 2;
+            if (!mbar_wait(&empty[s2 % STAGES], s2 / STAGES & 1, p.wait_limit_ns, abort_flag)) { ok = false; break; }
+          }
+          if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) { ok = false; break; }
+          tc_fence_after_sync();
+          const uint32_t sf = tmem + Tile::S_FIRST + (step & 1) * Tile::S_COLS;  // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows
+          const uint32_t s = smem_u32(sS + stage * Tile::S_BYTES);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            umma_copy_scales_pair(sf + h * 4, umma_desc_scales(s + h * SCALE_BLOCK));
+#pragma unroll
+            for (int b = 0; b < Tile::S_BLOCKS; ++b)
+              umma_copy_scales_pair(sf + 8 + (h * Tile::S_BLOCKS + b) * 4, umma_desc_scales(s + 1024 + b * 1024 + h * SCALE_BLOCK));
+          }
+          const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * P_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * Tile::B_BYTES));
+#pragma unroll
+          for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
+            umma_mxf4_pair(d, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * Tile::S_BLOCKS * 4, (k | i) != 0);
+          umma_commit_pair(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit_pair(&acc_full[acc]);
+        acc ^= 1;
+      }
+    }
+  } else if (warp >= P_EPI_WARP0) {
+    const int ew = warp - P_EPI_WARP0, row = ew * 32 + lane;
+    const bool issuer = threadIdx.x == P_EPI_WARP0 * 32;
+    int acc = 0, buf = 0;
+    uint32_t phase[2] = {0, 0};
+    for (int t = first; t < p.tiles; t += walkers) {
+      const int row0 = t % p.tiles_m * 256 + rank * 128, col0 = t / p.tiles_m * COLS;
+      const uint32_t ok = mbar_wait(&acc_full[acc], phase[acc], p.wait_limit_ns, abort_flag) ? 1u : 0u;
+      phase[acc] ^= 1;
+      if (!named_bar_and(1, P_EPI_THREADS, ok)) break;  // either all epilogue threads go on or all leave
+      tc_fence_after_sync();
+      const uint32_t src = tmem + ((uint32_t)(ew * 32) << 16) + (uint32_t)(acc ? Tile::ACC1 : 0);
+#pragma unroll 1
+      for (int i = 0; i < COLS / P_CHUNK; ++i) {
+        const int c = (acc ? i : (i + COLS / P_CHUNK - 1) % (COLS / P_CHUNK)) * P_CHUNK;  // shared columns first
+        float f[P_CHUNK];
+        tmem_ld_32x32(src + c, (uint32_t*)f);
+        tmem_ld_32x32(src + c + 32, (uint32_t*)f + 32);
+        tmem_ld_wait();
+        if (i == 0) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(acc_free), 0));
+        }
+        if (issuer) bulk_wait_read<1>();  // the store that read this buffer last
+        named_bar_sync(1, P_EPI_THREADS);
+        uint8_t* dst = sE + buf * P_OUT + row * 128;
+#pragma unroll
+        for (int j = 0; j < P_CHUNK / 8; ++j) {
+          uint4 v;
+          __nv_bfloat162* h = (__nv_bfloat162*)&v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(f[j * 8 + 2 * e], f[j * 8 + 2 * e + 1]);
+          *(uint4*)(dst + ((j ^ (row & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        named_bar_sync(1, P_EPI_THREADS);
+        if (issuer) {
+          if (row0 < p.M && col0 + c < p.N) tma_store_2d(&p.tmOut, sE + buf * P_OUT, col0 + c, row0);  // clipped to the matrix
+          bulk_commit();
+        }
+        buf ^= 1;
+      }
+      acc ^= 1;
+    }
+    if (issuer) bulk_wait<0>();
+  }
+  if (*abort_flag) {  // copies still in flight land before the shared memory goes away
+    const uint64_t t0 = timer_ns();
+    while (timer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA frees tensor memory that the other's MMAs write
+  if (warp == 2) tmem_dealloc<2>(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
+}
+
+// ------------------------------------------------------------------ one CTA per tile
+// One tile of 128 rows of the first operand by COLS rows of the second per CTA, over all of K in steps of 256 values (128 bytes).  The
+// scales of a step (1 KB per 128 rows) come with the operands' bytes into the same stage and are copied from there to tensor memory
+// by the thread that issues the MMAs, each stage to columns of its own: they are written again only after the stage's MMAs are done.
+// SWAP: the first operand is the weights (few rows of x).
+//   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
+constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128, G_RING = 208 * 1024;
+constexpr int G_SMEM = G_RING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+
+struct alignas(64) GemmParams {
+  CUtensorMap tmA, tmB;
+  const uint8_t *sa, *sb;   // scales of the two operands
+  __nv_bfloat16* out;
+  int* error_flag;
+  uint64_t wait_limit_ns;
+  int64_t rows_a, rows_b;   // rows of the operands
+  int64_t ld;               // of the output
+  int K, kb;                // kb: blocks of scales per row block
+  int tiles_a;
+};
+
+template <int COLS, bool SWAP>
+__global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  constexpr int B_BYTES = COLS * 128, SB_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + SB_BLOCKS * 1024;
+  constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, STAGES = G_RING / STAGE < 6 ? G_RING / STAGE : 6;
+  constexpr int S_COLS = 2 * 4 + 2 * 4 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
+  constexpr int TMEM = COLS + STAGES * S_COLS <= 128 ? 128 : COLS + STAGES * S_COLS <= 256 ? 256 : 512;
+  static_assert(COLS + STAGES * S_COLS <= 512, "tensor memory");
+  constexpr int PITCH = SWAP ? COLS + 1 : COLS + 4;
+  static_assert(128 * PITCH * 4 <= G_RING, "the finished tile reuses the ring");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * G_STAGE_A;
+  uint8_t* sS = sB + STAGES * B_BYTES;               // per stage: 1 KB of A's scales, then B's
+  uint64_t* full = (uint64_t*)(smem + G_RING);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t ta = blockIdx.x % p.tiles_a, tb = blockIdx.x / p.tiles_a;
+  const int64_t row_a = ta * 128, row_b = tb * COLS;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const int steps = (p.K + 255) / 256;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&p.tmA);
+      tma_prefetch_desc(&p.tmB);
+      const uint8_t* sa = p.sa + (row_a / 128) * p.kb * SCALE_BLOCK;
+      const uint8_t* sb = p.sb + (row_b / 128) * p.kb * SCALE_BLOCK;
+      // the second half of a 256-row tile may lie past the scales' last row block
+      const int sb_blocks = SB_BLOCKS == 2 && row_b + 128 < p.rows_b ? 2 : 1;
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int k = 0; k < steps; ++k) {
+        if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
+        uint8_t* s = sS + stage * S_BYTES;
+        mbar_expect_tx(&full[stage], G_STAGE_A + B_BYTES + 1024 + sb_blocks * 1024);
+        tma_load_2d(sA + stage * G_STAGE_A, &p.tmA, &full[stage], k * 64, (int)row_a);
+        tma_load_2d(sB + stage * B_BYTES, &p.tmB, &full[stage], k * 64, (int)row_b);
+        bulk_load(s, sa + (size_t)k * 1024, 1024, &full[stage]);
+        for (int b = 0; b < sb_blocks; ++b) bulk_load(s + 1024 + b * 1024, sb + ((size_t)b * p.kb + 2 * k) * SCALE_BLOCK, 1024, &full[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc[2] = {umma_idesc_mxf4(128, COLS, 0), umma_idesc_mxf4(128, COLS, 2)};
+      const uint32_t sfb_first = (uint32_t)(row_b % 128 / 32);  // rows of a narrow tile start inside a row block
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int k = 0; k < steps; ++k) {
+        if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) break;
+        tc_fence_after_sync();
+        const uint32_t sf = tmem + COLS + stage * S_COLS;  // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows
+        const uint32_t s = smem_u32(sS + stage * S_BYTES);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          umma_copy_scales(sf + h * 4, umma_desc_scales(s + h * SCALE_BLOCK));
+#pragma unroll
+          for (int b = 0; b < SB_BLOCKS; ++b) umma_copy_scales(sf + 8 + (h * SB_BLOCKS + b) * 4, umma_desc_scales(s + 1024 + b * 1024 + h * SCALE_BLOCK));
+        }
+        const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * G_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * B_BYTES));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
+          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, (k | i) != 0);
+        umma_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      umma_commit(acc_full);
+    }
+  }
+  __syncwarp();
+  // Every MMA of this CTA is complete, so every load has been consumed and the ring is free for the finished tile.
+  const bool ok = mbar_wait(acc_full, 0, p.wait_limit_ns, abort_flag) && !*abort_flag;
+  if (!ok) {
+    const uint64_t t0 = timer_ns();  // copies still in flight land before the shared memory is reused or goes away
+    while (timer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  tc_fence_after_sync();
+  float* tile = (float*)smem;  // [128][PITCH]
+  {
+    constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
+    const int c0 = (warp >> 2) * HALF;
+    float* mine = tile + ((warp & 3) * 32 + lane) * PITCH;
+    if (c0 < COLS) {
+#pragma unroll
+      for (int c = c0; c < c0 + HALF; c += 32) {
+        float f[32];
+        tmem_ld_32x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, (uint32_t*)f);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mine[c + j] = f[j];
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, TMEM);
+  if (SWAP) {
+    // row r of the tile is output column row_a + r, column c output row row_b + c
+    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
+      const int r = i & 127, c = i >> 7;
+      if (row_b + c < p.rows_b && row_a + r < p.rows_a) p.out[(row_b + c) * p.ld + row_a + r] = __float2bfloat16_rn(tile[r * PITCH + c]);
+    }
+  } else {
+    const bool vec = p.ld % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
+    for (int i = threadIdx.x; i < 128 * (COLS / 4); i += G_THREADS) {
+      const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+      if (row_a + r >= p.rows_a || row_b + c >= p.rows_b) continue;
+      const float* f = tile + r * PITCH + c;
+      __nv_bfloat16* dst = p.out + (row_a + r) * p.ld + row_b + c;
+      if (vec) {
+        uint2 o;
+        ((__nv_bfloat162*)&o)[0] = __floats2bfloat162_rn(f[0], f[1]);
+        ((__nv_bfloat162*)&o)[1] = __floats2bfloat162_rn(f[2], f[3]);
+        *(uint2*)dst = o;
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (row_b + c + j < p.rows_b) dst[j] = __float2bfloat16_rn(f[j]);
+      }
+    }
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
+}
+
+}  // namespace mx
+}  // namespace bshmem

@@ -11,17 +11,12 @@
 
 #include "../../include/bshmem/mxfp4.h"
 #include "../../include/bshmem/tcgen05.cuh"
+#include "gemm_mxfp4.cuh"
 #include "tensor_map.cuh"
 
 namespace bshmem {
 namespace mx {
 using namespace sm100;
-
-constexpr int BLOCK = 32;              // values per scale
-constexpr int SCALE_BLOCK = 512;       // bytes: 128 rows x 4 scales
-
-__host__ __device__ __forceinline__ int64_t k_blocks(int64_t K) { return (K + 255) / 256 * 2; }      // of 128 values, even
-__host__ __device__ __forceinline__ int64_t row_blocks(int64_t R) { return (R + 127) / 128; }
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -161,171 +156,6 @@ __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __
   }
 }
 
-// ------------------------------------------------------------------ product
-// One tile of 128 rows of the first operand by COLS rows of the second per CTA, over all of K in steps of 256 values (128 bytes).  The
-// scales of a step (1 KB per 128 rows) come with the operands' bytes into the same stage and are copied from there to tensor memory
-// by the thread that issues the MMAs, each stage to columns of its own: they are written again only after the stage's MMAs are done.
-// SWAP: the first operand is the weights (few rows of x).
-//   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
-constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128, G_RING = 208 * 1024;
-constexpr int G_SMEM = G_RING + 1024 /*alignment slack*/ + 256 /*barriers*/;
-
-struct alignas(64) GemmParams {
-  CUtensorMap tmA, tmB;
-  const uint8_t *sa, *sb;   // scales of the two operands
-  __nv_bfloat16* out;
-  int* error_flag;
-  uint64_t wait_limit_ns;
-  int64_t rows_a, rows_b;   // rows of the operands
-  int64_t ld;               // of the output
-  int K, kb;                // kb: blocks of scales per row block
-  int tiles_a;
-};
-
-template <int COLS, bool SWAP>
-__global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  constexpr int B_BYTES = COLS * 128, SB_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + SB_BLOCKS * 1024;
-  constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, STAGES = G_RING / STAGE < 6 ? G_RING / STAGE : 6;
-  constexpr int S_COLS = 2 * 4 + 2 * 4 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
-  constexpr int TMEM = COLS + STAGES * S_COLS <= 128 ? 128 : COLS + STAGES * S_COLS <= 256 ? 256 : 512;
-  static_assert(COLS + STAGES * S_COLS <= 512, "tensor memory");
-  constexpr int PITCH = SWAP ? COLS + 1 : COLS + 4;
-  static_assert(128 * PITCH * 4 <= G_RING, "the finished tile reuses the ring");
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * G_STAGE_A;
-  uint8_t* sS = sB + STAGES * B_BYTES;               // per stage: 1 KB of A's scales, then B's
-  uint64_t* full = (uint64_t*)(smem + G_RING);
-  uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;
-  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
-  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t ta = blockIdx.x % p.tiles_a, tb = blockIdx.x / p.tiles_a;
-  const int64_t row_a = ta * 128, row_b = tb * COLS;
-  if (threadIdx.x == 0) {
-    *abort_flag = 0;
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    mbar_init(acc_full, 1);
-    mbar_fence_init();
-    fence_proxy_async_smem();
-  }
-  if (warp == 2) {
-    tmem_alloc(tmem_slot, TMEM);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  const int steps = (p.K + 255) / 256;
-
-  if (warp == 0) {
-    if (elect_one()) {
-      tma_prefetch_desc(&p.tmA);
-      tma_prefetch_desc(&p.tmB);
-      const uint8_t* sa = p.sa + (row_a / 128) * p.kb * SCALE_BLOCK;
-      const uint8_t* sb = p.sb + (row_b / 128) * p.kb * SCALE_BLOCK;
-      // the second half of a 256-row tile may lie past the scales' last row block
-      const int sb_blocks = SB_BLOCKS == 2 && row_b + 128 < p.rows_b ? 2 : 1;
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int k = 0; k < steps; ++k) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
-        uint8_t* s = sS + stage * S_BYTES;
-        mbar_expect_tx(&full[stage], G_STAGE_A + B_BYTES + 1024 + sb_blocks * 1024);
-        tma_load_2d(sA + stage * G_STAGE_A, &p.tmA, &full[stage], k * 64, (int)row_a);
-        tma_load_2d(sB + stage * B_BYTES, &p.tmB, &full[stage], k * 64, (int)row_b);
-        bulk_load(s, sa + (size_t)k * 1024, 1024, &full[stage]);
-        for (int b = 0; b < sb_blocks; ++b) bulk_load(s + 1024 + b * 1024, sb + ((size_t)b * p.kb + 2 * k) * SCALE_BLOCK, 1024, &full[stage]);
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-      }
-    }
-  } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc[2] = {umma_idesc_mxf4(128, COLS, 0), umma_idesc_mxf4(128, COLS, 2)};
-      const uint32_t sfb_first = (uint32_t)(row_b % 128 / 32);  // rows of a narrow tile start inside a row block
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int k = 0; k < steps; ++k) {
-        if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) break;
-        tc_fence_after_sync();
-        const uint32_t sf = tmem + COLS + stage * S_COLS;  // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows
-        const uint32_t s = smem_u32(sS + stage * S_BYTES);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          umma_copy_scales(sf + h * 4, umma_desc_scales(s + h * SCALE_BLOCK));
-#pragma unroll
-          for (int b = 0; b < SB_BLOCKS; ++b) umma_copy_scales(sf + 8 + (h * SB_BLOCKS + b) * 4, umma_desc_scales(s + 1024 + b * 1024 + h * SCALE_BLOCK));
-        }
-        const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * G_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * B_BYTES));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
-          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, (k | i) != 0);
-        umma_commit(&empty[stage]);
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-      }
-      umma_commit(acc_full);
-    }
-  }
-  __syncwarp();
-  // Every MMA of this CTA is complete, so every load has been consumed and the ring is free for the finished tile.
-  const bool ok = mbar_wait(acc_full, 0, p.wait_limit_ns, abort_flag) && !*abort_flag;
-  if (!ok) {
-    const uint64_t t0 = timer_ns();  // copies still in flight land before the shared memory is reused or goes away
-    while (timer_ns() - t0 < 200000) __nanosleep(1000);
-  }
-  tc_fence_after_sync();
-  float* tile = (float*)smem;  // [128][PITCH]
-  {
-    constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
-    const int c0 = (warp >> 2) * HALF;
-    float* mine = tile + ((warp & 3) * 32 + lane) * PITCH;
-    if (c0 < COLS) {
-#pragma unroll
-      for (int c = c0; c < c0 + HALF; c += 32) {
-        float f[32];
-        tmem_ld_32x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, (uint32_t*)f);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) mine[c + j] = f[j];
-      }
-    }
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == 2) tmem_dealloc(tmem, TMEM);
-  if (SWAP) {
-    // row r of the tile is output column row_a + r, column c output row row_b + c
-    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
-      const int r = i & 127, c = i >> 7;
-      if (row_b + c < p.rows_b && row_a + r < p.rows_a) p.out[(row_b + c) * p.ld + row_a + r] = __float2bfloat16_rn(tile[r * PITCH + c]);
-    }
-  } else {
-    const bool vec = p.ld % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
-    for (int i = threadIdx.x; i < 128 * (COLS / 4); i += G_THREADS) {
-      const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
-      if (row_a + r >= p.rows_a || row_b + c >= p.rows_b) continue;
-      const float* f = tile + r * PITCH + c;
-      __nv_bfloat16* dst = p.out + (row_a + r) * p.ld + row_b + c;
-      if (vec) {
-        uint2 o;
-        ((__nv_bfloat162*)&o)[0] = __floats2bfloat162_rn(f[0], f[1]);
-        ((__nv_bfloat162*)&o)[1] = __floats2bfloat162_rn(f[2], f[3]);
-        *(uint2*)dst = o;
-      } else {
-        for (int j = 0; j < 4; ++j)
-          if (row_b + c + j < p.rows_b) dst[j] = __float2bfloat16_rn(f[j]);
-      }
-    }
-  }
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
-}
-
 static int launched(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return BSHMEM_MX_OK;
@@ -346,21 +176,81 @@ static int launch_dequantize(const void* data, const void* scales, int64_t R, in
   return launched("bshmem_mxfp4_dequantize");
 }
 
+// Tensor map of scales: rows are row blocks, elements words; a box is 1 KB (256 values of K) of `blocks` row blocks.
+static int make_scale_map(CUtensorMap* out, const void* base, int64_t rows, int64_t K, uint32_t blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return BSHMEM_FUSED_ERR_DRIVER;
+  cuuint64_t dims[2] = {(cuuint64_t)k_blocks(K) * (SCALE_BLOCK / 4), (cuuint64_t)row_blocks(rows)};
+  cuuint64_t strides[1] = {dims[0] * 4};
+  cuuint32_t box[2] = {256, blocks}, estr[2] = {1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : BSHMEM_FUSED_ERR_DRIVER;
+}
+static int map_status(int st) { return st == 0 ? BSHMEM_MX_OK : st == BSHMEM_FUSED_ERR_ALIGNMENT ? BSHMEM_MX_ERR_ALIGNMENT : BSHMEM_MX_ERR_DRIVER; }
+// Raises a kernel's shared-memory limit, once per GPU (`ready`: the GPUs done, bit = ordinal).
+static bool reserve_smem(const void* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < 64 && (ready.load(std::memory_order_acquire) >> device & 1)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
+  return true;
+}
+static int sm_count() {
+  int device = 0, sms = 0;
+  cudaGetDevice(&device);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  return sms > 1 ? sms : 2;
+}
+
+template <int COLS>
+static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns, cudaStream_t stream) {
+  PairParams p;
+  memset(&p, 0, sizeof(p));
+  int st = make_map(&p.tmA, a->x, (uint64_t)a->M, (uint64_t)a->K / 4, 128);  // bytes, in pairs: the box is 128 rows by 128 bytes
+  if (!st) st = make_map(&p.tmB, a->w, (uint64_t)a->N, (uint64_t)a->K / 4, COLS / 2);
+  if (!st) st = make_map(&p.tmOut, a->out, (uint64_t)a->M, (uint64_t)a->N, 128);
+  if (!st) st = make_scale_map(&p.tmSA, a->x_scales, a->M, a->K, 1);
+  if (!st) st = make_scale_map(&p.tmSB, a->w_scales, a->N, a->K, COLS / 128);
+  if (st) return map_status(st);
+  p.error_flag = a->error_flag;
+  p.wait_limit_ns = wait_limit_ns;
+  p.M = (int)a->M; p.N = (int)a->N; p.K = (int)a->K;
+  p.tiles_m = (int)((a->M + 255) / 256);
+  const int64_t tiles = (int64_t)p.tiles_m * ((a->N + COLS - 1) / COLS);
+  if (tiles > 0x3fffffff) return BSHMEM_MX_ERR_SHAPE;
+  p.tiles = (int)tiles;
+  static std::atomic<uint64_t> ready;
+  if (!reserve_smem((const void*)gemm_pair_kernel<COLS>, PairTile<COLS>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
+  const int most = sm_count() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (p.tiles < most ? p.tiles : most));
+  cfg.blockDim = dim3(P_THREADS);
+  cfg.dynamicSmemBytes = PairTile<COLS>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, gemm_pair_kernel<COLS>, p) != cudaSuccess) return launched("bshmem_mxfp4_gemm");
+  return BSHMEM_MX_OK;
+}
+
 template <int COLS, bool SWAP>
 static int launch_gemm(GemmParams& p, const void* a, const void* b, cudaStream_t stream) {
   int st = make_map(&p.tmA, a, (uint64_t)p.rows_a, (uint64_t)p.K / 4, 128);  // bytes, in pairs: the box is 128 rows by 128 bytes
   if (!st) st = make_map(&p.tmB, b, (uint64_t)p.rows_b, (uint64_t)p.K / 4, COLS);
-  if (st) return st == BSHMEM_FUSED_ERR_ALIGNMENT ? BSHMEM_MX_ERR_ALIGNMENT : BSHMEM_MX_ERR_DRIVER;
+  if (st) return map_status(st);
   p.tiles_a = (int)((p.rows_a + 127) / 128);
   const int64_t tiles = (int64_t)p.tiles_a * ((p.rows_b + COLS - 1) / COLS);
   if (tiles > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
   static std::atomic<uint64_t> ready;
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return BSHMEM_MX_ERR_DRIVER;
-  if (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1)) {
-    if (cudaFuncSetAttribute((const void*)gemm_kernel<COLS, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, G_SMEM) != cudaSuccess) return BSHMEM_MX_ERR_DRIVER;
-    if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
-  }
+  if (!reserve_smem((const void*)gemm_kernel<COLS, SWAP>, G_SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
   gemm_kernel<COLS, SWAP><<<(int)tiles, G_THREADS, G_SMEM, stream>>>(p);
   return launched("bshmem_mxfp4_gemm");
 }
@@ -416,6 +306,7 @@ extern "C" int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* a, cudaStream_t
   p.ld = a->N;
   p.K = (int)a->K;
   p.kb = (int)k_blocks(a->K);
+  if (!swap && a->N % 8 == 0 && ((uintptr_t)a->out & 15) == 0) return launch_pair<256>(a, p.wait_limit_ns, stream);  // whole 16-byte units of output rows
   if (!swap) return launch_gemm<256, false>(p, a->x, a->w, stream);
   if (a->M <= 32) return launch_gemm<32, true>(p, a->w, a->x, stream);
   if (a->M <= 64) return launch_gemm<64, true>(p, a->w, a->x, stream);
