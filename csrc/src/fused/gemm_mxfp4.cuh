@@ -214,48 +214,59 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_co
 }
 
 // ------------------------------------------------------------------ one CTA per tile
-// One tile of 128 rows of the first operand by COLS rows of the second per CTA, over all of K in steps of 256 values (128 bytes).  The
-// scales of a step (1 KB per 128 rows) come with the operands' bytes into the same stage and are copied from there to tensor memory
-// by the thread that issues the MMAs, each stage to columns of its own: they are written again only after the stage's MMAs are done.
-// SWAP: the first operand is the weights (few rows of x).
+// One tile of 128 rows of the first operand by COLS rows of the second per CTA, in steps of 256 values of K.
+// SWAP: the first operand is the weights.  For few rows of x, where reading the weights is what takes the time: an SM takes in some
+// 60 bytes a clock, so all SMs have to read, and a cluster of CTAs divides K.  Each sends its sums to the shared memory of the CTA
+// that owns the column (column number modulo the cluster's size), which adds them in order.  (Owners that fetch the sums instead wait
+// for a round trip per value: 64 x 1024 x 8192 took 19 us that way.)  Without SWAP the kernel serves outputs whose rows are no whole
+// 16-byte units.
 //   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
-constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128, G_RING = 208 * 1024;
-constexpr int G_SMEM = G_RING + 1024 /*alignment slack*/ + 256 /*barriers*/;
+constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128;
+template <int COLS, bool SWAP>
+struct SingleTile {
+  static constexpr int B_BYTES = COLS * 128, S_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + S_BLOCKS * 1024;
+  static constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, OUT = SWAP ? 128 * COLS * 4 : 0;  // OUT: the finished tile, [split][COLS / split][128]
+  static constexpr int FIT = (225 * 1024 - OUT) / STAGE, STAGES = FIT < 8 ? FIT : 8;
+  static constexpr int RING = STAGES * STAGE, SMEM = RING + OUT + 1024 /*alignment slack*/ + 256 /*barriers*/;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
 
 struct alignas(64) GemmParams {
-  CUtensorMap tmA, tmB;
-  const uint8_t *sa, *sb;   // scales of the two operands
+  CUtensorMap tmA, tmB, tmSA, tmSB;
   __nv_bfloat16* out;
   int* error_flag;
   uint64_t wait_limit_ns;
   int64_t rows_a, rows_b;   // rows of the operands
   int64_t ld;               // of the output
-  int K, kb;                // kb: blocks of scales per row block
-  int tiles_a;
+  int K, tiles_a;
+  int split;                // CTAs that divide K (a cluster)
+  int early;                // the first operand is complete before the kernel ahead of this one on the stream began
 };
 
 template <int COLS, bool SWAP>
 __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  constexpr int B_BYTES = COLS * 128, SB_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + SB_BLOCKS * 1024;
-  constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, STAGES = G_RING / STAGE < 6 ? G_RING / STAGE : 6;
-  constexpr int S_COLS = 2 * 4 + 2 * 4 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
-  constexpr int TMEM = COLS + STAGES * S_COLS <= 128 ? 128 : COLS + STAGES * S_COLS <= 256 ? 256 : 512;
+  using Tile = SingleTile<COLS, SWAP>;
+  constexpr int B_BYTES = Tile::B_BYTES, SB_BLOCKS = Tile::S_BLOCKS, S_BYTES = Tile::S_BYTES, STAGE = Tile::STAGE, STAGES = Tile::STAGES;
+  constexpr int S_COLS = 8 + 8 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
+  constexpr int TMEM = COLS + STAGES * S_COLS <= 256 ? 256 : 512;
   static_assert(COLS + STAGES * S_COLS <= 512, "tensor memory");
-  constexpr int PITCH = SWAP ? COLS + 1 : COLS + 4;
-  static_assert(128 * PITCH * 4 <= G_RING, "the finished tile reuses the ring");
+  constexpr int PITCH = COLS + 4;
+  static_assert(SWAP || 128 * PITCH * 4 <= Tile::RING, "the finished tile reuses the ring");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * G_STAGE_A;
   uint8_t* sS = sB + STAGES * B_BYTES;               // per stage: 1 KB of A's scales, then B's
-  uint64_t* full = (uint64_t*)(smem + G_RING);
+  float* sums = (float*)(smem + Tile::RING);
+  uint64_t* full = (uint64_t*)(smem + Tile::RING + Tile::OUT);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t ta = blockIdx.x % p.tiles_a, tb = blockIdx.x / p.tiles_a;
-  const int64_t row_a = ta * 128, row_b = tb * COLS;
+  const int split = SWAP ? p.split : 1, rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int tile_number = (int)blockIdx.x / split;
+  const int64_t row_a = (int64_t)(tile_number % p.tiles_a) * 128, row_b = (int64_t)(tile_number / p.tiles_a) * COLS;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < STAGES; ++i) {
@@ -273,27 +284,32 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  if (split > 1) cluster_arrive();
   const uint32_t tmem = *tmem_slot;
-  const int steps = (p.K + 255) / 256;
+  const int all_steps = (p.K + 255) / 256, k0 = (int)((int64_t)all_steps * rank / split), k1 = (int)((int64_t)all_steps * (rank + 1) / split);
+  // The launch may overlap the end of the kernel before it.  Where that kernel made the second operand only, the first stages of the
+  // first operand are fetched before waiting for it.
+  if (!p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == 0) {
     if (elect_one()) {
       tma_prefetch_desc(&p.tmA);
       tma_prefetch_desc(&p.tmB);
-      const uint8_t* sa = p.sa + (row_a / 128) * p.kb * SCALE_BLOCK;
-      const uint8_t* sb = p.sb + (row_b / 128) * p.kb * SCALE_BLOCK;
-      // the second half of a 256-row tile may lie past the scales' last row block
-      const int sb_blocks = SB_BLOCKS == 2 && row_b + 128 < p.rows_b ? 2 : 1;
       int stage = 0;
       uint32_t phase = 0;
-      for (int k = 0; k < steps; ++k) {
+      auto load_a = [&](int k, int to) {
+        mbar_expect_tx(&full[to], STAGE);
+        tma_load_2d(sA + to * G_STAGE_A, &p.tmA, &full[to], k * 64, (int)row_a);
+        tma_load_2d(sS + to * S_BYTES, &p.tmSA, &full[to], k * 256, (int)(row_a / 128));
+      };
+      const int ahead = p.early ? (k1 - k0 < STAGES ? k1 - k0 : STAGES) : 0;
+      for (int k = 0; k < ahead; ++k) load_a(k0 + k, k);
+      if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int k = k0; k < k1; ++k) {
         if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
-        uint8_t* s = sS + stage * S_BYTES;
-        mbar_expect_tx(&full[stage], G_STAGE_A + B_BYTES + 1024 + sb_blocks * 1024);
-        tma_load_2d(sA + stage * G_STAGE_A, &p.tmA, &full[stage], k * 64, (int)row_a);
+        if (k - k0 >= ahead) load_a(k, stage);
         tma_load_2d(sB + stage * B_BYTES, &p.tmB, &full[stage], k * 64, (int)row_b);
-        bulk_load(s, sa + (size_t)k * 1024, 1024, &full[stage]);
-        for (int b = 0; b < sb_blocks; ++b) bulk_load(s + 1024 + b * 1024, sb + ((size_t)b * p.kb + 2 * k) * SCALE_BLOCK, 1024, &full[stage]);
+        tma_load_2d(sS + stage * S_BYTES + 1024, &p.tmSB, &full[stage], k * 256, (int)(row_b / 128));
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
@@ -303,10 +319,11 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
       const uint32_t sfb_first = (uint32_t)(row_b % 128 / 32);  // rows of a narrow tile start inside a row block
       int stage = 0;
       uint32_t phase = 0;
-      for (int k = 0; k < steps; ++k) {
+      for (int k = k0; k < k1; ++k) {
         if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) break;
         tc_fence_after_sync();
-        const uint32_t sf = tmem + COLS + stage * S_COLS;  // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows
+        // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows.  Written again only after the stage's MMAs are done.
+        const uint32_t sf = tmem + COLS + stage * S_COLS;
         const uint32_t s = smem_u32(sS + stage * S_BYTES);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -317,7 +334,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
         const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * G_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * B_BYTES));
 #pragma unroll
         for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
-          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, (k | i) != 0);
+          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, k > k0 || i > 0);
         umma_commit(&empty[stage]);
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
@@ -332,47 +349,65 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
     while (timer_ns() - t0 < 200000) __nanosleep(1000);
   }
   tc_fence_after_sync();
-  float* tile = (float*)smem;  // [128][PITCH]
-  {
-    constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
-    const int c0 = (warp >> 2) * HALF;
-    float* mine = tile + ((warp & 3) * 32 + lane) * PITCH;
+  const int quarter = (warp & 3) * 32;
+  constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
+  const int c0 = (warp >> 2) * HALF;   // this warp's rows are quarter + lane, its columns [c0, c0 + HALF)
+  if constexpr (SWAP) {
+    // row r of the tile is output column row_a + r, column c output row row_b + c
+    if (split > 1) cluster_wait();     // the others run: their shared memory may be written
+    const int share = COLS / split;
     if (c0 < COLS) {
 #pragma unroll
       for (int c = c0; c < c0 + HALF; c += 32) {
         float f[32];
-        tmem_ld_32x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, (uint32_t*)f);
+        tmem_ld_32x32(tmem + ((uint32_t)quarter << 16) + (uint32_t)c, (uint32_t*)f);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) mine[c + j] = f[j];
+        for (int j = 0; j < 32; ++j) {
+          float* at = sums + ((rank * share + (c + j) / split) * 128 + quarter + lane);
+          if (split == 1) *at = f[j];
+          else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(at), (uint32_t)((c + j) & (split - 1)))), "f"(f[j]) : "memory");
+        }
       }
     }
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == 2) tmem_dealloc(tmem, TMEM);
-  if (SWAP) {
-    // row r of the tile is output column row_a + r, column c output row row_b + c
-    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
-      const int r = i & 127, c = i >> 7;
-      if (row_b + c < p.rows_b && row_a + r < p.rows_a) p.out[(row_b + c) * p.ld + row_a + r] = __float2bfloat16_rn(tile[r * PITCH + c]);
-    }
-  } else {
+    tc_fence_before_sync();
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, TMEM);
+    const int cols = p.rows_b - row_b < COLS ? (int)(p.rows_b - row_b) : COLS, r = lane * 4;
     const bool vec = p.ld % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
-    for (int i = threadIdx.x; i < 128 * (COLS / 4); i += G_THREADS) {
-      const int r = i / (COLS / 4), c = i % (COLS / 4) * 4;
-      if (row_a + r >= p.rows_a || row_b + c >= p.rows_b) continue;
-      const float* f = tile + r * PITCH + c;
-      __nv_bfloat16* dst = p.out + (row_a + r) * p.ld + row_b + c;
-      if (vec) {
-        uint2 o;
-        ((__nv_bfloat162*)&o)[0] = __floats2bfloat162_rn(f[0], f[1]);
-        ((__nv_bfloat162*)&o)[1] = __floats2bfloat162_rn(f[2], f[3]);
-        *(uint2*)dst = o;
+    for (int i = warp; i * split + rank < cols; i += G_THREADS / 32) {   // a warp takes a column: 128 values of an output row
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int q = 0; q < split; ++q) {
+        const float4 s = *(const float4*)(sums + (q * share + i) * 128 + r);
+        v.x += s.x, v.y += s.y, v.z += s.z, v.w += s.w;
+      }
+      __nv_bfloat16* dst = p.out + (row_b + i * split + rank) * p.ld + row_a + r;
+      alignas(8) __nv_bfloat162 o[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+      if (vec && row_a + r + 4 <= p.rows_a) {
+        *(uint2*)dst = *(uint2*)o;
       } else {
         for (int j = 0; j < 4; ++j)
-          if (row_b + c + j < p.rows_b) dst[j] = __float2bfloat16_rn(f[j]);
+          if (row_a + r + j < p.rows_a) dst[j] = ((__nv_bfloat16*)o)[j];
       }
+    }
+  } else {
+    float* tile = (float*)smem;  // [128][PITCH]
+#pragma unroll
+    for (int c = c0; c < c0 + HALF; c += 32) {
+      float f[32];
+      tmem_ld_32x32(tmem + ((uint32_t)quarter << 16) + (uint32_t)c, (uint32_t*)f);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) *(float4*)(tile + (quarter + lane) * PITCH + c + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 2) tmem_dealloc(tmem, TMEM);
+    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
+      const int r = i / COLS, c = i % COLS;
+      if (row_a + r < p.rows_a && row_b + c < p.rows_b) p.out[(row_a + r) * p.ld + row_b + c] = __float2bfloat16_rn(tile[r * PITCH + c]);
     }
   }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);

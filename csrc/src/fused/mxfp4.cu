@@ -69,6 +69,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int K, int64_t stride, uint8_t* __restrict__ data,
                                                              uint8_t* __restrict__ scales) {
   constexpr int UNROLL = sizeof(T) == 4 ? 4 : 8, WORDS = sizeof(T) * 8 / 16;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may set up, and fetch its weights, beside this kernel
   const RowSlot slot = row_slot();
   const int half = (threadIdx.x >> 4) & 1, part = threadIdx.x & 15;
   const int KB = (int)k_blocks(K), first = (int)blockIdx.y * (Q_CHUNK / 128), last = first + Q_CHUNK / 128 < KB ? first + Q_CHUNK / 128 : KB;
@@ -204,6 +205,28 @@ static int sm_count() {
   return sms > 1 ? sms : 2;
 }
 
+// A launch that may begin before the kernel ahead of it on the stream has ended (the kernels wait themselves).
+template <typename P>
+static int launch_clusters(void (*kernel)(P), const P& p, int grid, int threads, int smem, int cluster, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e == cudaSuccess) return BSHMEM_MX_OK;
+  fprintf(stderr, "bshmem_mxfp4_gemm: launch failed: %s\n", cudaGetErrorString(e));
+  return BSHMEM_MX_ERR_DRIVER;
+}
+
 template <int COLS>
 static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns, cudaStream_t stream) {
   PairParams p;
@@ -224,35 +247,36 @@ static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns
   static std::atomic<uint64_t> ready;
   if (!reserve_smem((const void*)gemm_pair_kernel<COLS>, PairTile<COLS>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
   const int most = sm_count() / 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (p.tiles < most ? p.tiles : most));
-  cfg.blockDim = dim3(P_THREADS);
-  cfg.dynamicSmemBytes = PairTile<COLS>::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, gemm_pair_kernel<COLS>, p) != cudaSuccess) return launched("bshmem_mxfp4_gemm");
-  return BSHMEM_MX_OK;
+  return launch_clusters(gemm_pair_kernel<COLS>, p, 2 * (p.tiles < most ? p.tiles : most), P_THREADS, PairTile<COLS>::SMEM, 2, stream);
 }
 
 template <int COLS, bool SWAP>
-static int launch_gemm(GemmParams& p, const void* a, const void* b, cudaStream_t stream) {
-  int st = make_map(&p.tmA, a, (uint64_t)p.rows_a, (uint64_t)p.K / 4, 128);  // bytes, in pairs: the box is 128 rows by 128 bytes
-  if (!st) st = make_map(&p.tmB, b, (uint64_t)p.rows_b, (uint64_t)p.K / 4, COLS);
+static int launch_gemm(const bshmem_mxfp4_gemm_args_t* g, uint64_t wait_limit_ns, cudaStream_t stream) {
+  GemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.rows_a = SWAP ? g->N : g->M;
+  p.rows_b = SWAP ? g->M : g->N;
+  int st = make_map(&p.tmA, SWAP ? g->w : g->x, (uint64_t)p.rows_a, (uint64_t)g->K / 4, 128);
+  if (!st) st = make_map(&p.tmB, SWAP ? g->x : g->w, (uint64_t)p.rows_b, (uint64_t)g->K / 4, COLS);
+  if (!st) st = make_scale_map(&p.tmSA, SWAP ? g->w_scales : g->x_scales, p.rows_a, g->K, 1);
+  if (!st) st = make_scale_map(&p.tmSB, SWAP ? g->x_scales : g->w_scales, p.rows_b, g->K, COLS > 128 ? 2 : 1);
   if (st) return map_status(st);
+  p.out = (__nv_bfloat16*)g->out;
+  p.error_flag = g->error_flag;
+  p.wait_limit_ns = wait_limit_ns;
+  p.ld = g->N;
+  p.K = (int)g->K;
   p.tiles_a = (int)((p.rows_a + 127) / 128);
   const int64_t tiles = (int64_t)p.tiles_a * ((p.rows_b + COLS - 1) / COLS);
-  if (tiles > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
+  // K is divided as long as that brings in SMs that would be idle, and leaves a CTA two steps at least.
+  p.split = 1;
+  const int steps = (p.K + 255) / 256, sms = sm_count();
+  while (SWAP && p.split < 8 && tiles * p.split * 2 <= sms && steps >= p.split * 4) p.split *= 2;
+  p.early = SWAP && g->w_ready;
+  if (tiles * p.split > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
   static std::atomic<uint64_t> ready;
-  if (!reserve_smem((const void*)gemm_kernel<COLS, SWAP>, G_SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
-  gemm_kernel<COLS, SWAP><<<(int)tiles, G_THREADS, G_SMEM, stream>>>(p);
-  return launched("bshmem_mxfp4_gemm");
+  if (!reserve_smem((const void*)gemm_kernel<COLS, SWAP>, SingleTile<COLS, SWAP>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
+  return launch_clusters(gemm_kernel<COLS, SWAP>, p, (int)tiles * p.split, G_THREADS, SingleTile<COLS, SWAP>::SMEM, p.split, stream);
 }
 
 }  // namespace mx
@@ -293,22 +317,10 @@ extern "C" int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* a, cudaStream_t
   if (st || a->M == 0 || a->N == 0) return st ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK;
   if (!a->x || !a->x_scales || !a->w || !a->w_scales || !a->out || !a->error_flag) return BSHMEM_MX_ERR_ARGS;
   if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales) & 15) return BSHMEM_MX_ERR_ALIGNMENT;
-  GemmParams p;
-  memset(&p, 0, sizeof(p));
-  const bool swap = a->M <= 128;
-  p.sa = (const uint8_t*)(swap ? a->w_scales : a->x_scales);
-  p.sb = (const uint8_t*)(swap ? a->x_scales : a->w_scales);
-  p.out = (__nv_bfloat16*)a->out;
-  p.error_flag = a->error_flag;
-  p.wait_limit_ns = a->wait_limit_ms ? (uint64_t)a->wait_limit_ms * 1000000ull : 10000000000ull;
-  p.rows_a = swap ? a->N : a->M;
-  p.rows_b = swap ? a->M : a->N;
-  p.ld = a->N;
-  p.K = (int)a->K;
-  p.kb = (int)k_blocks(a->K);
-  if (!swap && a->N % 8 == 0 && ((uintptr_t)a->out & 15) == 0) return launch_pair<256>(a, p.wait_limit_ns, stream);  // whole 16-byte units of output rows
-  if (!swap) return launch_gemm<256, false>(p, a->x, a->w, stream);
-  if (a->M <= 32) return launch_gemm<32, true>(p, a->w, a->x, stream);
-  if (a->M <= 64) return launch_gemm<64, true>(p, a->w, a->x, stream);
-  return launch_gemm<128, true>(p, a->w, a->x, stream);
+  const uint64_t limit = a->wait_limit_ms ? (uint64_t)a->wait_limit_ms * 1000000ull : 10000000000ull;
+  if (a->M <= 32) return launch_gemm<32, true>(a, limit, stream);
+  if (a->M <= 64) return launch_gemm<64, true>(a, limit, stream);
+  if (a->M <= 128) return launch_gemm<128, true>(a, limit, stream);
+  if (a->N % 8 == 0 && ((uintptr_t)a->out & 15) == 0) return launch_pair<256>(a, limit, stream);  // whole 16-byte units of output rows
+  return launch_gemm<256, false>(a, limit, stream);
 }

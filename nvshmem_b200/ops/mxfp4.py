@@ -24,7 +24,7 @@ _ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32", 3: "opera
 
 class _GemmArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("w", C.c_void_p), ("w_scales", C.c_void_p), ("out", C.c_void_p), ("M", C.c_int64), ("N", C.c_int64),
-                ("K", C.c_int64), ("wait_limit_ms", C.c_uint32), ("error_flag", C.c_void_p)]
+                ("K", C.c_int64), ("wait_limit_ms", C.c_uint32), ("error_flag", C.c_void_p), ("w_ready", C.c_int)]
 
 
 def _lib():
@@ -133,7 +133,8 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
     ``x`` that is not quantised yet is quantised in the call (:func:`quantize_mxfp4`).  M and N may be any number."""
     if not isinstance(w, MxFp4):
         raise FusedGemmError("w must be quantised (quantize_mxfp4)")
-    if not isinstance(x, MxFp4):
+    fresh = not isinstance(x, MxFp4)
+    if fresh:
         x = quantize_mxfp4(x)
     if x.shape[1] != w.shape[1]:
         raise FusedGemmError(f"shape mismatch: x {x.shape} w {w.shape}")
@@ -148,5 +149,6 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
     a.x, a.x_scales, a.w, a.w_scales, a.out = x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr()
     a.M, a.N, a.K = M, N, w.shape[1]
     a.error_flag = _error_flag(out.device).data_ptr()
+    a.w_ready = fresh and M > 0   # the kernel ahead is the one that quantises x; w is older
     _raise(_lib().bshmem_mxfp4_gemm(C.byref(a), H.current_stream_handle()), "bshmem_mxfp4_gemm")
     return out
