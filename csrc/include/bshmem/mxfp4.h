@@ -33,8 +33,11 @@ typedef struct {
   int64_t M, N, K;
   uint32_t wait_limit_ms;    /* bound of the waits inside the kernel (0: 10 s) */
   int* error_flag;           /* device int; set to 1 if a wait ran out */
-  int w_ready;               /* 1: w was complete before the last kernel launched on the stream began, so that reading it need not
-                                wait for that kernel (it quantised x, say) */
+  /* Optional: x before quantisation, [M][K] of raw_type with raw_stride elements between rows.  It is quantised into x and x_scales
+   * (which are then room for it) by a kernel of its own ahead of the product. */
+  const void* raw_x;
+  int raw_type;
+  int64_t raw_stride;
 } bshmem_mxfp4_gemm_args_t;
 
 /* data pointers 16-byte aligned. */

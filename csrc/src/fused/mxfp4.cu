@@ -272,7 +272,7 @@ static int launch_gemm(const bshmem_mxfp4_gemm_args_t* g, uint64_t wait_limit_ns
   p.split = 1;
   const int steps = (p.K + 255) / 256, sms = sm_count();
   while (SWAP && p.split < 8 && tiles * p.split * 2 <= sms && steps >= p.split * 4) p.split *= 2;
-  p.early = SWAP && g->w_ready;
+  p.early = SWAP && g->raw_x;  // the kernel ahead quantised x, and began after everything before it was complete
   if (tiles * p.split > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
   static std::atomic<uint64_t> ready;
   if (!reserve_smem((const void*)gemm_kernel<COLS, SWAP>, SingleTile<COLS, SWAP>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
@@ -317,6 +317,10 @@ extern "C" int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* a, cudaStream_t
   if (st || a->M == 0 || a->N == 0) return st ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK;
   if (!a->x || !a->x_scales || !a->w || !a->w_scales || !a->out || !a->error_flag) return BSHMEM_MX_ERR_ARGS;
   if (((uintptr_t)a->x_scales | (uintptr_t)a->w_scales) & 15) return BSHMEM_MX_ERR_ALIGNMENT;
+  if (a->raw_x) {
+    const int q = bshmem_mxfp4_quantize(a->raw_x, a->raw_type, a->M, a->K, a->raw_stride, (void*)a->x, (void*)a->x_scales, stream);
+    if (q) return q;
+  }
   const uint64_t limit = a->wait_limit_ms ? (uint64_t)a->wait_limit_ms * 1000000ull : 10000000000ull;
   if (a->M <= 32) return launch_gemm<32, true>(a, limit, stream);
   if (a->M <= 64) return launch_gemm<64, true>(a, limit, stream);

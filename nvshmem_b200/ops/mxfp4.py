@@ -14,7 +14,7 @@ import ctypes as C
 
 import torch
 
-from ..bindings import host as H
+from ._launch import device_of, stream_of
 from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
 
 BLOCK = 32
@@ -24,7 +24,7 @@ _ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32", 3: "opera
 
 class _GemmArgs(C.Structure):
     _fields_ = [("x", C.c_void_p), ("x_scales", C.c_void_p), ("w", C.c_void_p), ("w_scales", C.c_void_p), ("out", C.c_void_p), ("M", C.c_int64), ("N", C.c_int64),
-                ("K", C.c_int64), ("wait_limit_ms", C.c_uint32), ("error_flag", C.c_void_p), ("w_ready", C.c_int)]
+                ("K", C.c_int64), ("wait_limit_ms", C.c_uint32), ("error_flag", C.c_void_p), ("raw_x", C.c_void_p), ("raw_type", C.c_int), ("raw_stride", C.c_int64)]
 
 
 def _lib():
@@ -43,14 +43,6 @@ def _lib():
 def _raise(st: int, name: str) -> None:
     if st != 0:
         raise FusedGemmError(f"{name}: {_ERRORS.get(st, st)}")
-
-
-def _check_device(*tensors) -> None:
-    for t in tensors:
-        if not t.is_cuda:
-            raise FusedGemmError("tensors must be on the GPU")
-        if t.get_device() != torch.cuda.current_device():
-            raise FusedGemmError("tensors must be on the current device")
 
 
 def _scale_shape(R: int, K: int) -> tuple[int, int, int]:
@@ -98,10 +90,10 @@ class MxFp4:
         """The values, ``[R, K]``.  Exact in bf16 and fp32; fp16 rounds where its range ends."""
         if dtype not in _TYPES:
             raise FusedGemmError("dtype must be bfloat16, float16 or float32")
-        _check_device(self.data, self.scales)
+        device = device_of(FusedGemmError, self.data, self.scales)
         R, K = self.shape
         out = torch.empty(R, K, dtype=dtype, device=self.data.device)
-        _raise(_lib().bshmem_mxfp4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), R, K, _TYPES[dtype], out.data_ptr(), H.current_stream_handle()),
+        _raise(_lib().bshmem_mxfp4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), R, K, _TYPES[dtype], out.data_ptr(), stream_of(device)),
                "bshmem_mxfp4_dequantize")
         return out
 
@@ -112,20 +104,23 @@ def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
     A block of 32 values along K gets the scale ``2 ** (floor(log2(max|x|)) - 2)``, at least ``2 ** -127``; its values are ``x / scale``
     rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to even) and saturated at 6.  A block with an infinity or a
     NaN gets the scale NaN, and so do all its values."""
+    x, device = _checked(x)
+    R, K = x.shape
+    data = torch.empty((R, K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(_scale_shape(R, K), dtype=torch.uint8, device=x.device)
+    _raise(_lib().bshmem_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], R, K, x.stride(0), data.data_ptr(), scales.data_ptr(), stream_of(device)), "bshmem_mxfp4_quantize")
+    return MxFp4(data, scales, (R, K))
+
+
+def _checked(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`x` as a matrix that can be quantised, and its device."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _TYPES:
         raise FusedGemmError("x must be a [R, K] tensor of bfloat16, float16 or float32")
-    R, K = x.shape
+    K = x.shape[1]
     if K < BLOCK or K % BLOCK:
         raise FusedGemmError(f"K must be a multiple of {BLOCK}, not {K}")
-    _check_device(x)
-    x = x.detach()
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    data = torch.empty(R, K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_shape(R, K), dtype=torch.uint8, device=x.device)
-    _raise(_lib().bshmem_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], R, K, x.stride(0), data.data_ptr(), scales.data_ptr(), H.current_stream_handle()),
-           "bshmem_mxfp4_quantize")
-    return MxFp4(data, scales, (R, K))
+    device = device_of(FusedGemmError, x)
+    return (x if x.stride(1) == 1 else x.contiguous()), device
 
 
 def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -133,22 +128,28 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
     ``x`` that is not quantised yet is quantised in the call (:func:`quantize_mxfp4`).  M and N may be any number."""
     if not isinstance(w, MxFp4):
         raise FusedGemmError("w must be quantised (quantize_mxfp4)")
-    fresh = not isinstance(x, MxFp4)
-    if fresh:
-        x = quantize_mxfp4(x)
-    if x.shape[1] != w.shape[1]:
-        raise FusedGemmError(f"shape mismatch: x {x.shape} w {w.shape}")
-    _check_device(x.data, x.scales, w.data, w.scales)
-    M, N = x.shape[0], w.shape[0]
-    if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=w.data.device)
+    raw = not isinstance(x, MxFp4)
+    if raw:
+        x, _ = _checked(x)
+    (M, K), N = x.shape, w.shape[0]
+    if K != w.shape[1]:
+        raise FusedGemmError(f"shape mismatch: x {tuple(x.shape)} w {w.shape}")
+    dev = w.data.device
+    if raw:
+        device = device_of(FusedGemmError, w.data, w.scales, out)
+        # room for x as it is quantised: the values, then the scales
+        rb, kb, _ = _scale_shape(M, K)
+        room = torch.empty((M * K // 2 + 127) // 128 * 128 + rb * kb * 512, dtype=torch.uint8, device=dev)
+        data = room.data_ptr()
+        operand = data, data + (M * K // 2 + 127) // 128 * 128
+        source = x.data_ptr(), _TYPES[x.dtype], x.stride(0)
     else:
-        _check_device(out)
+        device = device_of(FusedGemmError, x.data, x.scales, w.data, w.scales, out)
+        operand, source = (x.data.data_ptr(), x.scales.data_ptr()), (None, 0, 0)
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    else:
         _check_out(out, M, N)
-    a = _GemmArgs()
-    a.x, a.x_scales, a.w, a.w_scales, a.out = x.data.data_ptr(), x.scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr()
-    a.M, a.N, a.K = M, N, w.shape[1]
-    a.error_flag = _error_flag(out.device).data_ptr()
-    a.w_ready = fresh and M > 0   # the kernel ahead is the one that quantises x; w is older
-    _raise(_lib().bshmem_mxfp4_gemm(C.byref(a), H.current_stream_handle()), "bshmem_mxfp4_gemm")
+    a = _GemmArgs(*operand, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), M, N, K, 0, _error_flag(dev).data_ptr(), *source)
+    _raise(_lib().bshmem_mxfp4_gemm(C.byref(a), stream_of(device)), "bshmem_mxfp4_gemm")
     return out

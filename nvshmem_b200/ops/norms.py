@@ -15,7 +15,7 @@ import ctypes as C
 
 import torch
 
-from ..bindings import host as H
+from ._launch import device_of, first_order, stream_of
 from .fused_gemm import _error_flag, fused_lib
 
 MAX_H = 16384
@@ -58,64 +58,43 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 class _Plan:
     """The settings of a call: everything that is not a tensor."""
-    __slots__ = ("T", "H", "gate_mode", "residual_scale", "branch_scale", "eps", "weight_offset", "dtype")
+    __slots__ = ("T", "H", "device", "gate_mode", "residual_scale", "branch_scale", "eps", "weight_offset", "dtype")
 
-    def args(self, h, residual, post, pre, gate) -> _Args:
-        a = _Args()
-        a.T, a.H, a.gate_mode = self.T, self.H, self.gate_mode
-        a.type, a.res_type = _TYPES[self.dtype], _TYPES[residual.dtype]
+    def launch(self, fn, name, h, residual, post, pre, gate, r=None, y=None, stat=None, dr=None, dy=None, dh=None, dresidual=None, dpost=None, dpre=None,
+               dgate=None, partials=None) -> None:
         wt = post if post is not None else pre if pre is not None else gate
-        a.wt_type = a.type if wt is None else _TYPES[wt.dtype]
-        a.residual_scale, a.branch_scale, a.eps, a.weight_offset = self.residual_scale, self.branch_scale, self.eps, self.weight_offset
-        a.h, a.residual, a.post, a.pre, a.gate = _ptr(h), residual.data_ptr(), _ptr(post), _ptr(pre), _ptr(gate)
-        a.error_flag = _error_flag(residual.device).data_ptr()
-        a.res_stride = residual.stride(0)
-        if h is not None:
-            a.h_stride = h.stride(0)
-        if self.gate_mode == _FULL:
-            a.gate_stride = gate.stride(0)
-        return a
-
-
-def _launch(fn, a: _Args, name: str) -> None:
-    st = fn(C.byref(a), C.c_void_p(H.current_stream_handle()))
-    if st != 0:
-        raise NormError(f"{name}: {_ERRORS.get(st, st)}")
+        t = _TYPES[self.dtype]
+        a = _Args(self.T, self.H, t, _TYPES[residual.dtype], t if wt is None else _TYPES[wt.dtype], self.gate_mode, 0 if h is None else h.stride(0), residual.stride(0),
+                  gate.stride(0) if self.gate_mode == _FULL else 0, 0 if dr is None else dr.stride(0), 0 if dy is None else dy.stride(0), self.residual_scale,
+                  self.branch_scale, self.eps, self.weight_offset, _ptr(h), residual.data_ptr(), _ptr(post), _ptr(pre), _ptr(gate), _ptr(r), _ptr(y), _ptr(stat),
+                  _ptr(dr), _ptr(dy), _ptr(dh), _ptr(dresidual), _ptr(dpost), _ptr(dpre), _ptr(dgate), _error_flag(residual.device).data_ptr(), _ptr(partials))
+        st = fn(C.byref(a), stream_of(self.device))
+        if st != 0:
+            raise NormError(f"{name}: {_ERRORS.get(st, st)}")
 
 
 def _forward(plan: _Plan, h, residual, post, pre, gate, want_r: bool, want_stat: bool):
-    a = plan.args(h, residual, post, pre, gate)
-    dev = residual.device
-    r = torch.empty(plan.T, plan.H, dtype=residual.dtype, device=dev) if want_r else None
-    y = torch.empty(plan.T, plan.H, dtype=plan.dtype, device=dev) if pre is not None else None
-    stat = torch.empty(2, plan.T, dtype=torch.float32, device=dev) if want_stat else None
-    a.r, a.y, a.stat = _ptr(r), _ptr(y), _ptr(stat)
-    _launch(_lib().bshmem_block_norms, a, "bshmem_block_norms")
+    dev, shape = residual.device, (plan.T, plan.H)
+    r = torch.empty(shape, dtype=residual.dtype, device=dev) if want_r else None
+    y = torch.empty(shape, dtype=plan.dtype, device=dev) if pre is not None else None
+    stat = torch.empty((2, plan.T), dtype=torch.float32, device=dev) if want_stat else None
+    plan.launch(_lib().bshmem_block_norms, "bshmem_block_norms", h, residual, post, pre, gate, r, y, stat)
     return r, y, stat
 
 
 def _backward(plan: _Plan, h, residual, post, pre, gate, stat, dr, dy, needs):
     """Gradients of (h, residual, post, pre, gate), None where `needs` is false."""
-    tensors = (h, residual, post, pre, gate)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None for t, need in zip(tensors, needs)]
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None for t, need in zip((h, residual, post, pre, gate), needs)]
     dh, dres, dpost, dpre, dgate = grads
-    if dy is None and dpre is not None:
-        dpre.zero_()
     if plan.T == 0 or (dr is None and dy is None):
         return [g if g is None else g.zero_() for g in grads]
-    a = plan.args(h, residual, post, pre, gate)
-    a.stat = stat.data_ptr()
-    if dr is not None:
-        dr = _rows(dr)
-        a.dr, a.dr_stride = dr.data_ptr(), dr.stride(0)
-    if dy is not None:
-        dy = _rows(dy)
-        a.dy, a.dy_stride = dy.data_ptr(), dy.stride(0)
-    a.dh, a.dresidual, a.dpost, a.dpre, a.dgate = _ptr(dh), _ptr(dres), _ptr(dpost), _ptr(dpre) if dy is not None else None, _ptr(dgate)
+    if dy is None and dpre is not None:
+        dpre.zero_()
+    partials = None
     if dpost is not None or dpre is not None or (dgate is not None and plan.gate_mode == _CHANNEL):
         partials = torch.empty(_lib().bshmem_block_norms_partials(plan.T, plan.H), dtype=torch.float32, device=residual.device)
-        a.partials = partials.data_ptr()
-    _launch(_lib().bshmem_block_norms_backward, a, "bshmem_block_norms_backward")
+    plan.launch(_lib().bshmem_block_norms_backward, "bshmem_block_norms_backward", h, residual, post, pre, gate, None, None, stat, None if dr is None else _rows(dr),
+                None if dy is None else _rows(dy), dh, dres, dpost, None if dy is None else dpre, dgate, partials)
     return grads
 
 
@@ -131,7 +110,7 @@ class _BlockNorms(torch.autograd.Function):
         return tuple(outs) if len(outs) > 1 else outs[0]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, *grads):
         h, residual, post, pre, gate, stat = ctx.saved_tensors
         grads = list(grads)
@@ -161,20 +140,15 @@ def _check_weights(plan: _Plan, **weights) -> None:
             raise NormError(f"{name} must be of shape {(plan.H,)}")
 
 
-def _check_device(*tensors) -> None:
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise NormError("tensors must be on the GPU")
-        if t is not None and t.get_device() != torch.cuda.current_device():
-            raise NormError("tensors must be on the current device")
-
-
 def _run(plan: _Plan, want_r: bool, h, residual, post, pre, gate):
     tensors = (h, residual, post, pre, gate)
-    _check_device(*tensors)
+    plan.device = device_of(NormError, *tensors)
     residual = _rows(residual)
     h = None if h is None else _rows(h)
-    post, pre = (None if w is None else w.contiguous() for w in (post, pre))
+    if post is not None:
+        post = post.contiguous()
+    if pre is not None:
+        pre = pre.contiguous()
     if gate is not None:
         gate = _rows(gate) if plan.gate_mode == _FULL else gate.contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):

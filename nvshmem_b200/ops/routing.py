@@ -13,7 +13,7 @@ import ctypes as C
 
 import torch
 
-from ..bindings import host as H
+from ._launch import device_of, first_order, stream_of
 from .fused_gemm import fused_lib
 
 MAX_EXPERTS, MAX_TOPK = 1024, 16
@@ -43,30 +43,24 @@ def _lib():
     return lib
 
 
-def _launch(fn, a: _Args, name: str) -> None:
-    st = fn(C.byref(a), C.c_void_p(H.current_stream_handle()))
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(fn, name, logits, K, score, renormalize=0, scale=1.0, bias=None, valid=None, idx=None, weight=None, dweight=None, dlogits=None, loss=None, counts=None,
+            coef=None, workspace=None, dloss=None) -> None:
+    T, E = logits.shape
+    a = _Args(T, E, K, _TYPES[logits.dtype], score, renormalize, logits.stride(0), scale, logits.data_ptr(), _ptr(bias), _ptr(valid), _ptr(idx), _ptr(weight), _ptr(dweight),
+              _ptr(dlogits), _ptr(loss), _ptr(counts), coef, workspace, _ptr(dloss))
+    st = fn(C.byref(a), stream_of(logits.get_device()))
     if st != 0:
         raise RoutingError(f"{name}: {_ERRORS.get(st, st)}")
 
 
-def _args(logits: torch.Tensor, K: int, score: int, valid) -> _Args:
-    a = _Args()
-    a.T, a.E = logits.shape
-    a.K, a.type, a.score, a.stride, a.logits = K, _TYPES[logits.dtype], score, logits.stride(0), logits.data_ptr()
-    if valid is not None:
-        a.valid = valid.data_ptr()
-    return a
-
-
 def _route(logits, K, score, bias, renormalize, scale, valid):
-    a = _args(logits, K, score, valid)
-    T = logits.shape[0]
-    idx = torch.empty(T, K, dtype=torch.int32, device=logits.device)
-    weight = torch.empty(T, K, dtype=torch.float32, device=logits.device)
-    a.renormalize, a.scale, a.idx, a.weight = renormalize, scale, idx.data_ptr(), weight.data_ptr()
-    if bias is not None:
-        a.bias = bias.data_ptr()
-    _launch(_lib().bshmem_route, a, "bshmem_route")
+    idx = torch.empty((logits.shape[0], K), dtype=torch.int32, device=logits.device)
+    weight = torch.empty((logits.shape[0], K), dtype=torch.float32, device=logits.device)
+    _launch(_lib().bshmem_route, "bshmem_route", logits, K, score, renormalize, scale, bias, valid, idx, weight)
     return idx, weight
 
 
@@ -81,56 +75,47 @@ class _Route(torch.autograd.Function):
         return idx, weight
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, _, dweight):
         if dweight is None:
             return (None,) * 7
         logits, idx, weight = ctx.saved_tensors
         K, score, renormalize, scale = ctx.settings
-        dweight = dweight.contiguous()
         dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a = _args(logits, K, score, None)
-        a.renormalize, a.scale, a.idx, a.weight = renormalize, scale, idx.data_ptr(), weight.data_ptr()
-        a.dweight, a.dlogits = dweight.data_ptr(), dlogits.data_ptr()
-        _launch(_lib().bshmem_route_backward, a, "bshmem_route_backward")
-        return (dlogits,) + (None,) * 6
+        _launch(_lib().bshmem_route_backward, "bshmem_route_backward", logits, K, score, renormalize, scale, idx=idx, weight=weight, dweight=dweight.contiguous(), dlogits=dlogits)
+        return dlogits, None, None, None, None, None, None
 
 
-def _balance(logits, idx, score, valid, want_coef):
-    a = _args(logits, idx.shape[1], score, valid)
+def _balance(logits, idx, score, valid):
     T, E = logits.shape
     dev = logits.device
     loss, counts = torch.empty((), dtype=torch.float32, device=dev), torch.empty(E, dtype=torch.int32, device=dev)
-    coef = torch.empty(E, dtype=torch.float32, device=dev) if want_coef else None
-    workspace = torch.empty(_lib().bshmem_balance_workspace(T, E), dtype=torch.uint8, device=dev)
-    a.idx, a.loss, a.counts, a.workspace = idx.data_ptr(), loss.data_ptr(), counts.data_ptr(), workspace.data_ptr()
-    if want_coef:
-        a.coef = coef.data_ptr()
-    _launch(_lib().bshmem_balance, a, "bshmem_balance")
-    return loss, counts, coef
+    # dloss / dp per expert (kept for backward), then the kernel's workspace
+    buffer = torch.empty(4 * E + _lib().bshmem_balance_workspace(T, E), dtype=torch.uint8, device=dev)
+    at = buffer.data_ptr()
+    _launch(_lib().bshmem_balance, "bshmem_balance", logits, idx.shape[1], score, valid=valid, idx=idx, loss=loss, counts=counts, coef=at, workspace=at + 4 * E)
+    return loss, counts, buffer
 
 
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, idx, score, valid):
-        loss, counts, coef = _balance(logits, idx, score, valid, True)
-        ctx.save_for_backward(logits, coef, valid)
+        loss, counts, buffer = _balance(logits, idx, score, valid)
+        ctx.save_for_backward(logits, buffer, valid)
         ctx.settings = (idx.shape[1], score)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, dloss, _):
         if dloss is None:
-            return (None,) * 4
-        logits, coef, valid = ctx.saved_tensors
+            return None, None, None, None
+        logits, buffer, valid = ctx.saved_tensors
         dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        a = _args(logits, ctx.settings[0], ctx.settings[1], valid)
-        a.coef, a.dloss, a.dlogits = coef.data_ptr(), dloss.data_ptr(), dlogits.data_ptr()
-        _launch(_lib().bshmem_balance_backward, a, "bshmem_balance_backward")
-        return (dlogits,) + (None,) * 3
+        _launch(_lib().bshmem_balance_backward, "bshmem_balance_backward", logits, *ctx.settings, valid=valid, dlogits=dlogits, coef=buffer.data_ptr(), dloss=dloss)
+        return dlogits, None, None, None
 
 
 def _check(logits, topk, score, valid) -> None:
@@ -145,14 +130,6 @@ def _check(logits, topk, score, valid) -> None:
         raise RoutingError("score is 'softmax' or 'sigmoid'")
     if valid is not None and (valid.dtype != torch.bool or tuple(valid.shape) != (T,)):
         raise RoutingError(f"valid must be a bool tensor of shape {(T,)}")
-
-
-def _check_device(*tensors) -> None:
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise RoutingError("tensors must be on the GPU")
-        if t is not None and t.get_device() != torch.cuda.current_device():
-            raise RoutingError("tensors must be on the current device")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -171,9 +148,10 @@ def moe_route(logits: torch.Tensor, topk: int, score: str = "softmax", bias: tor
     _check(logits, topk, score, valid)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (logits.shape[1],)):
         raise RoutingError(f"bias must be float32 of shape {(logits.shape[1],)}")
-    _check_device(logits, bias, valid)
+    device_of(RoutingError, logits, bias, valid)
     logits = _rows(logits)
-    bias, valid = (None if t is None else t.detach().contiguous() for t in (bias, valid))
+    bias = None if bias is None else bias.detach().contiguous()
+    valid = None if valid is None else valid.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Route.apply(logits, topk, SCORES[score], bias, int(renormalize), float(scale), valid)
     return _route(logits, topk, SCORES[score], bias, int(renormalize), float(scale), valid)
@@ -193,9 +171,9 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, score: str = "softmax"
     _check(logits, idx.shape[1], score, valid)
     if idx.shape[0] != logits.shape[0]:
         raise RoutingError(f"idx is of {idx.shape[0]} tokens, logits of {logits.shape[0]}")
-    _check_device(logits, idx, valid)
+    device_of(RoutingError, logits, idx, valid)
     logits, idx = _rows(logits), idx.contiguous()
     valid = None if valid is None else valid.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Balance.apply(logits, idx, SCORES[score], valid)
-    return _balance(logits, idx, SCORES[score], valid, False)[:2]
+    return _balance(logits, idx, SCORES[score], valid)[:2]
