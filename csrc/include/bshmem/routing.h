@@ -41,7 +41,7 @@ typedef struct {
   /* balance */
   float* loss;              /* [1] */
   int32_t* counts;          /* [E] */
-  float* coef;              /* [E]: dloss / dp_te = coef_e; written by balance unless null, read by its backward */
+  float* coef;              /* [E]: dloss / dp_te less its mean over e; written by balance unless null, read by its backward */
   void* workspace;          /* bshmem_balance_workspace(T, E) bytes */
   const float* dloss;       /* [1], device */
 } bshmem_route_args_t;

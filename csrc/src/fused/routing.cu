@@ -2,7 +2,9 @@
 //
 // A warp takes a token: lane l holds the logits of experts l, l + 32, ... in registers, so a row is read once in whole lines and
 // everything after that is shuffles.  The choice is K rounds of a maximum over the warp of keys that order like the floats
-// (redux.sync), the lowest expert among equal keys.
+// (redux.sync), the lowest expert among equal keys.  A round is some 50 instructions for 256 experts, half of them on the half-rate integer
+// pipe, which is what bounds many tokens: 8192 x 256 takes 5.1 us with one expert a token and 9.9 us with eight (8.9 MB: 1.4 us of
+// memory time).  A decode batch (64 x 256, top-8) takes 3.0 us, most of it the launch and the chain of rounds.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -30,6 +32,7 @@ __device__ __forceinline__ uint32_t key32(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float value32(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ uint64_t key64(double v) {
   if (!(v > -CUDART_INF)) return 0ull;
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
@@ -60,6 +63,95 @@ __device__ __forceinline__ void load_row(float (&l)[VPL], const T* row, int E, i
     const int e = lane + 32 * i;
     l[i] = e < E ? to_f(row[e]) : -CUDART_INF_F;
   }
+}
+
+// The `rounds` largest of the warp's keys, the lowest expert first among equal ones: lane k gets the k-th as (expert, key), (-1, 0) where none
+// is left.
+template <int VPL>
+__device__ __forceinline__ void select(uint32_t (&key)[VPL], int rounds, int lane, int& expert, uint32_t& its_key) {
+  expert = -1;
+  its_key = 0;
+  for (int k = 0; k < rounds; ++k) {
+    uint32_t best = 0;
+    int e = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        e = lane + 32 * i;
+      }
+    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+    if (most == 0) break;
+    const int chosen = (int)__reduce_min_sync(0xffffffffu, best == most ? (unsigned)e : 0xffffffffu);
+    if (lane == k) {
+      expert = chosen;
+      its_key = most;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (lane + 32 * i == chosen) key[i] = 0;
+  }
+}
+
+// Score + bias of one expert in 64 bits; `sum` is the softmax's.
+__device__ __forceinline__ uint64_t key_of(const bshmem_route_args_t& a, double l, double top, double sum, int e) {
+  const double s = a.score == BSHMEM_ROUTE_SOFTMAX ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l));
+  return l > -CUDART_INF ? key64(s + (double)a.bias[e]) : 0ull;
+}
+template <typename T>
+__device__ __forceinline__ double sum_of(const bshmem_route_args_t& a, const T* row, float top, int lane) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int e = lane; e < a.E; e += 32) sum += exp((double)to_f(row[e]) - (double)top);
+  return warp_sum(sum);
+}
+
+// The experts of lanes 0 to n - 1 (-1: none) in the order of score + bias in 64 bits.
+template <typename T>
+__device__ __noinline__ int order64(const bshmem_route_args_t& a, const T* row, float top, int lane, int expert, int n) {
+  const double sum = a.score == BSHMEM_ROUTE_SOFTMAX ? sum_of(a, row, top, lane) : 1.0;
+  const uint64_t key = lane < n && expert >= 0 ? key_of(a, (double)to_f(row[expert]), (double)top, sum, expert) : 0ull;
+  int rank = 0, from = lane;
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = __shfl_sync(0xffffffffu, key, j);
+    const int e = __shfl_sync(0xffffffffu, expert, j);
+    rank += other > key || (other == key && (e < expert || (e == expert && j < lane)));
+  }
+  for (int j = 0; j < n; ++j)
+    if (__shfl_sync(0xffffffffu, rank, j) == lane) from = j;
+  return __shfl_sync(0xffffffffu, expert, from);
+}
+
+// The whole choice in 64 bits, for the odd token whose K-th, next and next but one lie that close: short code, not fast.
+template <typename T, int VPL>
+__device__ __noinline__ int select64(const bshmem_route_args_t& a, const T* row, float top, int lane) {
+  uint64_t key[VPL];
+  const double sum = a.score == BSHMEM_ROUTE_SOFTMAX ? sum_of(a, row, top, lane) : 1.0;
+  int expert = -1;
+#pragma unroll 1
+  for (int i = 0; i < VPL; ++i) {
+    const int e = lane + 32 * i;
+    key[i] = e < a.E ? key_of(a, (double)to_f(row[e]), (double)top, sum, e) : 0ull;
+  }
+#pragma unroll 1
+  for (int k = 0; k < a.K; ++k) {
+    uint64_t best = 0;
+    int at = 0;
+#pragma unroll 1
+    for (int i = 0; i < VPL; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
+    const uint32_t most = __reduce_max_sync(0xffffffffu, hi);
+    if (most == 0) break;  // the high half of a key of a finite number is never 0
+    const uint32_t most_lo = __reduce_max_sync(0xffffffffu, hi == most ? lo : 0u);
+    const int chosen = (int)__reduce_min_sync(0xffffffffu, hi == most && lo == most_lo ? (unsigned)(lane + 32 * at) : 0xffffffffu);
+    if (lane == k) expert = chosen;
+    if (lane + 32 * at == chosen) key[at] = 0;
+  }
+  return expert;
 }
 
 // Numerator of a score whose sum over a set of experts is divided out.  `top` is the largest logit of the set:
@@ -99,68 +191,38 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
     top = fmaxf(top, l[i]);
   }
   nan = __any_sync(0xffffffffu, nan);
-  int mine = -1;  // lane k: the k-th chosen expert
+  top = warp_max(top);
+  int mine;  // lane k: the k-th chosen expert
+  uint32_t key[VPL], mine_key;
   if constexpr (!BIAS) {
-    uint32_t key[VPL];
 #pragma unroll
     for (int i = 0; i < VPL; ++i) key[i] = key32(l[i]);
-    for (int k = 0; k < K; ++k) {
-      uint32_t best = 0;
-      int e = 0;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (key[i] > best) {
-          best = key[i];
-          e = lane + 32 * i;
-        }
-      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-      if (most == 0) break;
-      const int chosen = (int)__reduce_min_sync(0xffffffffu, best == most ? (unsigned)e : 0xffffffffu);
-      if (lane == k) mine = chosen;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (lane + 32 * i == chosen) key[i] = 0;
-    }
-    top = warp_max(top);
+    select(key, K, lane, mine, mine_key);
   } else {
-    top = warp_max(top);
-    uint64_t key[VPL];
-    double s[VPL], sum = 0.0;
+    // Score + bias in 32 bits with the fast exponential and division first.  They and the sum of up to 37 terms are off by less than 4e-6
+    // of a score, which is at most 1, and the sum with the bias by half a step.  Where two neighbours in the order are closer than twice
+    // that (two tokens in a hundred), the choice is made in 64 bits.  8192 x 256, top-8: 16.6 us; all in 64 bits 20; 9.9 without a bias.
+    float s[VPL], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      if (a.score == BSHMEM_ROUTE_SOFTMAX) s[i] = l[i] > -CUDART_INF_F ? exp((double)l[i] - (double)top) : 0.0;
-      else s[i] = 1.0 / (1.0 + exp(-(double)l[i]));
+      if (a.score == BSHMEM_ROUTE_SOFTMAX) s[i] = l[i] > -CUDART_INF_F ? __expf(l[i] - top) : 0.f;
+      else s[i] = __fdividef(1.f, 1.f + __expf(-l[i]));  // 0 from where the divisor passes 2^126 on
       sum += s[i];
     }
-    if (a.score == BSHMEM_ROUTE_SOFTMAX) {
-      sum = warp_sum(sum);
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) s[i] /= sum;
-    }
+    const float inv = a.score == BSHMEM_ROUTE_SOFTMAX ? 1.f / warp_sum(sum) : 1.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = lane + 32 * i;
-      key[i] = e < E && l[i] > -CUDART_INF_F ? key64(s[i] + (double)a.bias[e]) : 0ull;
+      key[i] = e < E && l[i] > -CUDART_INF_F ? key32(s[i] * inv + a.bias[e]) : 0u;
     }
-    for (int k = 0; k < K; ++k) {
-      uint64_t best = 0;
-      int e = 0;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (key[i] > best) {
-          best = key[i];
-          e = lane + 32 * i;
-        }
-      const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
-      const uint32_t most = __reduce_max_sync(0xffffffffu, hi);
-      if (most == 0) break;  // the high half of a key of a finite number is never 0
-      const uint32_t most_lo = __reduce_max_sync(0xffffffffu, hi == most ? lo : 0u);
-      const int chosen = (int)__reduce_min_sync(0xffffffffu, hi == most && lo == most_lo ? (unsigned)e : 0xffffffffu);
-      if (lane == k) mine = chosen;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (lane + 32 * i == chosen) key[i] = 0;
-    }
+    const int rounds = K + 2;
+    select(key, rounds, lane, mine, mine_key);
+    const uint32_t next = __shfl_down_sync(0xffffffffu, mine_key, 1);
+    const float v = value32(mine_key);
+    const unsigned unclear = __ballot_sync(0xffffffffu, lane <= K && mine_key && next && !(v - value32(next) > 1e-5f + 5e-7f * fabsf(v)));
+    if ((unclear >> (K - 1) & 3) == 3) mine = select64<T, VPL>(a, row, top, lane);  // what was not picked may belong to the K, too
+    else if (unclear & ((1u << K) - 1)) mine = order64(a, row, top, lane, mine, rounds);
+    if (lane >= K) mine = -1;
   }
   float w = 0.f;
   if (a.renormalize) {
@@ -179,7 +241,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
   } else if (mine >= 0) {
     w = sigmoid(to_f(row[mine]));
   }
-  if (nan && a.score == BSHMEM_ROUTE_SOFTMAX && mine >= 0) w = CUDART_NAN_F;  // the sum over all experts is NaN
+  if ((nan || top == CUDART_INF_F) && a.score == BSHMEM_ROUTE_SOFTMAX) w = CUDART_NAN_F;  // the sum over all experts is NaN
   if (lane < K) {
     a.idx[t * K + lane] = mine;
     a.weight[t * K + lane] = w * a.scale;
@@ -276,74 +338,139 @@ __host__ __device__ __forceinline__ Workspace workspace(void* base, int grid, in
   return w;
 }
 
-template <typename T, int VPL>
-__global__ void __launch_bounds__(THREADS) balance_kernel(const __grid_constant__ Params p) {
-  const bshmem_route_args_t& a = p.a;
-  __shared__ int s_count[32 * VPL];
-  __shared__ float s_p[WARPS][32 * VPL];
-  __shared__ int s_n;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K, E = a.E;
-  for (int e = threadIdx.x; e < 32 * VPL; e += THREADS) s_count[e] = 0;
-  if (threadIdx.x == 0) s_n = 0;
-  __syncthreads();
-  float acc[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
-  int n = 0;
-  for (long t = (long)blockIdx.x * WARPS + warp; t < a.T; t += (long)gridDim.x * WARPS) {
-    if (a.valid && !a.valid[t]) continue;
-    ++n;
-    float l[VPL], unused[1];
-    load_row(l, (const T*)a.logits + t * a.stride, E, lane);
-    if (lane < K) {
-      const int e = a.idx[t * K + lane];
-      if (e >= 0 && e < E) atomicAdd(&s_count[e], 1);
-    }
-    probabilities<VPL, false>(l, unused, a.score);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) acc[i] += l[i];
-  }
-  if (lane == 0 && n) atomicAdd(&s_n, n);
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) s_p[warp][lane + 32 * i] = acc[i];
-  __syncthreads();
-  const Workspace w = workspace(a.workspace, gridDim.x, E);
-  for (int e = threadIdx.x; e < E; e += THREADS) {
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) s += s_p[k][e];
-    w.p[(size_t)blockIdx.x * E + e] = s;
-    w.counts[(size_t)blockIdx.x * E + e] = s_count[e];
-  }
-  if (threadIdx.x == 0) w.n[blockIdx.x] = s_n;
+// What an expert of probability sum `p` and count `c` over n tokens adds to the loss; writes its count and dloss / dp, from which the
+// mean over the experts is taken off: it drops out of the gradient (the probabilities of a token sum to 1), and its rounding with it.
+__device__ __forceinline__ float finish_expert(const bshmem_route_args_t& a, int e, float p, int c, int n, int all) {
+  const double nn = n > 0 ? (double)n : 1.0, scale = (double)a.E / (a.K * nn * nn);
+  a.counts[e] = c;
+  if (a.coef) a.coef[e] = (float)(scale * ((double)c - (double)all / a.E));
+  return (float)(scale * c) * p;
 }
 
-// Adds the CTAs' sums in order and forms the loss.  One CTA of 1024 threads.
-__global__ void __launch_bounds__(1024) balance_finish_kernel(const __grid_constant__ Params p, int parts) {
+constexpr int B_THREADS = 512, B_WARPS = B_THREADS / 32;
+constexpr int ONE_CTA_TOKENS = 8 * B_WARPS;   // up to here one CTA does all: 61 x 40 in 5.4 us; two kernels took 2.9 + 3.2 us and a second launch
+
+template <typename T, int VPL>
+__global__ void __launch_bounds__(B_THREADS) balance_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the finishing kernel waits for this one itself
   const bshmem_route_args_t& a = p.a;
-  __shared__ int s_n;
+  __shared__ int s_count[32 * VPL];
+  __shared__ float s_p[B_WARPS][32 * VPL <= 512 ? 32 * VPL : 1];  // up to 512 experts; beyond, warps add up in turn
+  __shared__ float s_sum[32 * VPL <= 512 ? 1 : 32 * VPL];
+  __shared__ int s_n, s_all;
+  __shared__ float s_loss[B_WARPS];
+  constexpr bool TURNS = 32 * VPL > 512;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K, E = a.E;
+  for (int e = threadIdx.x; e < 32 * VPL; e += B_THREADS) {
+    s_count[e] = 0;
+    if (TURNS) s_sum[e] = 0.f;
+  }
+  if (threadIdx.x == 0) s_n = s_all = 0;
+  __syncthreads();
+  float acc[VPL], l[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+  int n = 0, found = 0;
+  const long first = (long)blockIdx.x * B_WARPS + warp, step = (long)gridDim.x * B_WARPS;
+  auto fetch = [&](long t) {
+    if (t < a.T) load_row(l, (const T*)a.logits + t * a.stride, E, lane);
+  };
+  fetch(first);
+  for (long t = first; t < a.T; t += step) {
+    float q[VPL], unused[1];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) q[i] = l[i];
+    fetch(t + step);   // on the way while this token is worked on
+    if (a.valid && !a.valid[t]) continue;
+    ++n;
+    if (lane < K) {
+      const int e = a.idx[t * K + lane];
+      if (e >= 0 && e < E) {
+        atomicAdd(&s_count[e], 1);
+        ++found;
+      }
+    }
+    probabilities<VPL, false>(q, unused, a.score);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) acc[i] += q[i];
+  }
+  found = __reduce_add_sync(0xffffffffu, found);
+  if (lane == 0 && n) atomicAdd(&s_n, n);
+  if (lane == 0 && found) atomicAdd(&s_all, found);
+  if constexpr (TURNS) {
+    for (int k = 0; k < B_WARPS; ++k) {
+      if (k == warp)
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) s_sum[lane + 32 * i] += acc[i];
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s_p[warp][lane + 32 * i] = acc[i];
+    __syncthreads();
+  }
+  const Workspace w = workspace(a.workspace, gridDim.x, E);
+  float term = 0.f;
+  for (int e = threadIdx.x; e < E; e += B_THREADS) {
+    float s = 0.f;
+    if constexpr (TURNS) {
+      s = s_sum[e];
+    } else {
+#pragma unroll
+      for (int k = 0; k < B_WARPS; ++k) s += s_p[k][e];
+    }
+    if (gridDim.x == 1) {
+      term += finish_expert(a, e, s, s_count[e], s_n, s_all);
+    } else {
+      w.p[(size_t)blockIdx.x * E + e] = s;
+      w.counts[(size_t)blockIdx.x * E + e] = s_count[e];
+    }
+  }
+  if (gridDim.x > 1) {
+    if (threadIdx.x == 0) w.n[blockIdx.x] = s_n;
+    return;
+  }
+  term = warp_sum(term);
+  if (lane == 0) s_loss[warp] = term;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < B_WARPS; ++k) term += s_loss[k];
+    *a.loss = term;
+  }
+}
+
+// Adds the CTAs' sums in order and forms the loss.  One CTA of 1024 threads; each column's CTAs are divided among 1024 / E of them.
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const __grid_constant__ Params p, int parts) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bshmem_route_args_t& a = p.a;
+  __shared__ int s_n, s_all;
   __shared__ float s_loss[32];
   __shared__ float s_p[1024];
   __shared__ int s_c[1024];
   const Workspace w = workspace(a.workspace, parts, a.E);
-  if (threadIdx.x == 0) s_n = 0;
-  __syncthreads();
-  int n = 0;
-  for (int k = threadIdx.x; k < parts; k += blockDim.x) n += w.n[k];
-  if (n) atomicAdd(&s_n, n);
-  // `lanes` threads of a column each add a part of the CTAs
+  if (threadIdx.x == 0) s_n = s_all = 0;
   int cols = 32;
   while (cols < a.E) cols *= 2;
   const int slices = 1024 / cols, e = threadIdx.x % cols, slice = threadIdx.x / cols;
   float ps = 0.f;
-  int cs = 0;
-  if (e < a.E)
+  int cs = 0, n = 0;
+  if (e < a.E) {
+#pragma unroll 8
     for (int k = slice; k < parts; k += slices) {
       ps += w.p[(size_t)k * a.E + e];
       cs += w.counts[(size_t)k * a.E + e];
     }
+  }
+  for (int k = threadIdx.x; k < parts; k += 1024) n += w.n[k];
   s_p[threadIdx.x] = ps;
   s_c[threadIdx.x] = cs;
+  __syncthreads();
+  const int all = __reduce_add_sync(0xffffffffu, cs);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) {
+    if (all) atomicAdd(&s_all, all);
+    if (n) atomicAdd(&s_n, n);
+  }
   __syncthreads();
   float term = 0.f;
   if (slice == 0 && e < a.E) {
@@ -351,11 +478,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const __grid_const
       ps += s_p[k * cols + e];
       cs += s_c[k * cols + e];
     }
-    const double nn = s_n > 0 ? (double)s_n : 1.0;
-    const float coef = (float)((double)a.E * cs / (a.K * nn * nn));
-    a.counts[e] = cs;
-    if (a.coef) a.coef[e] = coef;
-    term = coef * ps;
+    term = finish_expert(a, e, ps, cs, s_n, s_all);
   }
   term = warp_sum(term);
   if ((threadIdx.x & 31) == 0) s_loss[threadIdx.x >> 5] = term;
@@ -366,7 +489,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const __grid_const
   }
 }
 
-// dl_e = dloss p_e (coef_e - sum_j p_j coef_j), for sigmoids times (1 - s_e).
+// dl_e = dloss p_e (coef_e - sum_j p_j coef_j), for sigmoids times (1 - s_e); coef up to a constant.
 template <typename T, int VPL>
 __global__ void __launch_bounds__(THREADS) balance_backward_kernel(const __grid_constant__ Params p) {
   const bshmem_route_args_t& a = p.a;
@@ -407,8 +530,9 @@ static int balance_ctas(int T) {
   int device = 0, sms = 0;
   cudaGetDevice(&device);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  const int want = (T + WARPS - 1) / WARPS, most = sms > 0 ? sms : 1;
-  return want < 1 ? 1 : want < most ? want : most;
+  if (T <= ONE_CTA_TOKENS) return 1;
+  const int want = (T + B_WARPS - 1) / B_WARPS, most = sms > 0 ? sms : 1;
+  return want < most ? want : most;
 }
 
 // Calls f<T, VPL> for the type and the number of experts.
@@ -455,9 +579,18 @@ struct Balance {
   template <typename T, int VPL>
   int operator()() const {
     const int grid = balance_ctas(p.a.T);
-    balance_kernel<T, VPL><<<grid, THREADS, 0, stream>>>(p);
-    balance_finish_kernel<<<1, 1024, 0, stream>>>(p, grid);
-    return launched();
+    balance_kernel<T, VPL><<<grid, B_THREADS, 0, stream>>>(p);
+    if (grid == 1) return launched();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, balance_finish_kernel, p, grid) == cudaSuccess ? BSHMEM_ROUTE_OK : BSHMEM_ROUTE_ERR_DRIVER;
   }
 };
 struct BalanceBackward {

@@ -104,6 +104,33 @@ def test_ties_go_to_the_lowest_expert(bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("E", [24, 256, 1000])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_scores_that_32_bits_do_not_tell_apart(E, score):
+    """Score + bias of neighbouring experts differ by 1e-9 to 1e-6, in shuffled order: the choice is that of 64 bits."""
+    from nvshmem_b200.ops import routing
+    g = torch.Generator().manual_seed(E)
+    l = torch.randn(60, E, generator=g)
+    p = (torch.softmax(l.double(), -1) if score == "softmax" else torch.sigmoid(l.double()))[0]
+    l = l[:1] + torch.zeros(60, 1)
+    l[30:] += torch.randn(30, 1, generator=g) if score == "softmax" else 0.0
+    gap = torch.rand(E, generator=g).double() * 3 - 9
+    bias = (0.9 - p + torch.randperm(E, generator=g).double() * 10 ** gap).float()
+    _check_route(l.cuda(), min(E, 16), score, bias.cuda())
+
+
+@pytest.mark.gpu
+def test_biased_softmax_of_bad_logits():
+    from nvshmem_b200.ops import routing
+    l, b = _logits(3, 20, F32), torch.zeros(20, device="cuda")
+    clean = routing.moe_route(l, 3, bias=b)
+    l[1, 4], l[2, 6] = float("nan"), math.inf
+    idx, w = routing.moe_route(l, 3, bias=b)
+    assert torch.equal(idx[0], clean[0][0]) and torch.equal(w[0], clean[1][0]) and w[1:].isnan().all()
+    assert not (idx[1] == 4).any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("renormalize", [True, False])
