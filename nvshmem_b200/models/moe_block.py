@@ -1,7 +1,8 @@
 """Expert-parallel mixture-of-experts block on the fused dispatch / combine kernels.
 
 Each rank holds ``E / npes`` experts (a gated MLP each).  ``forward(x)``:
-router logits -> softmax -> top-k -> ``MoeDispatchCombine.dispatch`` (tokens travel to the ranks of
+router logits -> softmax -> top-k (plain torch, or ``ops.routing.moe_route`` in one kernel with
+``router="fused"``) -> ``MoeDispatchCombine.dispatch`` (tokens travel to the ranks of
 their experts, grouped by expert) -> the local experts' MLPs over their row groups -> ``combine``
 (the weighted sum comes back to the token's rank).  The experts run as two grouped GEMMs on the
 tcgen05 kernel (``ops.fused_gemm.grouped_gemm``): the group boundaries stay on the device, the gated
@@ -17,11 +18,20 @@ import torch
 
 from ..ops import fused_gemm as fg
 from ..ops.moe import MoeDispatchCombine
+from ..ops.routing import moe_route
 
 
 class ExpertParallelMoE(torch.nn.Module):
-    def __init__(self, tokens: int, hidden: int, ffn: int, experts: int, topk: int, payload: str = "bf16", seed: int = 0, wait_limit_ms: int = 0):
+    """``router``: "torch" (softmax and topk of torch; ties in torch's order) or "fused" (:func:`~nvshmem_b200.ops.routing.moe_route`: ties
+    go to the lowest expert).  The fused router also takes sigmoid scores (``score``) and a bias per expert for the choice
+    (:attr:`router_bias`, fp32 ``[experts]``, None at first)."""
+
+    def __init__(self, tokens: int, hidden: int, ffn: int, experts: int, topk: int, payload: str = "bf16", seed: int = 0, wait_limit_ms: int = 0,
+                 router: str = "torch", score: str = "softmax"):
         super().__init__()
+        if router not in ("torch", "fused") or (router == "torch" and score != "softmax"):
+            raise ValueError("router is 'torch' (softmax scores) or 'fused'")
+        self.fused_router, self.score, self.router_bias = router == "fused", score, None
         from .. import core
         self.rank, self.npes = core.my_pe(), core.n_pes()
         self.T, self.H, self.F, self.E, self.K = tokens, hidden, ffn, experts, topk
@@ -48,10 +58,12 @@ class ExpertParallelMoE(torch.nn.Module):
 
     def route(self, x: torch.Tensor):
         if self.T % 128 == 0 and self.E % 256 == 0 and self.H % 64 == 0:
-            logits = fg.gemm(x, self.router).float()   # the router is a GEMM like any other
+            logits = fg.gemm(x, self.router)   # the router is a GEMM like any other
         else:
-            logits = (x @ self.router.t()).float()
-        weight, idx = logits.softmax(-1).topk(self.K, dim=-1)
+            logits = x @ self.router.t()
+        if self.fused_router:
+            return moe_route(logits, self.K, score=self.score, bias=self.router_bias)
+        weight, idx = logits.float().softmax(-1).topk(self.K, dim=-1)
         weight = weight / weight.sum(-1, keepdim=True)
         return idx.to(torch.int32).contiguous(), weight.contiguous()
 

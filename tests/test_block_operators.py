@@ -1,0 +1,258 @@
+"""The operators around a block as they are used together: norm, router, exchange, experts, norm with gate and residual, 4-bit product;
+a training step of router, balance loss and norms; all of it captured and replayed, on other streams and side by side."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def nv():
+    import nvshmem_b200.core as nv
+    torch.cuda.set_device(0)
+    nv.init(device=0, uid=nv.get_unique_id(), rank=0, nranks=1)
+    yield nv
+    nv.finalize()
+
+
+def _rms(v, w, eps=1e-6):
+    return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * w
+
+
+class _Layer:
+    """A mixture-of-experts layer between its norms, and a product in 4 bits behind it."""
+
+    def __init__(self, T, H=512, F=256, E=8, K=2, N=384):
+        from nvshmem_b200.ops import fused_gemm as fg
+        from nvshmem_b200.ops.moe import MoeDispatchCombine
+        from nvshmem_b200.ops.mxfp4 import quantize_mxfp4
+        g = torch.Generator(device="cuda").manual_seed(T)
+        rn = lambda *s, scale=1.0: (torch.randn(*s, device="cuda", generator=g) * scale).to(BF16)
+        self.T, self.H, self.F, self.E, self.K = T, H, F, E, K
+        self.pre, self.post, self.nxt = (1 + rn(H, scale=0.1) for _ in range(3))
+        self.gate, self.router = 0.5 + rn(H, scale=0.1), rn(E, H, scale=H ** -0.5)
+        self.w_in, self.w_out, w = rn(E, 2 * F, H, scale=H ** -0.5), rn(E, H, F, scale=F ** -0.5), rn(N, H, scale=H ** -0.5)
+        self.gated, self.w4 = fg.interleave_gate_up(self.w_in), quantize_mxfp4(w)
+        self.moe = MoeDispatchCombine(T, H, K, E)
+        self.act = torch.empty(self.moe.cap_rows, F, dtype=BF16, device="cuda")
+
+    def __call__(self, x, valid):
+        from nvshmem_b200.ops import balance_loss, block_norms, gemm_mxfp4, moe_route, rms_norm
+        from nvshmem_b200.ops import fused_gemm as fg
+        y = rms_norm(x, self.pre)
+        logits = y @ self.router.t()
+        idx, weight = moe_route(logits, self.K, valid=valid)
+        loss, counts = balance_loss(logits, idx, valid=valid)
+        recv, offsets = self.moe.dispatch(y, idx)
+        fg.grouped_gemm(recv, self.gated, offsets, out=self.act, act="swiglu")
+        fg.grouped_gemm(self.act, self.w_out, offsets, out=self.moe.expert_out)
+        h = self.moe.combine(idx, weight)
+        r, z = block_norms(h, x, self.post, self.nxt, self.gate, residual_scale=0.5, branch_scale=2.0)
+        return {"idx": idx, "weight": weight, "loss": loss, "counts": counts, "r": r, "z": z, "out": gemm_mxfp4(z, self.w4)}
+
+
+@pytest.mark.parametrize("T", [1, 61, 192])
+def test_a_layer_of_them(nv, T):
+    """Against plain fp32.  The chain rounds to bf16 at the norm (2^-8 half a step, relative), the experts' activation and output, the
+    combine, r and z: six roundings, 6 * 2^-8 of a value's scale, taken at the largest value of the result."""
+    from nvshmem_b200.ops import fused_gemm as fg
+    layer = _Layer(T)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(T, layer.H, device="cuda", generator=g).to(BF16)
+    valid = torch.arange(T, device="cuda") < max(1, T - 5)
+    got = layer(x, valid)
+    torch.cuda.synchronize()
+    fg.check_errors()
+    # the plain form, from the same choice (the logits are a library product in bf16: its borders may fall either way)
+    y = _rms(x.float(), layer.pre.float()).to(BF16).float()
+    logits = y @ layer.router.float().t()
+    idx, w = got["idx"].long(), got["weight"]
+    assert (idx[~valid] == -1).all() and not w[~valid].any() and int(got["counts"].sum()) == int(valid.sum()) * layer.K
+    chosen = logits.gather(-1, idx.clamp(min=0))
+    assert ((chosen.softmax(-1) - w).abs()[valid] <= 0.05).all()
+    h = torch.zeros(T, layer.H, device="cuda")
+    for e in range(layer.E):
+        tok, slot = (idx == e).nonzero(as_tuple=True)
+        a = y[tok] @ layer.w_in[e].float().t()
+        a = torch.nn.functional.silu(a[:, :layer.F]) * a[:, layer.F:]
+        h.index_add_(0, tok, (a @ layer.w_out[e].float().t()) * w[tok, slot].unsqueeze(-1))
+    r = 0.5 * x.float() + 2.0 * layer.gate.float() * _rms(h, layer.post.float())
+    z = _rms(r, layer.nxt.float())
+    for name, want in (("r", r), ("z", z)):
+        err = (got[name].float() - want).abs().max()
+        assert err <= 6 * 2.0 ** -8 * want.abs().max(), (name, err)
+    # the rows behind the valid ones got nothing from the experts
+    assert torch.equal(got["r"][~valid].float(), (0.5 * x[~valid].float()).to(BF16).float())
+    from nvshmem_b200.ops.mxfp4 import quantize_mxfp4
+    want = quantize_mxfp4(got["z"]).dequantize(F32) @ layer.w4.dequantize(F32).t()
+    assert (got["out"].float() - want).abs().max() <= 2.0 ** -8 * want.abs().max() + 1e-5
+    layer.moe.close()
+
+
+@pytest.mark.parametrize("T", [61, 192])
+def test_a_layer_captured_and_replayed(nv, T):
+    from nvshmem_b200.ops import fused_gemm as fg
+    layer = _Layer(T)
+    x, valid = torch.empty(T, layer.H, dtype=BF16, device="cuda"), torch.empty(T, dtype=torch.bool, device="cuda")
+
+    def fill(seed):
+        torch.manual_seed(seed)
+        x.copy_(torch.randn(T, layer.H, device="cuda"))
+        valid.copy_(torch.rand(T, device="cuda") > 0.2)
+
+    fill(0)
+    layer(x, valid)
+    graphs = []
+    for _ in range(2):   # two graphs of the same calls, replayed in turn
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                out = layer(x, valid)
+        graphs.append((graph, out))
+    torch.cuda.synchronize()
+    for seed in (1, 2, 3):
+        fill(seed)
+        want = {k: v.clone() for k, v in layer(x, valid).items()}
+        graph, out = graphs[seed % 2]
+        for v in out.values():
+            v.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        fg.check_errors()
+        for k in want:
+            assert torch.equal(out[k], want[k]), k
+    layer.moe.close()
+
+
+def _step(d, K):
+    """Loss and gradients of a small training step: norm, router, weights, balance loss, norm with gate and residual."""
+    from nvshmem_b200.ops import balance_loss, block_norms, moe_route, rms_norm
+    y = rms_norm(d["x"], d["pre"])
+    logits = y @ d["router"].t()
+    idx, weight = moe_route(logits, K, score="sigmoid", renormalize=True, scale=1.5)
+    loss, counts = balance_loss(logits, idx)
+    r, z = block_norms(y * weight.sum(-1, keepdim=True) * weight[:, :1], d["x"], d["post"], d["nxt"], d["gate"])
+    total = loss + (r * d["dr"]).mean() + (z * d["dr"]).mean()
+    names = ("x", "pre", "router", "post", "nxt", "gate")
+    return (total, counts, idx, *torch.autograd.grad(total, [d[n] for n in names]))
+
+
+def _training_data(T, H, E, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rn = lambda *s, scale=1.0, shift=0.0: torch.randn(*s, device="cuda", generator=g) * scale + shift
+    d = {"x": rn(T, H), "pre": rn(H, scale=0.1, shift=1.0), "router": rn(E, H, scale=H ** -0.5), "post": rn(H, scale=0.1, shift=1.0), "nxt": rn(H, scale=0.1, shift=1.0),
+         "gate": rn(T, 1, scale=0.1, shift=0.5)}
+    return {**{k: v.requires_grad_(True) for k, v in d.items()}, "dr": rn(T, H)}
+
+
+@pytest.mark.parametrize("T,H,E,K", [(37, 96, 12, 3), (700, 1024, 64, 6)])
+def test_a_training_step_against_64_bits(T, H, E, K):
+    """Every operator is in fp32 here, off by some 2^-18 of the parts it adds; the chain of six of them, with products between in fp32
+    over H terms, stays below 2^-12 of the largest value of each gradient."""
+    d = _training_data(T, H, E, 5)
+    total, counts, idx, *grads = _step(d, K)
+    names = ("x", "pre", "router", "post", "nxt", "gate")
+    v = {n: d[n].detach().double().requires_grad_(True) for n in names}
+    y = _rms(v["x"], v["pre"])
+    logits = y @ v["router"].t()
+    s = torch.sigmoid(logits)
+    w = s.gather(-1, idx.long())
+    w = 1.5 * w / w.sum(-1, keepdim=True)
+    p = torch.softmax(logits, -1)   # the balance loss takes softmax scores unless told otherwise
+    n = torch.bincount(idx.flatten().long(), minlength=E)
+    loss = E * (n.double() / (T * K) * p.mean(0)).sum()
+    r = v["x"] + v["gate"] * _rms(y * w.sum(-1, keepdim=True) * w[:, :1], v["post"])
+    z = _rms(r, v["nxt"])
+    ref = loss + (r * d["dr"]).mean() + (z * d["dr"]).mean()
+    assert torch.equal(counts.long(), n) and abs(total.double() - ref) <= 2.0 ** -12 * abs(ref)
+    for name, got, want in zip(names, grads, torch.autograd.grad(ref, [v[k] for k in names])):
+        assert (got.double() - want).abs().max() <= 2.0 ** -12 * want.abs().max(), name
+
+
+def test_a_training_step_captured_and_replayed():
+    """Forward and backward in one graph, on leaves of its own, replayed on new values."""
+    T, H, E, K = 600, 1024, 64, 6
+    d = _training_data(T, H, E, 1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _step(d, K)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = _step(d, K)
+    torch.cuda.synchronize()
+    for seed in (2, 3):
+        fresh = _training_data(T, H, E, seed)
+        with torch.no_grad():
+            for k in d:
+                d[k].copy_(fresh[k])
+        want = [t.detach().clone() for t in _step(fresh, K)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(out, want):
+            assert torch.equal(got, ref)
+
+
+def test_calls_on_two_streams_at_once(nv):
+    """The same operators on two streams side by side give what they give alone: nothing is shared between calls."""
+    from nvshmem_b200.ops import balance_loss, block_norms, gemm_mxfp4, moe_route, quantize_mxfp4
+
+    def calls(d):
+        r, z = block_norms(d["h"], d["x"], d["w"], d["w"], d["w"])
+        idx, weight = moe_route(z[:, :64], 4)
+        loss, counts = balance_loss(z[:, :64], idx)
+        q = quantize_mxfp4(z)
+        return [r, z, idx, weight, loss, counts, q.data, gemm_mxfp4(z, d["q"]), gemm_mxfp4(z[:20], d["q"])]
+
+    data = []
+    for seed in (1, 2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF16)
+        data.append({"h": rn(700, 2048), "x": rn(700, 2048), "w": rn(2048), "q": quantize_mxfp4(rn(1024, 2048))})
+    want = [[t.clone() for t in calls(d)] for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for _ in range(5):
+        got = []
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(calls(d))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for t, ref in zip(a, b):
+                assert torch.equal(t, ref)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_moe_block_with_the_fused_router(nv, score):
+    from nvshmem_b200.models import ExpertParallelMoE
+    from nvshmem_b200.ops import fused_gemm as fg
+    T, H, F, E, K = 192, 256, 384, 8, 2
+    plain = ExpertParallelMoE(T, H, F, E, K, seed=3)
+    block = ExpertParallelMoE(T, H, F, E, K, seed=3, router="fused", score=score)
+    torch.manual_seed(17)
+    x = torch.randn(T, H, device="cuda").to(BF16)
+    idx, weight = block.route(x)
+    pidx, pweight = plain.route(x)
+    logits = x @ block.router.t()
+    clear = logits.float().sort(-1, descending=True).values[:, :K + 1].diff(dim=-1).abs().min(-1).values > 0   # tokens without equal logits at the border
+    assert torch.equal(idx[clear], pidx[clear]) and clear.float().mean() > 0.9
+    if score == "softmax":
+        assert (weight - pweight)[clear].abs().max() <= 1e-6
+        got, want = block(x)[clear], plain(x)[clear]
+        assert torch.equal(got, want) or (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+    block.router_bias = torch.zeros(E, device="cuda")
+    block.router_bias[3] = 100.0
+    assert (block.route(x)[0][:, 0] == 3).all()
+    torch.cuda.synchronize()
+    fg.check_errors()
+    plain.close()
+    block.close()
+    with pytest.raises(ValueError):
+        ExpertParallelMoE(T, H, F, E, K, score="sigmoid")
