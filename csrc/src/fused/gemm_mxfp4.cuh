@@ -49,6 +49,7 @@ struct alignas(64) PairParams {
   uint64_t wait_limit_ns;
   int M, N, K;
   int tiles_m, tiles;   // row tiles run fastest
+  __nv_bfloat16* direct;  // not null: rows of the output are no whole 16-byte units, and are stored value by value
 };
 
 template <int COLS>
@@ -190,9 +191,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_co
           for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(f[j * 8 + 2 * e], f[j * 8 + 2 * e + 1]);
           *(uint4*)(dst + ((j ^ (row & 7)) << 4)) = v;
         }
-        fence_proxy_async_smem();
+        if (!p.direct) fence_proxy_async_smem();
         named_bar_sync(1, P_EPI_THREADS);
-        if (issuer) {
+        if (p.direct) {
+          const uint8_t* rows = sE + buf * P_OUT;
+          for (int r = ew * 32; r < ew * 32 + 32 && row0 + r < p.M; ++r) {   // a warp takes a row: two values a lane
+            const int at = col0 + c + lane * 2;
+            const __nv_bfloat162 v = *(const __nv_bfloat162*)(rows + r * 128 + ((lane >> 2 ^ (r & 7)) << 4) + (lane & 3) * 4);
+            __nv_bfloat16* to = p.direct + (int64_t)(row0 + r) * p.N + at;
+            if (at < p.N) to[0] = v.x;
+            if (at + 1 < p.N) to[1] = v.y;
+          }
+        } else if (issuer) {
           if (row0 < p.M && col0 + c < p.N) tma_store_2d(&p.tmOut, sE + buf * P_OUT, col0 + c, row0);  // clipped to the matrix
           bulk_commit();
         }
@@ -213,50 +223,43 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_co
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);
 }
 
-// ------------------------------------------------------------------ one CTA per tile
-// One tile of 128 rows of the first operand by COLS rows of the second per CTA, in steps of 256 values of K.
-// SWAP: the first operand is the weights.  For few rows of x, where reading the weights is what takes the time: an SM takes in some
-// 60 bytes a clock, so all SMs have to read, and a cluster of CTAs divides K.  Each sends its sums to the shared memory of the CTA
-// that owns the column (column number modulo the cluster's size), which adds them in order.  (Owners that fetch the sums instead wait
-// for a round trip per value: 64 x 1024 x 8192 took 19 us that way.)  Without SWAP the kernel serves outputs whose rows are no whole
-// 16-byte units.
+// ------------------------------------------------------------------ few rows of x
+// One tile of 128 rows of w by COLS rows of x per CTA, in steps of 256 values of K: the weights are the tensor core's first operand.  Here
+// reading the weights is what takes the time: an SM takes in some 60 bytes a clock, so all SMs have to read, and a cluster of CTAs
+// divides K.  Each sends its sums to the shared memory of the CTA that owns the row of x (its number modulo the cluster's size), which
+// adds them in order.  (Owners that fetch the sums instead wait for a round trip per value: 64 x 1024 x 8192 took 19 us that way.)
 //   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
-constexpr int G_THREADS = 256, G_STAGE_A = 128 * 128;
-template <int COLS, bool SWAP>
-struct SingleTile {
-  static constexpr int B_BYTES = COLS * 128, S_BLOCKS = COLS > 128 ? 2 : 1, S_BYTES = 1024 + S_BLOCKS * 1024;
-  static constexpr int STAGE = G_STAGE_A + B_BYTES + S_BYTES, OUT = SWAP ? 128 * COLS * 4 : 0;  // OUT: the finished tile, [split][COLS / split][128]
+constexpr int F_THREADS = 256, F_STAGE_W = 128 * 128;
+template <int COLS>
+struct FewTile {
+  static constexpr int X_BYTES = COLS * 128, STAGE = F_STAGE_W + X_BYTES + 2048, OUT = 128 * COLS * 4;  // OUT: the finished tile, [split][COLS / split][128]
   static constexpr int FIT = (225 * 1024 - OUT) / STAGE, STAGES = FIT < 8 ? FIT : 8;
   static constexpr int RING = STAGES * STAGE, SMEM = RING + OUT + 1024 /*alignment slack*/ + 256 /*barriers*/;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-struct alignas(64) GemmParams {
-  CUtensorMap tmA, tmB, tmSA, tmSB;
+struct alignas(64) FewParams {
+  CUtensorMap tmW, tmX, tmSW, tmSX;
   __nv_bfloat16* out;
   int* error_flag;
   uint64_t wait_limit_ns;
-  int64_t rows_a, rows_b;   // rows of the operands
-  int64_t ld;               // of the output
-  int K, tiles_a;
+  int64_t M, N;
+  int K, tiles_w;
   int split;                // CTAs that divide K (a cluster)
-  int early;                // the first operand is complete before the kernel ahead of this one on the stream began
+  int early;                // the weights are complete before the kernel ahead of this one on the stream began
 };
 
-template <int COLS, bool SWAP>
-__global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  using Tile = SingleTile<COLS, SWAP>;
-  constexpr int B_BYTES = Tile::B_BYTES, SB_BLOCKS = Tile::S_BLOCKS, S_BYTES = Tile::S_BYTES, STAGE = Tile::STAGE, STAGES = Tile::STAGES;
-  constexpr int S_COLS = 8 + 8 * SB_BLOCKS;   // columns of tensor memory for a stage's scales
-  constexpr int TMEM = COLS + STAGES * S_COLS <= 256 ? 256 : 512;
-  static_assert(COLS + STAGES * S_COLS <= 512, "tensor memory");
-  constexpr int PITCH = COLS + 4;
-  static_assert(SWAP || 128 * PITCH * 4 <= Tile::RING, "the finished tile reuses the ring");
+template <int COLS>
+__global__ void __launch_bounds__(F_THREADS, 1) gemm_few_kernel(const __grid_constant__ FewParams p) {
+  using Tile = FewTile<COLS>;
+  constexpr int STAGES = Tile::STAGES, S_COLS = 16;   // S_COLS: columns of tensor memory for a stage's scales
+  constexpr int TMEM = 256;
+  static_assert(COLS + STAGES * S_COLS <= TMEM, "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * G_STAGE_A;
-  uint8_t* sS = sB + STAGES * B_BYTES;               // per stage: 1 KB of A's scales, then B's
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + STAGES * F_STAGE_W;
+  uint8_t* sS = sX + STAGES * Tile::X_BYTES;         // per stage: 1 KB of the weights' scales, 1 KB of x's
   float* sums = (float*)(smem + Tile::RING);
   uint64_t* full = (uint64_t*)(smem + Tile::RING + Tile::OUT);
   uint64_t* empty = full + STAGES;
@@ -264,9 +267,9 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = SWAP ? p.split : 1, rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int split = p.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
   const int tile_number = (int)blockIdx.x / split;
-  const int64_t row_a = (int64_t)(tile_number % p.tiles_a) * 128, row_b = (int64_t)(tile_number / p.tiles_a) * COLS;
+  const int64_t row_w = (int64_t)(tile_number % p.tiles_w) * 128, row_x = (int64_t)(tile_number / p.tiles_w) * COLS;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < STAGES; ++i) {
@@ -287,54 +290,55 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
   if (split > 1) cluster_arrive();
   const uint32_t tmem = *tmem_slot;
   const int all_steps = (p.K + 255) / 256, k0 = (int)((int64_t)all_steps * rank / split), k1 = (int)((int64_t)all_steps * (rank + 1) / split);
-  // The launch may overlap the end of the kernel before it.  Where that kernel made the second operand only, the first stages of the
-  // first operand are fetched before waiting for it.
+  // The launch may overlap the end of the kernel before it.  Where that kernel made x only, the first stages of the weights are
+  // fetched before waiting for it.
   if (!p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == 0) {
     if (elect_one()) {
-      tma_prefetch_desc(&p.tmA);
-      tma_prefetch_desc(&p.tmB);
+      tma_prefetch_desc(&p.tmW);
+      tma_prefetch_desc(&p.tmX);
+      tma_prefetch_desc(&p.tmSW);
+      tma_prefetch_desc(&p.tmSX);
       int stage = 0;
       uint32_t phase = 0;
-      auto load_a = [&](int k, int to) {
-        mbar_expect_tx(&full[to], STAGE);
-        tma_load_2d(sA + to * G_STAGE_A, &p.tmA, &full[to], k * 64, (int)row_a);
-        tma_load_2d(sS + to * S_BYTES, &p.tmSA, &full[to], k * 256, (int)(row_a / 128));
+      auto load_w = [&](int k, int to) {
+        mbar_expect_tx(&full[to], Tile::STAGE);
+        tma_load_2d(sW + to * F_STAGE_W, &p.tmW, &full[to], k * 64, (int)row_w);
+        tma_load_2d(sS + to * 2048, &p.tmSW, &full[to], k * 256, (int)(row_w / 128));
       };
       const int ahead = p.early ? (k1 - k0 < STAGES ? k1 - k0 : STAGES) : 0;
-      for (int k = 0; k < ahead; ++k) load_a(k0 + k, k);
+      for (int k = 0; k < ahead; ++k) load_w(k0 + k, k);
       if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int k = k0; k < k1; ++k) {
         if (!mbar_wait(&empty[stage], phase ^ 1, p.wait_limit_ns, abort_flag)) break;
-        if (k - k0 >= ahead) load_a(k, stage);
-        tma_load_2d(sB + stage * B_BYTES, &p.tmB, &full[stage], k * 64, (int)row_b);
-        tma_load_2d(sS + stage * S_BYTES + 1024, &p.tmSB, &full[stage], k * 256, (int)(row_b / 128));
+        if (k - k0 >= ahead) load_w(k, stage);
+        tma_load_2d(sX + stage * Tile::X_BYTES, &p.tmX, &full[stage], k * 64, (int)row_x);
+        tma_load_2d(sS + stage * 2048 + 1024, &p.tmSX, &full[stage], k * 256, (int)(row_x / 128));
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc[2] = {umma_idesc_mxf4(128, COLS, 0), umma_idesc_mxf4(128, COLS, 2)};
-      const uint32_t sfb_first = (uint32_t)(row_b % 128 / 32);  // rows of a narrow tile start inside a row block
+      const uint32_t sfx_first = (uint32_t)(row_x % 128 / 32);  // a tile of 64 rows may start in the middle of a row block
       int stage = 0;
       uint32_t phase = 0;
       for (int k = k0; k < k1; ++k) {
         if (!mbar_wait(&full[stage], phase, p.wait_limit_ns, abort_flag)) break;
         tc_fence_after_sync();
-        // A: 4 columns per 128 values of K; B: 4 per 128 values and 128 rows.  Written again only after the stage's MMAs are done.
+        // Four columns per 128 values of K for each operand.  Written again only after the stage's MMAs are done.
         const uint32_t sf = tmem + COLS + stage * S_COLS;
-        const uint32_t s = smem_u32(sS + stage * S_BYTES);
+        const uint32_t s = smem_u32(sS + stage * 2048);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           umma_copy_scales(sf + h * 4, umma_desc_scales(s + h * SCALE_BLOCK));
-#pragma unroll
-          for (int b = 0; b < SB_BLOCKS; ++b) umma_copy_scales(sf + 8 + (h * SB_BLOCKS + b) * 4, umma_desc_scales(s + 1024 + b * 1024 + h * SCALE_BLOCK));
+          umma_copy_scales(sf + 8 + h * 4, umma_desc_scales(s + 1024 + h * SCALE_BLOCK));
         }
-        const uint64_t da = umma_desc_k_sw128(smem_u32(sA + stage * G_STAGE_A)), db = umma_desc_k_sw128(smem_u32(sB + stage * B_BYTES));
+        const uint64_t da = umma_desc_k_sw128(smem_u32(sW + stage * F_STAGE_W)), db = umma_desc_k_sw128(smem_u32(sX + stage * Tile::X_BYTES));
 #pragma unroll
         for (int i = 0; i < 4; ++i)  // 64 values of K are 32 bytes
-          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * SB_BLOCKS * 4 + sfb_first, k > k0 || i > 0);
+          umma_mxf4(tmem, da + i * 2, db + i * 2, idesc[i & 1], sf + (i >> 1) * 4, sf + 8 + (i >> 1) * 4 + sfx_first, k > k0 || i > 0);
         umma_commit(&empty[stage]);
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
@@ -352,62 +356,43 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
   const int quarter = (warp & 3) * 32;
   constexpr int HALF = COLS / 2 < 32 ? 32 : COLS / 2;
   const int c0 = (warp >> 2) * HALF;   // this warp's rows are quarter + lane, its columns [c0, c0 + HALF)
-  if constexpr (SWAP) {
-    // row r of the tile is output column row_a + r, column c output row row_b + c
-    if (split > 1) cluster_wait();     // the others run: their shared memory may be written
-    const int share = COLS / split;
-    if (c0 < COLS) {
-#pragma unroll
-      for (int c = c0; c < c0 + HALF; c += 32) {
-        float f[32];
-        tmem_ld_32x32(tmem + ((uint32_t)quarter << 16) + (uint32_t)c, (uint32_t*)f);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          float* at = sums + ((rank * share + (c + j) / split) * 128 + quarter + lane);
-          if (split == 1) *at = f[j];
-          else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(at), (uint32_t)((c + j) & (split - 1)))), "f"(f[j]) : "memory");
-        }
-      }
-    }
-    tc_fence_before_sync();
-    if (split > 1) cluster_sync_all();
-    else __syncthreads();
-    if (warp == 2) tmem_dealloc(tmem, TMEM);
-    const int cols = p.rows_b - row_b < COLS ? (int)(p.rows_b - row_b) : COLS, r = lane * 4;
-    const bool vec = p.ld % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
-    for (int i = warp; i * split + rank < cols; i += G_THREADS / 32) {   // a warp takes a column: 128 values of an output row
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int q = 0; q < split; ++q) {
-        const float4 s = *(const float4*)(sums + (q * share + i) * 128 + r);
-        v.x += s.x, v.y += s.y, v.z += s.z, v.w += s.w;
-      }
-      __nv_bfloat16* dst = p.out + (row_b + i * split + rank) * p.ld + row_a + r;
-      alignas(8) __nv_bfloat162 o[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
-      if (vec && row_a + r + 4 <= p.rows_a) {
-        *(uint2*)dst = *(uint2*)o;
-      } else {
-        for (int j = 0; j < 4; ++j)
-          if (row_a + r + j < p.rows_a) dst[j] = ((__nv_bfloat16*)o)[j];
-      }
-    }
-  } else {
-    float* tile = (float*)smem;  // [128][PITCH]
+  // row r of the tile is output column row_w + r, column c output row row_x + c
+  if (split > 1) cluster_wait();     // the others run: their shared memory may be written
+  const int share = COLS / split;
+  if (c0 < COLS) {
 #pragma unroll
     for (int c = c0; c < c0 + HALF; c += 32) {
       float f[32];
       tmem_ld_32x32(tmem + ((uint32_t)quarter << 16) + (uint32_t)c, (uint32_t*)f);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) *(float4*)(tile + (quarter + lane) * PITCH + c + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+      for (int j = 0; j < 32; ++j) {
+        float* at = sums + ((rank * share + (c + j) / split) * 128 + quarter + lane);
+        if (split == 1) *at = f[j];
+        else asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(at), (uint32_t)((c + j) & (split - 1)))), "f"(f[j]) : "memory");
+      }
     }
-    tc_fence_before_sync();
-    __syncthreads();
-    if (warp == 2) tmem_dealloc(tmem, TMEM);
-    for (int i = threadIdx.x; i < 128 * COLS; i += G_THREADS) {
-      const int r = i / COLS, c = i % COLS;
-      if (row_a + r < p.rows_a && row_b + c < p.rows_b) p.out[(row_a + r) * p.ld + row_b + c] = __float2bfloat16_rn(tile[r * PITCH + c]);
+  }
+  tc_fence_before_sync();
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, TMEM);
+  const int cols = p.M - row_x < COLS ? (int)(p.M - row_x) : COLS, r = lane * 4;
+  const bool vec = p.N % 4 == 0 && ((uintptr_t)p.out & 7) == 0;
+  for (int i = warp; i * split + rank < cols; i += F_THREADS / 32) {   // a warp takes a column: 128 values of an output row
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int q = 0; q < split; ++q) {
+      const float4 s = *(const float4*)(sums + (q * share + i) * 128 + r);
+      v.x += s.x, v.y += s.y, v.z += s.z, v.w += s.w;
+    }
+    __nv_bfloat16* dst = p.out + (row_x + i * split + rank) * p.N + row_w + r;
+    alignas(8) __nv_bfloat162 o[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+    if (vec && row_w + r + 4 <= p.N) {
+      *(uint2*)dst = *(uint2*)o;
+    } else {
+      for (int j = 0; j < 4; ++j)
+        if (row_w + r + j < p.N) dst[j] = ((__nv_bfloat16*)o)[j];
     }
   }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.error_flag, 1);

@@ -233,7 +233,11 @@ static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns
   memset(&p, 0, sizeof(p));
   int st = make_map(&p.tmA, a->x, (uint64_t)a->M, (uint64_t)a->K / 4, 128);  // bytes, in pairs: the box is 128 rows by 128 bytes
   if (!st) st = make_map(&p.tmB, a->w, (uint64_t)a->N, (uint64_t)a->K / 4, COLS / 2);
-  if (!st) st = make_map(&p.tmOut, a->out, (uint64_t)a->M, (uint64_t)a->N, 128);
+  if (a->N % 8 == 0 && ((uintptr_t)a->out & 15) == 0) {
+    if (!st) st = make_map(&p.tmOut, a->out, (uint64_t)a->M, (uint64_t)a->N, 128);
+  } else {
+    p.direct = (__nv_bfloat16*)a->out;
+  }
   if (!st) st = make_scale_map(&p.tmSA, a->x_scales, a->M, a->K, 1);
   if (!st) st = make_scale_map(&p.tmSB, a->w_scales, a->N, a->K, COLS / 128);
   if (st) return map_status(st);
@@ -250,33 +254,64 @@ static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns
   return launch_clusters(gemm_pair_kernel<COLS>, p, 2 * (p.tiles < most ? p.tiles : most), P_THREADS, PairTile<COLS>::SMEM, 2, stream);
 }
 
-template <int COLS, bool SWAP>
-static int launch_gemm(const bshmem_mxfp4_gemm_args_t* g, uint64_t wait_limit_ns, cudaStream_t stream) {
-  GemmParams p;
+template <int COLS>
+static int launch_few(const bshmem_mxfp4_gemm_args_t* g, int split, uint64_t wait_limit_ns, cudaStream_t stream) {
+  FewParams p;
   memset(&p, 0, sizeof(p));
-  p.rows_a = SWAP ? g->N : g->M;
-  p.rows_b = SWAP ? g->M : g->N;
-  int st = make_map(&p.tmA, SWAP ? g->w : g->x, (uint64_t)p.rows_a, (uint64_t)g->K / 4, 128);
-  if (!st) st = make_map(&p.tmB, SWAP ? g->x : g->w, (uint64_t)p.rows_b, (uint64_t)g->K / 4, COLS);
-  if (!st) st = make_scale_map(&p.tmSA, SWAP ? g->w_scales : g->x_scales, p.rows_a, g->K, 1);
-  if (!st) st = make_scale_map(&p.tmSB, SWAP ? g->x_scales : g->w_scales, p.rows_b, g->K, COLS > 128 ? 2 : 1);
+  int st = make_map(&p.tmW, g->w, (uint64_t)g->N, (uint64_t)g->K / 4, 128);
+  if (!st) st = make_map(&p.tmX, g->x, (uint64_t)g->M, (uint64_t)g->K / 4, COLS);
+  if (!st) st = make_scale_map(&p.tmSW, g->w_scales, g->N, g->K, 1);
+  if (!st) st = make_scale_map(&p.tmSX, g->x_scales, g->M, g->K, 1);
   if (st) return map_status(st);
   p.out = (__nv_bfloat16*)g->out;
   p.error_flag = g->error_flag;
   p.wait_limit_ns = wait_limit_ns;
-  p.ld = g->N;
+  p.M = g->M;
+  p.N = g->N;
   p.K = (int)g->K;
-  p.tiles_a = (int)((p.rows_a + 127) / 128);
-  const int64_t tiles = (int64_t)p.tiles_a * ((p.rows_b + COLS - 1) / COLS);
-  // K is divided as long as that brings in SMs that would be idle, and leaves a CTA two steps at least.
-  p.split = 1;
-  const int steps = (p.K + 255) / 256, sms = sm_count();
-  while (SWAP && p.split < 8 && tiles * p.split * 2 <= sms && steps >= p.split * 4) p.split *= 2;
-  p.early = SWAP && g->raw_x;  // the kernel ahead quantised x, and began after everything before it was complete
-  if (tiles * p.split > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
+  p.tiles_w = (int)((g->N + 127) / 128);
+  p.split = split;
+  p.early = g->raw_x != nullptr;  // the kernel ahead quantised x, and began after everything before it was complete
+  const int64_t ctas = (int64_t)p.tiles_w * ((g->M + COLS - 1) / COLS) * split;
+  if (ctas > 0x7fffffff) return BSHMEM_MX_ERR_SHAPE;
   static std::atomic<uint64_t> ready;
-  if (!reserve_smem((const void*)gemm_kernel<COLS, SWAP>, SingleTile<COLS, SWAP>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
-  return launch_clusters(gemm_kernel<COLS, SWAP>, p, (int)tiles * p.split, G_THREADS, SingleTile<COLS, SWAP>::SMEM, p.split, stream);
+  if (!reserve_smem((const void*)gemm_few_kernel<COLS>, FewTile<COLS>::SMEM, ready)) return BSHMEM_MX_ERR_DRIVER;
+  return launch_clusters(gemm_few_kernel<COLS>, p, (int)ctas, F_THREADS, FewTile<COLS>::SMEM, split, stream);
+}
+
+// Which kernel takes a product, by a model of measured times (us, operands in memory): a fixed part and, per step of 256 values of K and
+// wave of tiles, what an SM takes to load its share.  Measured (few rows with 64 columns, pairs of 128 and 256 columns):
+//     64 x 8192 x 8192   12.6 / 12.8 / 16.2      512 x 2048 x 2048    7.5 /  6.4 /  7.8
+//    100 x 8192 x 8192   14.2 / 13.0 / 16.5      512 x 4096 x 7168   22.9 / 12.1 / 15.2
+//    129 x 2048 x 8192    9.9 / 11.5 / 14.7      512 x 8192 x 8192   47.3 / 21.2 / 18.1
+//    300 x  512 x 8192    7.9 / 11.2 / 14.2     1024 x 8192 x 3584   59.5 / 20.4 / 17.4
+struct Plan {
+  int cols;    // 32, 64: few rows; 128, 256: pairs
+  int split;   // CTAs that divide K
+};
+static Plan plan_product(int64_t M, int64_t N, int64_t K, int sms) {
+  const int64_t steps = (K + 255) / 256;
+  Plan best = {0, 1};
+  double best_us = 0.0;
+  auto offer = [&](int cols, int split, double us) {
+    if (best.cols && us >= best_us) return;
+    best = {cols, split};
+    best_us = us;
+  };
+  for (int cols = 32; cols <= 64; cols *= 2) {
+    if (cols == 32 && M > 32) continue;   // scales of a tile start at a multiple of 64 rows
+    const int64_t tiles = (N + 127) / 128 * ((M + cols - 1) / cols);
+    // K is divided as long as that brings in SMs that would be idle, and leaves a CTA two steps at least.
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && steps >= split * 4) split *= 2;
+    const double waves = (double)((tiles * split + sms - 1) / sms), per_cta = (double)((steps + split - 1) / split);
+    offer(cols, split, 5.0 + (split > 1 ? 1.0 : 0.0) + waves * per_cta * (cols == 32 ? 0.22 : 0.29));
+  }
+  for (int cols = 128; cols <= 256; cols *= 2) {
+    const int64_t tiles = (M + 255) / 256 * ((N + cols - 1) / cols), pairs = sms / 2;
+    offer(cols, 1, 5.2 + (double)((tiles + pairs - 1) / pairs) * (double)steps * (cols == 128 ? 0.22 : 0.37));
+  }
+  return best;
 }
 
 }  // namespace mx
@@ -322,9 +357,15 @@ extern "C" int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* a, cudaStream_t
     if (q) return q;
   }
   const uint64_t limit = a->wait_limit_ms ? (uint64_t)a->wait_limit_ms * 1000000ull : 10000000000ull;
-  if (a->M <= 32) return launch_gemm<32, true>(a, limit, stream);
-  if (a->M <= 64) return launch_gemm<64, true>(a, limit, stream);
-  if (a->M <= 128) return launch_gemm<128, true>(a, limit, stream);
-  if (a->N % 8 == 0 && ((uintptr_t)a->out & 15) == 0) return launch_pair<256>(a, limit, stream);  // whole 16-byte units of output rows
-  return launch_gemm<256, false>(a, limit, stream);
+  const Plan plan = plan_product(a->M, a->N, a->K, sm_count());
+  if (plan.cols == 32) return launch_few<32>(a, plan.split, limit, stream);
+  if (plan.cols == 64) return launch_few<64>(a, plan.split, limit, stream);
+  return plan.cols == 128 ? launch_pair<128>(a, limit, stream) : launch_pair<256>(a, limit, stream);
+}
+
+// Test hook (host only): the tile width and the division of K that plan_product chooses.
+extern "C" void bshmem_mxfp4_test_plan(int64_t M, int64_t N, int64_t K, int sms, int* out) {
+  const Plan plan = plan_product(M, N, K, sms);
+  out[0] = plan.cols;
+  out[1] = plan.split;
 }

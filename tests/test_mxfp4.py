@@ -134,6 +134,40 @@ def test_product_sizes(M, N, K):
     _check_product(_data(M, K, torch.bfloat16, 1).cuda(), _data(N, K, torch.bfloat16, 2).cuda())
 
 
+# Products for each kernel, division of K, ragged edge and kind of store: (M, N, K) and the tile width and division that the rule takes on 148 SMs.
+PLANS = [((5, 130, 4096), (32, 8)), ((32, 1000, 2560), (32, 4)), ((20, 9000, 2048), (32, 2)), ((17, 19001, 512), (32, 1)), ((7, 120, 8192), (32, 8)),
+         ((50, 16001, 544), (64, 1)), ((130, 260, 4128), (64, 8)), ((300, 512, 8192), (64, 4)), ((129, 2043, 7168), (64, 2)),
+         ((65, 8, 64), (64, 1)), ((190, 2100, 96), (64, 1)), ((3000, 4168, 96), (256, 1)), ((300, 4097, 1088), (128, 1)), ((1030, 1100, 2080), (128, 1)), ((500, 2047, 3200), (128, 1)),
+         ((1024, 4096, 2048), (256, 1)), ((777, 8191, 1056), (256, 1)), ((2560, 4160, 544), (128, 1)), ((3000, 4160, 2080), (256, 1))]
+
+
+def test_the_rule_takes_every_kernel():
+    import ctypes
+    from nvshmem_b200.ops import mxfp4
+    out = (ctypes.c_int * 2)()
+    got = []
+    for shape, _ in PLANS:
+        mxfp4._lib().bshmem_mxfp4_test_plan(*(ctypes.c_int64(v) for v in shape), 148, out)
+        got.append((shape, tuple(out)))
+    assert got == PLANS
+    assert {c for _, (c, _) in got} == {32, 64, 128, 256} and {s for _, (_, s) in got} == {1, 2, 4, 8}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [s for s, _ in PLANS])
+def test_products_of_every_kernel(shape):
+    M, N, K = shape
+    w = _data(N, K, torch.bfloat16, 4).cuda()
+    _check_product(_data(M, K, torch.bfloat16, 3).cuda(), w)
+    # into the middle of a larger buffer: what lies around stays
+    from nvshmem_b200.ops import mxfp4
+    buf = torch.full((M + 2, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    x, wq = _data(M, K, torch.bfloat16, 3).cuda(), mxfp4.quantize_mxfp4(w)
+    if N % 8 == 0:
+        mxfp4.gemm_mxfp4(x, wq, out=buf[1:M + 1])
+        assert (buf[0] == 7).all() and (buf[M + 1] == 7).all() and torch.equal(buf[1:M + 1], mxfp4.gemm_mxfp4(x, wq))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,K", [(16, 8192, 8192), (3, 7168, 2048), (512, 4096, 7168), (1500, 2816, 1984), (2048, 2047, 1024), (4100, 1032, 512)])
 def test_larger_products(M, N, K):
