@@ -24,6 +24,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/bshmem/norms.h"
@@ -411,6 +412,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][3];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the kernel that adds the CTAs' sums waits for this one itself
   Rows<MODE, KIND> rows(p, smem, true);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
   const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN;
@@ -549,9 +551,13 @@ template <typename W>
 static __global__ void __launch_bounds__(32 * SLICES) column_sum_kernel(const __grid_constant__ bshmem_norm_args_t a, int parts) {
   const int i = blockIdx.x * 32 + threadIdx.x;
   const bool pre = blockIdx.y != 0, channel = a.gate_mode == BSHMEM_NORM_GATE_CHANNEL;
-  if (pre ? !a.dpre : !a.dpost && !(a.dgate && channel)) return;
+  if (pre ? !a.dpre : !a.dpost && !(a.dgate && channel)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the end of this kernel is the end of both
+    return;
+  }
   __shared__ float s[SLICES][33];
   float v = 0.f;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (i < a.H) {
 #pragma unroll 4
     for (int k = threadIdx.y; k < parts; k += SLICES) v += a.partials[((size_t)k * 2 + pre) * a.H + i];
@@ -638,13 +644,15 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
   r.ctas = r.parts * pair;
   return r;
 }
-// Raises a kernel's shared-memory limit to what it may take.
-static inline bool reserve_smem(const void* kernel, int bytes) {
-  return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
-}
+// Launches a kernel; `ready`: the GPUs (bit = ordinal) on which its shared-memory limit has been raised.
 template <typename P>
-static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, cudaStream_t stream) {
-  if (!reserve_smem((const void*)kernel, plan.smem)) return BSHMEM_NORM_ERR_DRIVER;
+static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, std::atomic<uint64_t>& ready, cudaStream_t stream) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return BSHMEM_NORM_ERR_DRIVER;
+  if (plan.smem > 48 * 1024 && (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1))) {
+    if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STAGE_SMEM) != cudaSuccess) return BSHMEM_NORM_ERR_DRIVER;
+    if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(plan.block);
@@ -657,6 +665,20 @@ static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, cudaStream
   cfg.attrs = &attr;
   cfg.numAttrs = plan.half ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+}
+// The second kernel of a backward pass is set up while the first runs, and waits for it itself.
+template <typename W>
+static int launch_column_sums(const bshmem_norm_args_t& a, int parts, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.H + 31) / 32, 2);
+  cfg.blockDim = dim3(32, SLICES);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, column_sum_kernel<W>, a, parts) == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
 }
 
 // The kernel of a plan.  A row alone (IN) has one type.
@@ -677,10 +699,9 @@ static int launch_rows(const bshmem_norm_args_t* a, cudaStream_t stream) {
   const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
   void (*const kernel)(RowParams) = plan.mode == STAGED ? by_kind<T, R, W, BACKWARD, STAGED>(plan.kind) : plan.mode == VECTOR ? by_kind<T, R, W, BACKWARD, VECTOR>(plan.kind)
                                                                                                         : kernel_of<T, R, W, BACKWARD, SCALAR, ANY>();
-  const int st = launch(kernel, plan, p, stream);
-  if (st || !BACKWARD || !a->partials) return st;
-  column_sum_kernel<W><<<dim3((a->H + 31) / 32, 2), dim3(32, SLICES), 0, stream>>>(*a, plan.parts);
-  return cudaGetLastError() == cudaSuccess ? BSHMEM_NORM_OK : BSHMEM_NORM_ERR_DRIVER;
+  static std::atomic<uint64_t> ready[3][4];
+  const int st = launch(kernel, plan, p, ready[plan.mode][plan.kind], stream);
+  return st || !BACKWARD || !a->partials ? st : launch_column_sums<W>(*a, plan.parts, stream);
 }
 template <typename T, typename R, typename W>
 static int launch_either(const bshmem_norm_args_t* a, bool backward, cudaStream_t stream) {
