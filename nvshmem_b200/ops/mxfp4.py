@@ -5,7 +5,7 @@
 * :func:`gemm_mxfp4` – ``x @ w.T`` of two such matrices on the tensor cores' block-scaled form, accumulated in fp32; a bf16,
   fp16 or fp32 ``x`` is quantised in the call.
 
-For serving: weights are quantised once, activations in every call.  K is a multiple of 32; rows and columns of the product may be
+For serving: weights are quantised once, activations in every call, and nothing here records gradients.  K is a multiple of 32; rows and columns of the product may be
 any number.  Work is issued on the current stream; all tensors lie on the current device.
 """
 from __future__ import annotations
@@ -19,7 +19,7 @@ from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
 
 BLOCK = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
+_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32 and at most 2^27", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
 
 
 class _GemmArgs(C.Structure):
@@ -106,8 +106,8 @@ def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
     NaN gets the scale NaN, and so do all its values."""
     x, device = _checked(x)
     R, K = x.shape
-    data = torch.empty((R, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(_scale_shape(R, K), dtype=torch.uint8, device=x.device)
+    data = x.new_empty((R, K // 2), dtype=torch.uint8)
+    scales = x.new_empty(_scale_shape(R, K), dtype=torch.uint8)
     _raise(_lib().bshmem_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], R, K, x.stride(0), data.data_ptr(), scales.data_ptr(), stream_of(device)), "bshmem_mxfp4_quantize")
     return MxFp4(data, scales, (R, K))
 
@@ -139,7 +139,7 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
         device = device_of(FusedGemmError, w.data, w.scales, out)
         # room for x as it is quantised: the values, then the scales
         rb, kb, _ = _scale_shape(M, K)
-        room = torch.empty((M * K // 2 + 127) // 128 * 128 + rb * kb * 512, dtype=torch.uint8, device=dev)
+        room = w.data.new_empty((M * K // 2 + 127) // 128 * 128 + rb * kb * 512)
         data = room.data_ptr()
         operand = data, data + (M * K // 2 + 127) // 128 * 128
         source = x.data_ptr(), _TYPES[x.dtype], x.stride(0)
@@ -147,7 +147,7 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
         device = device_of(FusedGemmError, x.data, x.scales, w.data, w.scales, out)
         operand, source = (x.data.data_ptr(), x.scales.data_ptr()), (None, 0, 0)
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = w.data.new_empty((M, N), dtype=torch.bfloat16)
     else:
         _check_out(out, M, N)
     a = _GemmArgs(*operand, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), M, N, K, 0, _error_flag(dev).data_ptr(), *source)

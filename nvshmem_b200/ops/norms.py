@@ -56,6 +56,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 class _Plan:
     """The settings of a call: everything that is not a tensor."""
     __slots__ = ("T", "H", "device", "gate_mode", "residual_scale", "branch_scale", "eps", "weight_offset", "dtype")
@@ -74,17 +78,16 @@ class _Plan:
 
 
 def _forward(plan: _Plan, h, residual, post, pre, gate, want_r: bool, want_stat: bool):
-    dev, shape = residual.device, (plan.T, plan.H)
-    r = torch.empty(shape, dtype=residual.dtype, device=dev) if want_r else None
-    y = torch.empty(shape, dtype=plan.dtype, device=dev) if pre is not None else None
-    stat = torch.empty((2, plan.T), dtype=torch.float32, device=dev) if want_stat else None
+    r = _dense_like(residual) if want_r else None
+    y = _dense_like(residual if h is None else h) if pre is not None else None
+    stat = residual.new_empty((2, plan.T), dtype=torch.float32) if want_stat else None
     plan.launch(_lib().bshmem_block_norms, "bshmem_block_norms", h, residual, post, pre, gate, r, y, stat)
     return r, y, stat
 
 
 def _backward(plan: _Plan, h, residual, post, pre, gate, stat, dr, dy, needs):
     """Gradients of (h, residual, post, pre, gate), None where `needs` is false."""
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need and t is not None else None for t, need in zip((h, residual, post, pre, gate), needs)]
+    grads = [_dense_like(t) if need and t is not None else None for t, need in zip((h, residual, post, pre, gate), needs)]
     dh, dres, dpost, dpre, dgate = grads
     if plan.T == 0 or (dr is None and dy is None):
         return [g if g is None else g.zero_() for g in grads]
@@ -92,7 +95,7 @@ def _backward(plan: _Plan, h, residual, post, pre, gate, stat, dr, dy, needs):
         dpre.zero_()
     partials = None
     if dpost is not None or dpre is not None or (dgate is not None and plan.gate_mode == _CHANNEL):
-        partials = torch.empty(_lib().bshmem_block_norms_partials(plan.T, plan.H), dtype=torch.float32, device=residual.device)
+        partials = residual.new_empty(_lib().bshmem_block_norms_partials(plan.T, plan.H), dtype=torch.float32)
     plan.launch(_lib().bshmem_block_norms_backward, "bshmem_block_norms_backward", h, residual, post, pre, gate, None, None, stat, None if dr is None else _rows(dr),
                 None if dy is None else _rows(dy), dh, dres, dpost, None if dy is None else dpre, dgate, partials)
     return grads
@@ -124,6 +127,8 @@ def _check_rows(name: str, t: torch.Tensor, shape) -> None:
         raise NormError(f"{name} must be a [T, H] tensor" + (f" of shape {tuple(shape)}" if shape is not None else ""))
     if t.dtype not in _TYPES:
         raise NormError(f"{name} must be bfloat16, float16 or float32, not {t.dtype}")
+    if t.shape[0] >= 2 ** 31 or not 1 <= t.shape[1] <= MAX_H:
+        raise NormError(f"fewer than 2^31 rows of 1 to {MAX_H} values, not {tuple(t.shape)}")
 
 
 def _check_weights(plan: _Plan, **weights) -> None:
@@ -165,8 +170,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, weight_of
     _check_rows("x", x, None)
     plan = _Plan()
     plan.T, plan.H = x.shape
-    if not 1 <= plan.H <= MAX_H:
-        raise NormError(f"rows of 1 to {MAX_H} values, not {plan.H}")
     plan.dtype, plan.gate_mode = x.dtype, _NONE
     plan.residual_scale, plan.branch_scale, plan.eps, plan.weight_offset = 1.0, 1.0, float(eps), float(weight_offset)
     if weight is None:
@@ -191,8 +194,6 @@ def block_norms(h: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tens
     _check_rows("residual", residual, h.shape)
     plan = _Plan()
     plan.T, plan.H = h.shape
-    if not 1 <= plan.H <= MAX_H:
-        raise NormError(f"rows of 1 to {MAX_H} values, not {plan.H}")
     plan.dtype = h.dtype
     if residual.dtype not in (h.dtype, torch.float32):
         raise NormError(f"residual must be {h.dtype} or float32")

@@ -58,8 +58,8 @@ def _launch(fn, name, logits, K, score, renormalize=0, scale=1.0, bias=None, val
 
 
 def _route(logits, K, score, bias, renormalize, scale, valid):
-    idx = torch.empty((logits.shape[0], K), dtype=torch.int32, device=logits.device)
-    weight = torch.empty((logits.shape[0], K), dtype=torch.float32, device=logits.device)
+    idx = logits.new_empty((logits.shape[0], K), dtype=torch.int32)
+    weight = logits.new_empty((logits.shape[0], K), dtype=torch.float32)
     _launch(_lib().bshmem_route, "bshmem_route", logits, K, score, renormalize, scale, bias, valid, idx, weight)
     return idx, weight
 
@@ -81,17 +81,16 @@ class _Route(torch.autograd.Function):
             return (None,) * 7
         logits, idx, weight = ctx.saved_tensors
         K, score, renormalize, scale = ctx.settings
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
         _launch(_lib().bshmem_route_backward, "bshmem_route_backward", logits, K, score, renormalize, scale, idx=idx, weight=weight, dweight=dweight.contiguous(), dlogits=dlogits)
         return dlogits, None, None, None, None, None, None
 
 
 def _balance(logits, idx, score, valid):
     T, E = logits.shape
-    dev = logits.device
-    loss, counts = torch.empty((), dtype=torch.float32, device=dev), torch.empty(E, dtype=torch.int32, device=dev)
+    loss, counts = logits.new_empty((), dtype=torch.float32), logits.new_empty(E, dtype=torch.int32)
     # dloss / dp per expert (kept for backward), then the kernel's workspace
-    buffer = torch.empty(4 * E + _lib().bshmem_balance_workspace(T, E), dtype=torch.uint8, device=dev)
+    buffer = logits.new_empty(4 * E + _lib().bshmem_balance_workspace(T, E), dtype=torch.uint8)
     at = buffer.data_ptr()
     _launch(_lib().bshmem_balance, "bshmem_balance", logits, idx.shape[1], score, valid=valid, idx=idx, loss=loss, counts=counts, coef=at, workspace=at + 4 * E)
     return loss, counts, buffer
@@ -113,7 +112,7 @@ class _Balance(torch.autograd.Function):
         if dloss is None:
             return None, None, None, None
         logits, buffer, valid = ctx.saved_tensors
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dlogits = torch.empty_like(logits, memory_format=torch.contiguous_format)
         _launch(_lib().bshmem_balance_backward, "bshmem_balance_backward", logits, *ctx.settings, valid=valid, dlogits=dlogits, coef=buffer.data_ptr(), dloss=dloss)
         return dlogits, None, None, None
 

@@ -142,6 +142,14 @@ def test_many_rows(gate, post, pre, T, H, dt, rt, wt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate,post,pre", [("channel", True, True), ("token", True, False), ("full", True, True), ("none", False, True)])
+@pytest.mark.parametrize("T,H", [(160, 16384), (300, 8200), (90, 9216)])
+def test_many_long_rows(gate, post, pre, T, H):
+    """Above 8192 columns a pair of CTAs takes half a row each."""
+    _check(_norm_inputs(T, H, BF16, BF16, F32, gate, post, pre))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T,H", [(900, 1024), (1201, 1536), (640, 3000), (310, 5128), (333, 7168), (2000, 4096), (500, 8184)])
 @pytest.mark.parametrize("dt,rt,wt", [(BF16, BF16, BF16), (BF16, F32, F32)])
 def test_many_rows_sizes(T, H, dt, rt, wt):
@@ -244,6 +252,36 @@ def test_rows_of_zeros_and_bad_rows_stay_apart():
     assert r[3].isnan().all() and y[4].isnan().any()
     for i in (0, 2, 5):
         assert torch.equal(r[i], good[0][i]) and torch.equal(y[i], good[1][i])
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused():
+    """A graph of the gradients may be asked for, but not gone through."""
+    from nvshmem_b200.ops import moe_route, rms_norm
+    x, w = torch.randn(5, 64, device="cuda", requires_grad=True), torch.ones(64, device="cuda")
+    for out in (rms_norm(x, w), moe_route(x, 4)[1]):
+        (plain,) = torch.autograd.grad(out.sum(), x, retain_graph=True)
+        (g,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.gpu
+def test_tiny_rows_without_eps():
+    """Values of 1e-13 with eps = 0: nothing between overflows."""
+    d = _norm_inputs(20, 1024, F32, F32, F32, "channel")
+    for k in ("h", "residual"):
+        d[k] = d[k] * 1e-13
+    from nvshmem_b200.ops import norms
+    leaves = [d[n].requires_grad_(True) for n in ("h", "residual", "post", "pre", "gate")]
+    r, y = norms.block_norms(*leaves, branch_scale=1e-13, eps=0.0)
+    grads = torch.autograd.grad([r, y], leaves, [d["dr"] * 1e13, d["dy"]])
+    want, mag = _reference({**d, "dr": d["dr"] * 1e13}, 1.0, 1e-13, 0.0, 0.0)
+    _compare(y.detach(), want["y"], mag["y"], "y")
+    for n, g in zip(("h", "residual", "post", "pre", "gate"), grads):
+        assert g.isfinite().all()
+        _compare(g, want["d_" + n], mag["d_" + n], n)
 
 
 @pytest.mark.gpu
