@@ -190,12 +190,11 @@ struct Rows {
       return global(row);
     }
   }
-  // All threads are past their last look at the stage of `row` (`behind` = 0) or of the row before it (1): it takes the next row that
-  // falls to it.
-  __device__ __forceinline__ void refill(size_t row, int behind) const {
+  // All threads are past their last look at `row`, which was in `its_stage`: the stage takes the next row that falls to it.
+  __device__ __forceinline__ void refill(size_t row, int its_stage) const {
     if constexpr (MODE == STAGED) {
-      const size_t next = row + (size_t)(p.stages - behind) * step;
-      if ((threadIdx.x & 31) == 0 && row >= first + behind * step && next < (size_t)p.a.T) load(next, stage >= behind ? stage - behind : p.stages - 1);
+      const size_t next = row + (size_t)p.stages * step;
+      if ((threadIdx.x & 31) == 0 && next < (size_t)p.a.T) load(next, its_stage);
     }
   }
   __device__ __forceinline__ void next() {
@@ -313,7 +312,8 @@ template <typename T, typename R, typename W, Mode MODE, Kind KIND>
 __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sums[2][SUM_ROWS][1];
+  constexpr int SUMS = MODE == STAGED && KIND == BOTH ? 2 : 1;
+  __shared__ float sums[2][SUM_ROWS][SUMS];
   Rows<MODE, KIND> rows(p, smem, false);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
   const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN, has_y = KIND == ANY ? a.y != nullptr : KIND != OUT;
@@ -328,11 +328,68 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
       for (int i = 0; i < 4; ++i) wp[c][i] += a.weight_offset;
     }
   }
+  if constexpr (MODE == STAGED && KIND == BOTH) {
+    // One barrier a row: the sum of squares of the next row's h goes together with the one of this row's r.
+    auto squares = [&](const RowSource& src) {
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        float h[4];
+        rows.template load4<T>(h, src.h, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += h[i] * h[i];
+      }
+      return sum;
+    };
+    int buf = 1;
+    RowSource src = rows.wait(rows.first);   // there are more rows than CTAs
+    float v[2] = {squares(src), 0.f};
+    rows.sum(v, sums[0]);
+    for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+      const float inv = rsqrtf(v[0] * inv_h + a.eps);
+      float r[ROW_CH][4];
+      v[0] = v[1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+        float x[4];
+        rows.template load4<T>(r[c], src.h, c);
+        rows.template load4<R>(x, src.residual, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          r[c][i] = r[c][i] * inv * u[c][i] + a.residual_scale * x[i];
+          v[1] += r[c][i] * r[c][i];
+        }
+        rows.store4(rows.template out<R>(a.r, row), c, r[c]);
+      }
+      const int stage = rows.stage;
+      rows.next();
+      if (row + rows.step < (size_t)a.T) {
+        src = rows.wait(row + rows.step);
+        v[0] = squares(src);
+      }
+      rows.sum(v, sums[buf]);
+      buf ^= 1;
+      rows.refill(row, stage);  // after a barrier: every thread has taken the row out of its stage
+      const float inv_r = rsqrtf(v[1] * inv_h + a.eps);
+      if (rows.tid == 0 && a.stat) {
+        a.stat[row] = inv;
+        a.stat[a.T + row] = inv_r;
+      }
+#pragma unroll
+      for (int c = 0; c < ROW_CH; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[c][i] *= inv_r * wp[c][i];
+        rows.store4(rows.template out<T>(a.y, row), c, r[c]);
+      }
+    }
+    rows.end();
+    return;
+  }
   int buf = 0;
   for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
     const float tg = token ? load1<W>(a.gate, row) : 1.f;
     const RowSource src = rows.wait(row);
-    float r[ROW_CH][4], ss[1];
+    float r[ROW_CH][4], ss[SUMS] = {};
     if (has_h) {
       float inv = 1.f, res[MODE == STAGED ? 1 : ROW_CH][4];
       ss[0] = 0.f;
@@ -392,7 +449,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
     } else if (MODE == STAGED) {
       __syncthreads();
     }
-    rows.refill(row, 0);  // after a barrier: every thread has taken the row out of its stage
+    rows.refill(row, rows.stage);  // after a barrier: every thread has taken the row out of its stage
     rows.next();
     if (has_y) {
 #pragma unroll
@@ -488,7 +545,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
     }
     rows.sum(v, sums[buf]);
     buf ^= 1;
-    rows.refill(row, 1);  // the barrier of the sum: every thread is done with the row before
+    if (row != rows.first) rows.refill(row - rows.step, rows.stage ? rows.stage - 1 : p.stages - 1);  // the barrier of the sum: all are done with the row before
     const float c1 = ((s2 * v[0]) * inv_h * s2) * s2;              // c1 s2^2, as rhat = s2 r; in this order it does not overflow
     const float qg = v[1] - c1 * v[2], c2 = has_post ? s1 * qg * tg * inv_h : 0.f;
     if (token && a.dgate && rows.tid == 0) store1<W>(a.dgate, row, qg);
