@@ -16,6 +16,12 @@ the 126 MB L2 where DRAM figures matter, a few hundred MB on the device at most,
   python -m perftest.kernel_case --kernel grouped_gemm_small   # the same with 16 rows per group, K 2048: the weights' HBM traffic
   python -m perftest.kernel_case --kernel gemm_decode     # few output tiles: 128 x 3584 x 8192 with GELU, weights cold in L2
   python -m perftest.kernel_case --kernel gemm_transposed # both operands stored with K outermost, 2048 x 4096 x 4096
+  python -m perftest.kernel_case --kernel block_norms     # the norms around a block, forward, 4096 x 8192 bf16 (residual and parameters fp32: block_norms_f32)
+  python -m perftest.kernel_case --kernel block_norms_backward | block_norms_backward_f32
+  python -m perftest.kernel_case --kernel moe_route | balance_loss   # 8192 tokens, 256 experts, top-8
+  python -m perftest.kernel_case --kernel mxfp4_quantize | mxfp4_dequantize   # 8192 x 8192, bf16 in, fp32 out
+  python -m perftest.kernel_case --kernel mxfp4_gemm      # 8192 x 8192 x 3584 in microscaled 4-bit floats
+  python -m perftest.kernel_case --kernel mxfp4_gemm_decode   # 16 x 8192 x 8192, weights cold in L2
   BSHMEM_FUSED_2CTA=0 python -m perftest.kernel_case --kernel gemm   # the one-CTA-per-tile variant of the GEMM kernel
 Prints the CUDA-event time of the last launch.
 """
@@ -94,6 +100,45 @@ def main():
         offs_d = offs.to(dev)
         ms = timed(lambda: fg.grouped_gemm(x, w, offs_d, out=out, act="swiglu"), args.launches)
         print(f"{args.kernel}: {ms:.4f} ms, {2 * R * N * K / ms / 1e9:.1f} TFLOP/s ({G} groups, rows {int(sizes.min())}-{int(sizes.max())})")
+        fg.check_errors()
+        return
+    if args.kernel.startswith("block_norms"):
+        from nvshmem_b200.ops import block_norms
+        T, H = 4096, 8192
+        wide = torch.float32 if args.kernel.endswith("_f32") else torch.bfloat16
+        rn = lambda *s, dt=wide: torch.randn(*s, device=dev).to(dt).requires_grad_("backward" in args.kernel)
+        h, res, post, pre, gate = rn(T, H, dt=torch.bfloat16), rn(T, H), rn(H), rn(H), rn(H)
+        call = lambda: block_norms(h, res, post, pre, gate)
+        if "backward" in args.kernel:
+            outs, leaves = call(), [h, res, post, pre, gate]
+            grads = [torch.randn_like(o) for o in outs]
+            ms = timed(lambda: torch.autograd.grad(outs, leaves, grads, retain_graph=True), args.launches)
+        else:
+            ms = timed(call, args.launches)
+        size = T * H * (2 + res.element_size())
+        print(f"{args.kernel}: {ms * 1e3:.1f} us, {size * (3 if 'backward' in args.kernel else 2) / ms / 1e6:.0f} GB/s")
+        return
+    if args.kernel in ("moe_route", "balance_loss"):
+        from nvshmem_b200.ops import balance_loss, moe_route
+        logits = torch.randn(8192, 256, device=dev)
+        idx, _ = moe_route(logits, 8)
+        ms = timed((lambda: moe_route(logits, 8)) if args.kernel == "moe_route" else (lambda: balance_loss(logits, idx)), args.launches)
+        print(f"{args.kernel}: {ms * 1e3:.1f} us")
+        return
+    if args.kernel.startswith("mxfp4"):
+        from nvshmem_b200.ops import gemm_mxfp4, quantize_mxfp4
+        M, N, K = {"mxfp4_gemm": (8192, 8192, 3584), "mxfp4_gemm_decode": (16, 8192, 8192)}.get(args.kernel, (8192, 0, 8192))
+        x = torch.randn(M, K, device=dev).to(torch.bfloat16)
+        q = quantize_mxfp4(x)
+        if N:
+            ws = [quantize_mxfp4(torch.randn(N, K, device=dev)) for _ in range(6)]  # taken in turn
+            out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+            turn = iter(range(args.launches))
+            ms = timed(lambda: gemm_mxfp4(q, ws[next(turn) % 6], out=out), args.launches)
+            print(f"{args.kernel}: {ms * 1e3:.1f} us, {2 * M * N * K / ms / 1e9:.0f} TFLOP/s, weights at {N * K * 17 / 32 / ms / 1e6:.0f} GB/s")
+        else:
+            ms = timed((lambda: quantize_mxfp4(x)) if args.kernel == "mxfp4_quantize" else (lambda: q.dequantize(torch.float32)), args.launches)
+            print(f"{args.kernel}: {ms * 1e3:.1f} us, {M * K * ((2 if args.kernel == 'mxfp4_quantize' else 4) + 17 / 32) / ms / 1e6:.0f} GB/s")
         fg.check_errors()
         return
     import nvshmem_b200.core as nv
