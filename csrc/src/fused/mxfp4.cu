@@ -322,7 +322,7 @@ using namespace bshmem::mx;
 
 extern "C" size_t bshmem_mxfp4_scale_bytes(int64_t R, int64_t K) { return R > 0 && K > 0 ? (size_t)(row_blocks(R) * k_blocks(K)) * SCALE_BLOCK : 0; }
 
-static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 1 << 27 ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
+static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 1 << 26 ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
 
 extern "C" int bshmem_mxfp4_quantize(const void* x, int type, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const int st = check_matrix(R, K);

@@ -19,7 +19,7 @@ from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
 
 BLOCK = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32 and at most 2^27", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
+_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32 and at most 2^26", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
 
 
 class _GemmArgs(C.Structure):
@@ -92,7 +92,7 @@ class MxFp4:
             raise FusedGemmError("dtype must be bfloat16, float16 or float32")
         device = device_of(FusedGemmError, self.data, self.scales)
         R, K = self.shape
-        out = torch.empty(R, K, dtype=dtype, device=self.data.device)
+        out = self.data.new_empty((R, K), dtype=dtype)
         _raise(_lib().bshmem_mxfp4_dequantize(self.data.data_ptr(), self.scales.data_ptr(), R, K, _TYPES[dtype], out.data_ptr(), stream_of(device)),
                "bshmem_mxfp4_dequantize")
         return out
@@ -109,7 +109,9 @@ def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
     data = x.new_empty((R, K // 2), dtype=torch.uint8)
     scales = x.new_empty(_scale_shape(R, K), dtype=torch.uint8)
     _raise(_lib().bshmem_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], R, K, x.stride(0), data.data_ptr(), scales.data_ptr(), stream_of(device)), "bshmem_mxfp4_quantize")
-    return MxFp4(data, scales, (R, K))
+    q = MxFp4.__new__(MxFp4)   # the shapes are right by construction
+    q.data, q.scales, q.shape = data, scales, (R, K)
+    return q
 
 
 def _checked(x: torch.Tensor) -> tuple[torch.Tensor, int]:

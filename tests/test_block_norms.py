@@ -135,7 +135,8 @@ def test_more_rows_than_ctas(T, H):
 @pytest.mark.gpu
 @pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
 @pytest.mark.parametrize("post,pre", [(True, True), (True, False), (False, True), (False, False)])
-@pytest.mark.parametrize("T,H,dt,rt,wt", [(320, 1032, BF16, F32, BF16), (700, 2048, F16, F16, F32), (301, 4104, F32, F32, F32)])
+@pytest.mark.parametrize("T,H,dt,rt,wt", [(320, 1032, BF16, F32, BF16), (700, 2048, F16, F16, F32), (301, 4104, F32, F32, F32), (1300, 2048, BF16, BF16, BF16),
+                                          (420, 8192, BF16, F32, F32), (1250, 1024, F32, F32, F32)])
 def test_many_rows(gate, post, pre, T, H, dt, rt, wt):
     """More rows than the SMs take at once, which walk them through a ring in shared memory."""
     _check(_norm_inputs(T, H, dt, rt, wt, gate, post, pre), off=1.0)
@@ -158,7 +159,7 @@ def test_many_rows_sizes(T, H, dt, rt, wt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,wt", [(BF16, BF16), (BF16, F32), (F16, F16), (F32, F32)])
-@pytest.mark.parametrize("T,H", [(1, 128), (77, 1000), (260, 7168), (400, 1024), (1000, 7168)])
+@pytest.mark.parametrize("T,H", [(1, 128), (77, 1000), (260, 7168), (400, 1024), (1000, 7168), (1400, 1024), (160, 16384)])
 def test_rms_norm(T, H, dt, wt):
     from nvshmem_b200.ops import norms
     d = _norm_inputs(T, H, dt, dt, wt, "none")
