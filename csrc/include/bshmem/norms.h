@@ -38,7 +38,7 @@ typedef struct {
   const void *dr, *dy;
   void *dh, *dresidual, *dpost, *dpre, *dgate;
   int* error_flag;  /* device int; set to 1 if a copy inside a kernel did not arrive in time */
-  float* partials;  /* bshmem_block_norms_partials(T, H) floats, needed for dpost, dpre and the channel gate's gradient */
+  float* partials;  /* bshmem_block_norms_partials(T, H) floats, 16-byte aligned, needed for dpost, dpre and the channel gate's gradient */
 } bshmem_norm_args_t;
 
 int bshmem_block_norms(const bshmem_norm_args_t* args, cudaStream_t stream);

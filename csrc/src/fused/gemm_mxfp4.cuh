@@ -24,8 +24,10 @@ __host__ __device__ __forceinline__ int64_t row_blocks(int64_t R) { return (R + 
 
 // ------------------------------------------------------------------ CTA pairs
 // Pairs of CTAs walk tiles of 256 rows of x by COLS rows of w (persistent).  Each CTA loads its own 128 rows of x and half the rows of w, the
-// even one issues the MMAs for both, and each CTA's tensor memory gets its own 128 x COLS accumulator: half the traffic from L2 per
-// operation of a single CTA's tile, which at this rate is what bounds it (64 bytes a clock and SM instead of 96).
+// even one issues the MMAs for both, and each CTA's tensor memory gets its own 128 x COLS accumulator: 70 bytes
+// a clock and SM at the full rate of the tensor cores, instead of a single CTA's 102.  Some 50 arrive (12 TB/s over all SMs), which is what
+// bounds it: 8192 x 8192 x 3584 in 82 us (5.9 PFLOP/s), 8192^3 in 165 (6.7), tensor cores busy 0.72 of the time.  One CTA per 128 x 256 tile
+// without overlapped epilogue took 131 us.
 // Tensor memory (COLS = 256): two accumulators, which overlap by the 48 columns that two steps' scales take:
 //   [0, 256) accumulator 0    [208, 464) accumulator 1    [464, 512) scales
 // The epilogue drains the shared columns of a tile first; from then on the other accumulator may be written.
@@ -227,7 +229,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_co
 // One tile of 128 rows of w by COLS rows of x per CTA, in steps of 256 values of K: the weights are the tensor core's first operand.  Here
 // reading the weights is what takes the time: an SM takes in some 60 bytes a clock, so all SMs have to read, and a cluster of CTAs
 // divides K.  Each sends its sums to the shared memory of the CTA that owns the row of x (its number modulo the cluster's size), which
-// adds them in order.  (Owners that fetch the sums instead wait for a round trip per value: 64 x 1024 x 8192 took 19 us that way.)
+// adds them in order.  (Owners that fetch the sums instead wait for a round trip per value: 64 x 1024 x 8192 took 19 us that way, 7.5 now.)
+// 16 x 8192 x 8192: 11.7 us with cold weights (36 MB), 8.9 with warm ones, of which 5.4 are what the smallest product takes.
 //   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
 constexpr int F_THREADS = 256, F_STAGE_W = 128 * 128;
 template <int COLS>

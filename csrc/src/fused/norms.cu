@@ -47,7 +47,7 @@ extern "C" int bshmem_block_norms_backward(const bshmem_norm_args_t* a, cudaStre
   if (st) return st;
   const bool sums = a->dpost || a->dpre || (a->dgate && a->gate_mode == BSHMEM_NORM_GATE_CHANNEL);
   if ((!a->dr && !a->dy) || (a->dpre && !a->dy) || (a->dpost && !a->post) || ((a->dh || a->dgate) && !a->h) || (a->dgate && !a->gate_mode)) return BSHMEM_NORM_ERR_ARGS;
-  if ((sums && !a->partials) || ((a->post || a->dy) && !a->stat) || !a->error_flag) return BSHMEM_NORM_ERR_ARGS;
+  if ((sums && (!a->partials || ((uintptr_t)a->partials & 15))) || ((a->post || a->dy) && !a->stat) || !a->error_flag) return BSHMEM_NORM_ERR_ARGS;
   bshmem_norm_args_t args = *a;
   if (!sums) args.partials = nullptr;
   return run(&args, true, stream);

@@ -5,7 +5,7 @@
 // take 8192 columns.  Each input is read once from memory and each output written once.
 //   STAGED  one thread copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that the bytes in
 //           flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which spill:
-//           backward at 4096 x 8192 took 269 us with it, 119 without.)
+//           backward at 4096 x 8192 took 269 us with it, 119 without, before the steps that followed.)
 //   VECTOR  rows are read where they lie, 8 or 16 bytes at a time: few rows, or rows too large for two stages
 //   SCALAR  the same one value at a time, for odd sizes and addresses
 //
@@ -16,8 +16,12 @@
 //   dpost = branch_scale sum over rows of gate G hhat     dpre = sum of dy rhat
 // c2 is linear in G, so one reduction of three sums serves a row.  (For a gate per token the sums are taken without the gate:
 // they are its gradient.)  Where the gate is per channel it is the same for every row, and one sum S = sum of G hhat gives both
-// dpost = branch_scale gate S and dgate = u S.  A CTA keeps its part of the two
-// sums over rows; a second kernel adds the CTAs' parts in order.
+// dpost = branch_scale gate S and dgate = u S.  A CTA keeps its part of the two sums over rows; a second kernel adds the CTAs' parts
+// in order.
+//
+// Bound by memory, and behind it by the instructions and the one barrier of a row.  4096 x 8192, kernel times (bytes over time): forward bf16 46 us
+// (5.8 TB/s), with an fp32 residual 65 (6.2); backward 89 (4.5) and 106 (5.7), the sums over rows 6 more.  Few rows: 8 x 7168 forward 3.4 us,
+// 777 x 1001 fp16 4.3 and 8.8 + 4.8.  Pairs: 2000 x 16384 bf16 66 and 107.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -106,8 +110,8 @@ __host__ __device__ __forceinline__ StageRows stage_rows(const bshmem_norm_args_
   return r;
 }
 
-// Rows that are absent are read from the residual's place (it is at least as long) and their values dropped, which takes no branch.
-// This CTA's columns of a row's inputs, wherever they are.
+// This CTA's columns of a row's inputs, wherever they are.  Rows that are absent are read from the residual's place (it is at least as
+// long) and their values dropped, which takes no branch.
 struct RowSource {
   const uint8_t *h, *residual, *dr, *dy, *gate;
 };
