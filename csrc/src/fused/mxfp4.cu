@@ -68,51 +68,59 @@ __device__ __forceinline__ uint32_t exponent_bits(const uint4* raw, const float*
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int K, int64_t stride, uint8_t* __restrict__ data,
                                                              uint8_t* __restrict__ scales) {
-  constexpr int UNROLL = sizeof(T) == 4 ? 4 : 8, WORDS = sizeof(T) * 8 / 16;
+  constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2, WORDS = sizeof(T) * 32 / 16;   // a lane takes blocks of 32 values, a warp 1024 values at a time
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may set up, and fetch its weights, beside this kernel
   const RowSlot slot = row_slot();
-  const int half = (threadIdx.x >> 4) & 1, part = threadIdx.x & 15;
-  const int KB = (int)k_blocks(K), first = (int)blockIdx.y * (Q_CHUNK / 128), last = first + Q_CHUNK / 128 < KB ? first + Q_CHUNK / 128 : KB;
+  const int lane = threadIdx.x & 31;
+  const int KB = (int)k_blocks(K), first = (int)blockIdx.y * Q_CHUNK, last = first + Q_CHUNK < KB * 128 ? first + Q_CHUNK : KB * 128;
   const bool row_live = slot.row < R;
-  const T* src = x + slot.row * stride + part * 8;
-  uint8_t* dst = data + slot.row * (K / 2) + part * 4;
+  const T* src = x + slot.row * stride;
+  uint8_t* dst = data + slot.row * (K / 2);
   uint8_t* sdst = scales + (slot.row / 128) * KB * SCALE_BLOCK + slot.scale;
 #pragma unroll 1
-  for (int base = first + half; base < last + half; base += 2 * UNROLL) {
-    const int left = row_live ? K - base * 128 - part * 8 : 0;  // values from this lane's first on
+  for (int base = first + lane * 32; base < last + lane * 32; base += 1024 * UNROLL) {
     uint4 raw[UNROLL][WORDS];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const T* from = src + base * 128 + u * 256;
+      const bool live = row_live && base + u * 1024 < K;
       if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) raw[u][i] = left > u * 256 ? ((const uint4*)from)[i] : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? ((const uint4*)(src + base + u * 1024))[i] : make_uint4(0u, 0u, 0u, 0u);
       } else {
         T* v = (T*)raw[u];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = left > u * 256 ? from[i] : T(0.f);
+        for (int i = 0; i < 32; ++i) v[i] = live ? src[base + u * 1024 + i] : T(0.f);
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      float f[8];
-      const T* v = (const T*)raw[u];
+      const int at = base + u * 1024;
+      uint32_t amax = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
-      uint32_t amax = exponent_bits<T>(raw[u], f);
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      for (int g = 0; g < 4; ++g) {
+        float f[8];
+        const T* v = (const T*)raw[u] + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
+        amax = max(amax, exponent_bits<T>(raw[u] + g * (WORDS / 4), f));
+      }
       const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
       const uint32_t code = biased == 255 ? 255 : max(biased, 2u) - 2;
       const float inv = __uint_as_float((254u - min(code, 254u)) << 23);  // 2^(127 - code)
+      uint32_t packed[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= inv;
-      uint32_t word = code << (8 * (part >> 2));  // the four scales of the sixteen lanes as one word
-      word |= __shfl_xor_sync(0xffffffffu, word, 4);
-      word |= __shfl_xor_sync(0xffffffffu, word, 8);
-      const int kb = base + 2 * u;
-      if (left > u * 256) *(uint32_t*)(dst + kb * 64) = pack_e2m1(f);
-      if (part == 0 && kb < KB) *(uint32_t*)(sdst + kb * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
+      for (int g = 0; g < 4; ++g) {
+        float f[8];
+        const T* v = (const T*)raw[u] + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]) * inv;
+        packed[g] = pack_e2m1(f);
+      }
+      uint32_t word = code << (8 * (lane & 3));  // four lanes' scales as one word
+      word |= __shfl_xor_sync(0xffffffffu, word, 1);
+      word |= __shfl_xor_sync(0xffffffffu, word, 2);
+      if (row_live && at < K) *(uint4*)(dst + at / 2) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+      if ((lane & 3) == 0 && at < KB * 128) *(uint32_t*)(sdst + at / 128 * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
     }
   }
 }
