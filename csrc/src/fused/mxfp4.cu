@@ -27,7 +27,7 @@ __device__ __forceinline__ __half from_f(__half, float v) { return __float2half_
 
 // ------------------------------------------------------------------ quantisation
 // Bound by memory: 2 or 4 bytes read and 17/32 written per value, and the reverse.  A warp takes 2048 values of a row, all its loads on
-// their way before the first is used.  The eight rows of a CTA are those whose scales share a 32-byte sector: r, r + 1 and the same
+// their way before the first is used, marked as read once; so are the values that are read back (8192 x 8192 to fp32 51.5 -> 44.5 us).  The eight rows of a CTA are those whose scales share a 32-byte sector: r, r + 1 and the same
 // 32, 64 and 96 rows on.
 constexpr int Q_THREADS = 256, Q_CHUNK = 2048;
 
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict
       const bool live = row_live && base + u * 1024 < K;
       if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? ((const uint4*)(src + base + u * 1024))[i] : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? __ldcs((const uint4*)(src + base + u * 1024) + i) : make_uint4(0u, 0u, 0u, 0u);
       } else {
         T* v = (T*)raw[u];
 #pragma unroll
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __
         const float v = __uint_as_float((q & 0x80000000u) | (q >> 28 & 7) << 22) * 0x1p126f;
         raw[j] = from_f(T(), v * scale);
       }
-      *(uint4*)(dst + col) = *(uint4*)raw;
+      __stcs((uint4*)(dst + col), *(uint4*)raw);
     }
   }
 }
