@@ -61,17 +61,13 @@ def _dense_like(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Plan:
-    """The settings of a call: everything that is not a tensor."""
-    __slots__ = ("T", "H", "device", "gate_mode", "residual_scale", "branch_scale", "eps", "weight_offset", "dtype")
+    """The settings of a call: everything that is not a tensor.  `head`: the first six fields of the C arguments."""
+    __slots__ = ("T", "H", "device", "gate_mode", "head", "scales")
 
-    def launch(self, fn, name, h, residual, post, pre, gate, r=None, y=None, stat=None, dr=None, dy=None, dh=None, dresidual=None, dpost=None, dpre=None,
-               dgate=None, partials=None) -> None:
-        wt = post if post is not None else pre if pre is not None else gate
-        t = _TYPES[self.dtype]
-        a = _Args(self.T, self.H, t, _TYPES[residual.dtype], t if wt is None else _TYPES[wt.dtype], self.gate_mode, 0 if h is None else h.stride(0), residual.stride(0),
-                  gate.stride(0) if self.gate_mode == _FULL else 0, 0 if dr is None else dr.stride(0), 0 if dy is None else dy.stride(0), self.residual_scale,
-                  self.branch_scale, self.eps, self.weight_offset, _ptr(h), residual.data_ptr(), _ptr(post), _ptr(pre), _ptr(gate), _ptr(r), _ptr(y), _ptr(stat),
-                  _ptr(dr), _ptr(dy), _ptr(dh), _ptr(dresidual), _ptr(dpost), _ptr(dpre), _ptr(dgate), _error_flag(residual.device).data_ptr(), _ptr(partials))
+    def strides(self, h, residual, gate):
+        return 0 if h is None else h.stride(0), residual.stride(0), gate.stride(0) if self.gate_mode == _FULL else 0
+
+    def launch(self, fn, a: _Args, name: str) -> None:
         st = fn(C.byref(a), stream_of(self.device))
         if st != 0:
             raise NormError(f"{name}: {_ERRORS.get(st, st)}")
@@ -81,7 +77,9 @@ def _forward(plan: _Plan, h, residual, post, pre, gate, want_r: bool, want_stat:
     r = _dense_like(residual) if want_r else None
     y = _dense_like(residual if h is None else h) if pre is not None else None
     stat = residual.new_empty((2, plan.T), dtype=torch.float32) if want_stat else None
-    plan.launch(_lib().bshmem_block_norms, "bshmem_block_norms", h, residual, post, pre, gate, r, y, stat)
+    a = _Args(*plan.head, *plan.strides(h, residual, gate), 0, 0, *plan.scales, _ptr(h), residual.data_ptr(), _ptr(post), _ptr(pre), _ptr(gate), _ptr(r), _ptr(y), _ptr(stat),
+              0, 0, 0, 0, 0, 0, 0, _error_flag(residual.device).data_ptr(), 0)
+    plan.launch(_lib().bshmem_block_norms, a, "bshmem_block_norms")
     return r, y, stat
 
 
@@ -96,8 +94,14 @@ def _backward(plan: _Plan, h, residual, post, pre, gate, stat, dr, dy, needs):
     partials = None
     if dpost is not None or dpre is not None or (dgate is not None and plan.gate_mode == _CHANNEL):
         partials = residual.new_empty(_lib().bshmem_block_norms_partials(plan.T, plan.H), dtype=torch.float32)
-    plan.launch(_lib().bshmem_block_norms_backward, "bshmem_block_norms_backward", h, residual, post, pre, gate, None, None, stat, None if dr is None else _rows(dr),
-                None if dy is None else _rows(dy), dh, dres, dpost, None if dy is None else dpre, dgate, partials)
+    if dr is not None:
+        dr = _rows(dr)
+    if dy is not None:
+        dy = _rows(dy)
+    a = _Args(*plan.head, *plan.strides(h, residual, gate), 0 if dr is None else dr.stride(0), 0 if dy is None else dy.stride(0), *plan.scales, _ptr(h), residual.data_ptr(),
+              _ptr(post), _ptr(pre), _ptr(gate), 0, 0, stat.data_ptr(), _ptr(dr), _ptr(dy), _ptr(dh), _ptr(dres), _ptr(dpost), 0 if dy is None else _ptr(dpre), _ptr(dgate),
+              _error_flag(residual.device).data_ptr(), _ptr(partials))
+    plan.launch(_lib().bshmem_block_norms_backward, a, "bshmem_block_norms_backward")
     return grads
 
 
@@ -122,27 +126,33 @@ class _BlockNorms(torch.autograd.Function):
         return (None, None, *_backward(ctx.plan, h, residual, post, pre, gate, stat, dr, dy, ctx.needs_input_grad[2:]))
 
 
-def _check_rows(name: str, t: torch.Tensor, shape) -> None:
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise NormError(f"{name} must be a [T, H] tensor" + (f" of shape {tuple(shape)}" if shape is not None else ""))
-    if t.dtype not in _TYPES:
-        raise NormError(f"{name} must be bfloat16, float16 or float32, not {t.dtype}")
-    if t.shape[0] >= 2 ** 31 or not 1 <= t.shape[1] <= MAX_H:
-        raise NormError(f"fewer than 2^31 rows of 1 to {MAX_H} values, not {tuple(t.shape)}")
+def _check_rows(name: str, t: torch.Tensor) -> tuple[int, int]:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in _TYPES:
+        raise NormError(f"{name} must be a [T, H] tensor of bfloat16, float16 or float32")
+    T, H = t.shape
+    if T >= 2 ** 31 or not 1 <= H <= MAX_H:
+        raise NormError(f"fewer than 2^31 rows of 1 to {MAX_H} values, not {(T, H)}")
+    return T, H
 
 
-def _check_weights(plan: _Plan, **weights) -> None:
-    seen = None
-    for name, w in weights.items():
+def _settings(h, residual, post, pre, gate, T, H, gate_mode, residual_scale, branch_scale, eps, weight_offset) -> _Plan:
+    """The plan of a call, after a look at the parameters' types and shapes."""
+    dtype, wt = (residual if h is None else h).dtype, None
+    for name, w in (("the weight after the block", post), ("the weight before the block", pre), ("gate", gate)):
         if w is None:
             continue
-        if w.dtype not in (plan.dtype, torch.float32):
-            raise NormError(f"{name} must be {plan.dtype} or float32")
-        if seen is not None and w.dtype != seen:
+        if w.dtype is not dtype and w.dtype is not torch.float32:
+            raise NormError(f"{name} must be {dtype} or float32, not {w.dtype}")
+        if wt is not None and w.dtype is not wt:
             raise NormError("the weights and the gate must be of one type")
-        seen = w.dtype
-        if name != "gate" and tuple(w.shape) != (plan.H,):
-            raise NormError(f"{name} must be of shape {(plan.H,)}")
+        wt = w.dtype
+        if name != "gate" and (w.dim() != 1 or w.shape[0] != H):
+            raise NormError(f"{name} must be of shape {(H,)}, not {tuple(w.shape)}")
+    plan = _Plan()
+    plan.T, plan.H, plan.gate_mode = T, H, gate_mode
+    plan.head = T, H, _TYPES[dtype], _TYPES[residual.dtype], _TYPES[wt or dtype], gate_mode
+    plan.scales = float(residual_scale), float(branch_scale), float(eps), float(weight_offset)
+    return plan
 
 
 def _run(plan: _Plan, want_r: bool, h, residual, post, pre, gate):
@@ -156,7 +166,7 @@ def _run(plan: _Plan, want_r: bool, h, residual, post, pre, gate):
         pre = pre.contiguous()
     if gate is not None:
         gate = _rows(gate) if plan.gate_mode == _FULL else gate.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and (residual.requires_grad or any([t is not None and t.requires_grad for t in tensors])):
         out = _BlockNorms.apply(plan, want_r, h, residual, post, pre, gate)
         if want_r and pre is not None:
             return out
@@ -167,15 +177,10 @@ def _run(plan: _Plan, want_r: bool, h, residual, post, pre, gate):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, weight_offset: float = 0.0) -> torch.Tensor:
     """``x * rsqrt(mean(x^2) + eps) * (weight + weight_offset)`` row by row: ``x [T, H]``, ``weight [H]`` of x's type or fp32;
     the result has x's type.  Rows may lie apart (any stride between rows)."""
-    _check_rows("x", x, None)
-    plan = _Plan()
-    plan.T, plan.H = x.shape
-    plan.dtype, plan.gate_mode = x.dtype, _NONE
-    plan.residual_scale, plan.branch_scale, plan.eps, plan.weight_offset = 1.0, 1.0, float(eps), float(weight_offset)
+    T, H = _check_rows("x", x)
     if weight is None:
         raise NormError("weight must be given")
-    _check_weights(plan, weight=weight)
-    return _run(plan, False, None, x, None, weight, None)[1]
+    return _run(_settings(None, x, None, weight, None, T, H, _NONE, 1.0, 1.0, eps, weight_offset), False, None, x, None, weight, None)[1]
 
 
 def block_norms(h: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor | None = None, pre_weight: torch.Tensor | None = None,
@@ -190,24 +195,15 @@ def block_norms(h: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tens
     with ``norm(v) = v * rsqrt(mean(v^2) + eps)``; returns ``(r, y)``, ``r`` of the residual's type and ``y`` of h's.  ``residual`` is
     of h's type or fp32; the weights and the gate are all of h's type or all fp32.  ``gate`` is None, one value per channel ``[H]``,
     per token ``[T, 1]``, or ``[T, H]``.  ``y`` is computed from ``r`` before its rounding."""
-    _check_rows("h", h, None)
-    _check_rows("residual", residual, h.shape)
-    plan = _Plan()
-    plan.T, plan.H = h.shape
-    plan.dtype = h.dtype
-    if residual.dtype not in (h.dtype, torch.float32):
-        raise NormError(f"residual must be {h.dtype} or float32")
-    _check_weights(plan, post_weight=post_weight, pre_weight=pre_weight, gate=gate)
+    T, H = _check_rows("h", h)
+    if not isinstance(residual, torch.Tensor) or residual.shape != h.shape or (residual.dtype is not h.dtype and residual.dtype is not torch.float32):
+        raise NormError(f"residual must be a tensor of shape {(T, H)} in {h.dtype} or float32")
     if gate is None:
-        plan.gate_mode = _NONE
-    elif tuple(gate.shape) == (plan.H,):
-        plan.gate_mode = _CHANNEL
-    elif tuple(gate.shape) == (plan.T, 1):
-        plan.gate_mode = _TOKEN
-    elif tuple(gate.shape) == (plan.T, plan.H):
-        plan.gate_mode = _FULL
+        mode = _NONE
     else:
-        raise NormError(f"gate must be of shape {(plan.H,)}, {(plan.T, 1)} or {(plan.T, plan.H)}, not {tuple(gate.shape)}")
-    plan.residual_scale, plan.branch_scale = float(residual_scale), float(branch_scale)
-    plan.eps, plan.weight_offset = float(eps), float(weight_offset)
+        shape = tuple(gate.shape)
+        mode = _CHANNEL if shape == (H,) else _TOKEN if shape == (T, 1) else _FULL if shape == (T, H) else None
+        if mode is None:
+            raise NormError(f"gate must be of shape {(H,)}, {(T, 1)} or {(T, H)}, not {shape}")
+    plan = _settings(h, residual, post_weight, pre_weight, gate, T, H, mode, residual_scale, branch_scale, eps, weight_offset)
     return _run(plan, True, h, residual, post_weight, pre_weight, gate)

@@ -309,3 +309,20 @@ def test_refusals():
     for call in bad:
         with pytest.raises(NormError):
             call()
+
+
+def test_refusals_name_the_argument():
+    """Shapes and types are refused for what they are, before the look at the device; a tensor given twice is checked in each place."""
+    from nvshmem_b200.ops import norms
+    h, w, token = torch.zeros(4, 64, dtype=BF16), torch.ones(64, dtype=BF16), torch.ones(4, 1, dtype=BF16)
+    bad = [(lambda: norms.rms_norm(h, w[:32]), "before the block must be of shape"), (lambda: norms.rms_norm(h, w.half()), "must be torch.bfloat16 or float32"),
+           (lambda: norms.rms_norm(h, w[None]), "before the block must be of shape"), (lambda: norms.rms_norm(torch.zeros(2, 16385), torch.ones(16385)), "rows of 1 to"),
+           (lambda: norms.block_norms(h, h[:3]), "residual"), (lambda: norms.block_norms(h, h.half()), "residual"), (lambda: norms.block_norms(h.float(), h), "residual"),
+           (lambda: norms.block_norms(h, h, w[:63]), "after the block must be of shape"), (lambda: norms.block_norms(h, h, w, w.float()), "one type"),
+           (lambda: norms.block_norms(h, h, token, gate=token), "after the block must be of shape"),
+           (lambda: norms.block_norms(h, h, None, token, gate=token), "before the block must be of shape"),
+           (lambda: norms.block_norms(h, h, gate=w[:4]), "gate must be of shape"), (lambda: norms.block_norms(h, h, gate=token.float().double()), "gate must be"),
+           (lambda: norms.block_norms(h, h, w, w), "on the GPU")]
+    for call, message in bad:
+        with pytest.raises(norms.NormError, match=message):
+            call()
