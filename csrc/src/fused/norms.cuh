@@ -642,14 +642,10 @@ static inline bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Rows and parameters may be read and written 16 bytes at a time.
 static inline bool vectors(const bshmem_norm_args_t* a) {
   if (a->H % 8) return false;
-  const void* ptrs[] = {a->h, a->residual, a->post, a->pre, a->gate, a->r, a->y, a->dr, a->dy, a->dh, a->dresidual, a->dgate};
+  const bool per_token = a->gate_mode == BSHMEM_NORM_GATE_TOKEN;   // read one by one
+  const void* ptrs[] = {a->h, a->residual, a->post, a->pre, per_token ? nullptr : a->gate, a->r, a->y, a->dr, a->dy, a->dh, a->dresidual, per_token ? nullptr : a->dgate};
   for (const void* q : ptrs)
-    if (!aligned(q)) {
-      if (q == a->gate || q == a->dgate) {
-        if (a->gate_mode == BSHMEM_NORM_GATE_TOKEN) continue;
-      }
-      return false;
-    }
+    if (!aligned(q)) return false;
   return !((a->h_stride | a->res_stride | a->dr_stride | a->dy_stride) & 7) && (a->gate_mode != BSHMEM_NORM_GATE_FULL || !(a->gate_stride & 7));
 }
 

@@ -326,3 +326,17 @@ def test_refusals_name_the_argument():
     for call, message in bad:
         with pytest.raises(norms.NormError, match=message):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, F32])
+def test_a_weight_and_a_gate_in_one_unaligned_place(dt):
+    """A gate per token that shares its memory with the weights, which do not start on 16 bytes."""
+    from nvshmem_b200.ops import norms
+    d = _norm_inputs(64, 64, dt, dt, dt, "token")
+    w = torch.cat([d["post"][:1], d["post"]])[1:]
+    assert w.data_ptr() % 16
+    gate = w.view(64, 1)
+    got = norms.block_norms(d["h"], d["residual"], w, w, gate)
+    want = norms.block_norms(d["h"], d["residual"], w.clone(), w.clone(), gate.clone())
+    assert all(torch.equal(g, x) for g, x in zip(got, want))
