@@ -2,8 +2,8 @@
 //
 // A warp takes a token: lane l holds the logits of experts l, l + 32, ... in registers, so a row is read once in whole lines and
 // everything after that is shuffles.  The choice is K rounds of a maximum over the warp of keys that order like the floats
-// (redux.sync), the lowest expert among equal keys.  A round is some 50 instructions for 256 experts, half of them on the half-rate integer
-// pipe, which is what bounds many tokens: 8192 x 256 takes 5.1 us with one expert a token and 9.9 us with eight (8.9 MB: 1.4 us of
+// (redux.sync), the lowest expert among equal keys, over the few keys that a bound leaves.  Bound by integer instructions and, at
+// 55 tokens an SM, by the latency of one token: 8192 x 256 takes 5.2 us with one expert a token and 7.1 us with eight (8.9 MB: 1.4 us of
 // memory time).  A decode batch (64 x 256, top-8) takes 3.0 us, most of it the launch and the chain of rounds.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -91,6 +91,46 @@ __device__ __forceinline__ void select(uint32_t (&key)[VPL], int rounds, int lan
     for (int i = 0; i < VPL; ++i)
       if (lane + 32 * i == chosen) key[i] = 0;
   }
+}
+
+// The same by way of a bound: of the lanes' largest keys the one in place `rounds` is no larger than any key that is chosen, and few
+// keys reach it (some 10 to 14 of 256 for eight experts, whatever their scale).  Those are set side by side, in the order of the experts, a
+// key a lane.  A round over all keys takes some 50 instructions for 256 experts, and over these seven: 8192 x 256 top-8 9.8 us by select
+// alone, 7.1 so; 512 experts 15.6 and 9.1.  One expert takes 5.3 by select and 5.7 so; up to 128 experts there is no difference.
+// Should more than 32 reach the bound, as when the largest share a few lanes, the rounds go over all keys.
+struct Candidate {
+  uint32_t key;
+  int expert;
+};
+template <int VPL>
+__device__ __forceinline__ void select_bounded(uint32_t (&key)[VPL], int rounds, int lane, Candidate* room, int& expert, uint32_t& its_key) {
+  if (rounds > 1) {
+    uint32_t head = 0, bound = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) head = max(head, key[i]);
+    for (int k = 0; k < rounds; ++k) {
+      bound = __reduce_max_sync(0xffffffffu, head);
+      if (head == bound) head = 0;   // equal ones at once, which only lowers the bound
+    }
+    bound = max(bound, 1u);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const bool in = key[i] >= bound;
+      const unsigned mask = __ballot_sync(0xffffffffu, in);
+      const int at = n + __popc(mask & ((1u << lane) - 1));
+      if (in && at < 32) room[at] = {key[i], lane + 32 * i};
+      n += __popc(mask);
+    }
+    if (n <= 32) {
+      __syncwarp();
+      uint32_t one[1] = {lane < n ? room[lane].key : 0u};
+      select(one, rounds, lane, expert, its_key);
+      if (expert >= 0) expert = room[expert].expert;
+      return;
+    }
+  }
+  select(key, rounds, lane, expert, its_key);
 }
 
 // Score + bias of one expert in 64 bits; `sum` is the softmax's.
@@ -192,16 +232,22 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
   }
   nan = __any_sync(0xffffffffu, nan);
   top = warp_max(top);
+  constexpr bool BOUNDED = VPL >= 8;
+  __shared__ Candidate s_room[BOUNDED ? WARPS : 1][32];
   int mine;  // lane k: the k-th chosen expert
   uint32_t key[VPL], mine_key;
+  auto choose = [&](int rounds) {
+    if constexpr (!BOUNDED) select(key, rounds, lane, mine, mine_key);
+    else select_bounded(key, rounds, lane, s_room[threadIdx.x >> 5], mine, mine_key);
+  };
   if constexpr (!BIAS) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) key[i] = key32(l[i]);
-    select(key, K, lane, mine, mine_key);
+    choose(K);
   } else {
     // Score + bias in 32 bits with the fast exponential and division first.  They and the sum of up to 37 terms are off by less than 4e-6
     // of a score, which is at most 1, and the sum with the bias by half a step.  Where two neighbours in the order are closer than twice
-    // that (two tokens in a hundred), the choice is made in 64 bits.  8192 x 256, top-8: 16.6 us; all in 64 bits 20; 9.9 without a bias.
+    // that (two tokens in a hundred), the choice is made in 64 bits.  8192 x 256, top-8: 12.5 us, 7.1 without a bias.  (All in 64 bits took 20 us where this took 16.6.)
     float s[VPL], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -216,7 +262,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
       key[i] = e < E && l[i] > -CUDART_INF_F ? key32(s[i] * inv + a.bias[e]) : 0u;
     }
     const int rounds = K + 2;
-    select(key, rounds, lane, mine, mine_key);
+    choose(rounds);
     const uint32_t next = __shfl_down_sync(0xffffffffu, mine_key, 1);
     const float v = value32(mine_key);
     const unsigned unclear = __ballot_sync(0xffffffffu, lane <= K && mine_key && next && !(v - value32(next) > 1e-5f + 5e-7f * fabsf(v)));

@@ -287,3 +287,21 @@ def test_refusals():
     for call in bad:
         with pytest.raises(RoutingError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E, K", [(100, 8), (256, 8), (256, 16), (384, 8), (512, 1), (1000, 16), (1024, 6)])
+def test_where_the_largest_lie(E, K, dt):
+    """The largest logits in a few columns modulo 32, in the first and the last columns, few finite ones, many equal ones: the order is that of a stable sort."""
+    from nvshmem_b200.ops import moe_route
+    g = torch.Generator().manual_seed(E + K)
+    e = torch.arange(E)
+    rows = [torch.randn(E, generator=g) + 10.0 * (e % 32 < n) for n in (1, 2, 4, 5, 8, 31)]
+    rows += [torch.randn(E, generator=g) + 10.0 * (e % 32 == E % 32), torch.randn(E, generator=g) + 10.0 * (e < 40), torch.randn(E, generator=g) + 10.0 * (e >= E - 3)]
+    rows += [torch.randn(E, generator=g).masked_fill(e % 32 >= n, -float("inf")) for n in (1, 2, 3, 9)]
+    rows += [torch.randn(E, generator=g).masked_fill(torch.randperm(E, generator=g) >= n, -float("inf")) for n in (0, 1, K - 1, K, K + 1, 40)]
+    rows += [torch.zeros(E), (e % 2).float(), (e // 32).float(), -(e // 32).float(), torch.randint(0, 3, (E,), generator=g).float(), torch.randint(0, 40, (E,), generator=g).float()]
+    logits = torch.stack(rows).to(dt).cuda()
+    for bias in (None, torch.zeros(E, device="cuda")):   # a bias orders by the sigmoids, where logits from 37 on are equal
+        _check_route(logits, K, score="sigmoid", bias=bias)
