@@ -125,9 +125,10 @@ struct Rows {
   volatile int* abort_flag = nullptr;
   StageRows at;
   int tid, threads, base, cols, stage = 0;  // base, cols: this CTA's columns
-  uint32_t phase = 0;
+  uint32_t phase = 0, copies = 0;  // copies: the parts of a row that this thread copies, by number
   size_t first, step;
 
+  static constexpr uint32_t ARRIVE = 1u << 31;   // of one thread
   static constexpr uint64_t WAIT_NS = 10000000000ull;  // the waits are for this CTA's own copies
 
   __device__ __forceinline__ RowSource global(size_t row) const {
@@ -141,23 +142,22 @@ struct Rows {
     g.gate = (const uint8_t*)a.gate + (row * a.gate_stride + base) * ws;
     return g;
   }
-  // Starts the copy of a row into a stage that nobody reads any more.  One thread of each of the first five warps (of all, if there are
-  // fewer), so that no warp is held up by all the copies.
+  // Starts this thread's share of the copy of a row into a stage that nobody reads any more.  Only the addresses that it needs are formed:
+  // its warp issues whatever one of its lanes does.
   __device__ __forceinline__ void load(size_t row, int to) const {
-    const RowSource g = global(row);
-    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    auto mine = [&](int copy) { return copy % warps == warp; };
-    const int ts = type_bytes(p.a.type), rs = type_bytes(p.a.res_type), ws = type_bytes(p.a.wt_type);
     uint8_t* dst = data + (size_t)to * p.stage_bytes;
     uint64_t* bar = &full[to];
-    if (mine(0)) {
-      sm100::mbar_expect_tx(bar, at.bytes);  // the phase ends when this has arrived and the bytes of all copies are in
-      if (at.residual >= 0) sm100::bulk_load(dst + at.residual, g.residual, cols * rs, bar);
-    }
-    if (at.h >= 0 && mine(1)) sm100::bulk_load(dst + at.h, g.h, cols * ts, bar);
-    if (at.dr >= 0 && mine(2)) sm100::bulk_load(dst + at.dr, g.dr, cols * rs, bar);
-    if (at.dy >= 0 && mine(3)) sm100::bulk_load(dst + at.dy, g.dy, cols * ts, bar);
-    if (at.gate >= 0 && mine(4)) sm100::bulk_load(dst + at.gate, g.gate, cols * ws, bar);
+    auto copy = [&](int number, int offset, const void* rows, int64_t stride, int bytes) {
+      if (copies >> number & 1) sm100::bulk_load(dst + offset, (const uint8_t*)rows + (row * stride + base) * bytes, cols * bytes, bar);
+    };
+    const bshmem_norm_args_t& a = p.a;
+    const int ts = type_bytes(a.type), rs = type_bytes(a.res_type), ws = type_bytes(a.wt_type);
+    if (copies & ARRIVE) sm100::mbar_expect_tx(bar, at.bytes);  // the phase ends when this has arrived and the bytes of all copies are in
+    copy(0, at.residual, a.residual, a.res_stride, rs);
+    copy(1, at.h, a.h, a.h_stride, ts);
+    copy(2, at.dr, a.dr, a.dr_stride, rs);
+    copy(3, at.dy, a.dy, a.dy_stride, ts);
+    copy(4, at.gate, a.gate, a.gate_stride, ws);
   }
   __device__ __forceinline__ Rows(const RowParams& params, uint8_t* smem, bool backward) : p(params) {
     const int pair = p.half ? 2 : 1, rank = p.half ? blockIdx.x & 1 : 0, groups = blockDim.x / p.threads;
@@ -179,7 +179,15 @@ struct Rows {
         sm100::fence_proxy_async_smem();
       }
       __syncthreads();
-      if ((threadIdx.x & 31) == 0)
+      // One thread of each of the first five warps (of all, if there are fewer), so that no warp is held up by all the copies.
+      if ((threadIdx.x & 31) == 0) {
+        const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, offsets[5] = {at.residual, at.h, at.dr, at.dy, at.gate};
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+          if (offsets[i] >= 0 && i % warps == warp) copies |= 1u << i;
+        if (warp == 0) copies |= ARRIVE;
+      }
+      if (copies)
         for (int i = 0; i < p.stages; ++i)
           if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
     }
@@ -198,7 +206,7 @@ struct Rows {
   __device__ __forceinline__ void refill(size_t row, int its_stage) const {
     if constexpr (MODE == STAGED) {
       const size_t next = row + (size_t)p.stages * step;
-      if ((threadIdx.x & 31) == 0 && next < (size_t)p.a.T) load(next, its_stage);
+      if (copies && next < (size_t)p.a.T) load(next, its_stage);
     }
   }
   __device__ __forceinline__ void next() {
