@@ -126,12 +126,12 @@ struct Rows {
   StageRows at;
   int tid, threads, base, cols, stage = 0;  // base, cols: this CTA's columns
   uint32_t phase = 0, copies = 0;  // copies: the parts of a row that this thread copies, by number
-  size_t first, step;
+  uint32_t first, step;  // rows are below 2^31, and what is added to them far below
 
   static constexpr uint32_t ARRIVE = 1u << 31;   // of one thread
   static constexpr uint64_t WAIT_NS = 10000000000ull;  // the waits are for this CTA's own copies
 
-  __device__ __forceinline__ RowSource global(size_t row) const {
+  __device__ __forceinline__ RowSource global(uint32_t row) const {
     const bshmem_norm_args_t& a = p.a;
     const size_t ts = type_bytes(a.type), rs = type_bytes(a.res_type), ws = type_bytes(a.wt_type);
     RowSource g;
@@ -144,7 +144,7 @@ struct Rows {
   }
   // Starts this thread's share of the copy of a row into a stage that nobody reads any more.  Only the addresses that it needs are formed:
   // its warp issues whatever one of its lanes does.
-  __device__ __forceinline__ void load(size_t row, int to) const {
+  __device__ __forceinline__ void load(uint32_t row, int to) const {
     uint8_t* dst = data + (size_t)to * p.stage_bytes;
     uint64_t* bar = &full[to];
     auto copy = [&](int number, int offset, const void* rows, int64_t stride, int bytes) {
@@ -166,8 +166,8 @@ struct Rows {
     cols = !p.half ? p.a.H : rank ? p.a.H - p.half : p.half;
     at = stage_rows(p.a, cols, backward, KIND);
     tid = threadIdx.x % threads;
-    first = (size_t)(blockIdx.x / pair) * groups + threadIdx.x / threads;
-    step = (size_t)(gridDim.x / pair) * groups;
+    first = (blockIdx.x / pair) * groups + threadIdx.x / threads;
+    step = (gridDim.x / pair) * groups;
     if constexpr (MODE == STAGED) {
       data = smem;
       full = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
@@ -189,11 +189,11 @@ struct Rows {
       }
       if (copies)
         for (int i = 0; i < p.stages; ++i)
-          if (first + i * step < (size_t)p.a.T) load(first + i * step, i);
+          if (first + i * step < (uint32_t)p.a.T) load(first + i * step, i);
     }
     if (p.half) sm100::cluster_sync_all();  // the other CTA runs: its shared memory may be written
   }
-  __device__ __forceinline__ RowSource wait(size_t row) const {
+  __device__ __forceinline__ RowSource wait(uint32_t row) const {
     if constexpr (MODE == STAGED) {
       sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
       const uint8_t* s = data + (size_t)stage * p.stage_bytes;
@@ -203,10 +203,10 @@ struct Rows {
     }
   }
   // All threads are past their last look at `row`, which was in `its_stage`: the stage takes the next row that falls to it.
-  __device__ __forceinline__ void refill(size_t row, int its_stage) const {
+  __device__ __forceinline__ void refill(uint32_t row, int its_stage) const {
     if constexpr (MODE == STAGED) {
-      const size_t next = row + (size_t)p.stages * step;
-      if (copies && next < (size_t)p.a.T) load(next, its_stage);
+      const uint32_t next = row + p.stages * step;
+      if (copies && next < (uint32_t)p.a.T) load(next, its_stage);
     }
   }
   __device__ __forceinline__ void next() {
@@ -270,7 +270,7 @@ struct Rows {
   template <typename W>
   __device__ __forceinline__ const W* mine(const void* parameter) const { return (const W*)parameter + base; }
   template <typename T>
-  __device__ __forceinline__ T* out(void* rows, size_t row) const { return (T*)rows + row * p.a.H + base; }
+  __device__ __forceinline__ T* out(void* rows, uint32_t row) const { return (T*)rows + (size_t)row * p.a.H + base; }
 
   // u = branch_scale (post + offset) gate, without the gate where it differs from row to row.  The loads do not hang on one another.
   template <typename W>
@@ -287,27 +287,49 @@ struct Rows {
 #pragma unroll
     for (int i = 0; i < 4; ++i) u[i] = (has_post ? u[i] + a.weight_offset : 1.f) * (channel ? g[i] : 1.f) * a.branch_scale;
   }
-  // Sum over a row's threads, the same value in every one of them.  One barrier per sum: consecutive sums use two buffers in turn.
+  // Sums over a row's threads, the same values in every one of them.  One barrier per sum: consecutive sums use two buffers in turn.
+  // Two to four values: a lane gives away half of what it holds at each of the first exchanges, so that 6 shuffles do what 5 a value would; a
+  // lane then holds value `lane % PLACES`, its bits the other way round.
   template <int N>
-  __device__ __forceinline__ void sum(float (&v)[N], float (*s)[N]) const {
+  static constexpr int PLACES = N == 1 ? 1 : N == 2 ? 2 : 4;
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N], float (*s)[PLACES<N>]) const {
+    static_assert(N <= 4, "places");
+    constexpr int P = PLACES<N>;
+    const int lane = threadIdx.x & 31;
+    auto exchange = [&](float keep_low, float keep_high, int bit) {  // the sum of what the lanes with (without) the bit keep
+      const bool high = lane & bit;
+      return (high ? keep_high : keep_low) + __shfl_xor_sync(0xffffffffu, high ? keep_low : keep_high, bit);
+    };
+    float x = v[0];
+    if constexpr (P == 2) x = exchange(v[0], v[1], 1);
+    if constexpr (P == 4) {
+      float y[2];
+      y[0] = exchange(v[0], v[2], 1);
+      y[1] = N == 4 ? exchange(v[1], v[N - 1], 1) : exchange(v[1], 0.f, 1);
+      x = exchange(y[0], y[1], 2);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = P; o < 32; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+    auto lane_of = [](int i) { return P == 4 ? (i >> 1) + (i & 1) * 2 : i; };
+    if (blockDim.x != threads) {  // a warp's row
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    if (blockDim.x != threads) return;  // a warp's row
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (lane == 0)
-#pragma unroll
-      for (int i = 0; i < N; ++i) s[warp][i] = v[i];
+      for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, x, lane_of(i));
+      return;
+    }
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (lane < P) s[warp][lane] = x;
     __syncthreads();
+    x = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lane < warps ? s[lane][i] : 0.f;
+    for (int w = 0; w < ROW_THREADS / 32; w += 32 / P) {
+      const int from = w + lane / P;
+      if (from < warps) x += s[from][lane % P];
+    }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
+    for (int o = P; o < 32; o *= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, x, lane_of(i));
     if (!p.half) return;
     if (threadIdx.x == 0) {  // to the other CTA
       const uint32_t other = sm100::mapa_u32(sm100::smem_u32(&s[SUM_ROWS - 1][0]), (sm100::cluster_ctarank() ^ 1));
@@ -357,7 +379,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
     RowSource src = rows.wait(rows.first);   // there are more rows than CTAs
     float v[2] = {squares(src), 0.f};
     rows.sum(v, sums[0]);
-    for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+    for (uint32_t row = rows.first; row < (uint32_t)a.T; row += rows.step) {
       const float inv = rsqrtf(v[0] * inv_h + a.eps);
       float r[ROW_CH][4];
       v[0] = v[1] = 0.f;
@@ -375,7 +397,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
       }
       const int stage = rows.stage;
       rows.next();
-      if (row + rows.step < (size_t)a.T) {
+      if (row + rows.step < (uint32_t)a.T) {
         src = rows.wait(row + rows.step);
         v[0] = squares(src);
       }
@@ -398,7 +420,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
     return;
   }
   int buf = 0;
-  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+  for (uint32_t row = rows.first; row < (uint32_t)a.T; row += rows.step) {
     const float tg = token ? load1<W>(a.gate, row) : 1.f;
     const RowSource src = rows.wait(row);
     float r[ROW_CH][4], ss[SUMS] = {};
@@ -480,7 +502,7 @@ template <typename T, typename R, typename W, Mode MODE, Kind KIND>
 __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sums[2][SUM_ROWS][3];
+  __shared__ float sums[2][SUM_ROWS][4];   // room for three and an empty place
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the kernel that adds the CTAs' sums waits for this one itself
   Rows<MODE, KIND> rows(p, smem, true);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
@@ -501,15 +523,15 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
   }
   // The row's scalars, read one row ahead.
   float tg = 1.f, s1 = 1.f, s2 = 0.f, tg_next = 1.f, s1_next = 1.f, s2_next = 0.f;
-  auto scalars = [&](size_t row) {
-    if (row >= (size_t)a.T) return;
+  auto scalars = [&](uint32_t row) {
+    if (row >= (uint32_t)a.T) return;
     if (token) tg_next = load1<W>(a.gate, row);
     if (has_h && has_post) s1_next = a.stat[row];
     if (has_dy) s2_next = a.stat[a.T + row];
   };
   scalars(rows.first);
   int buf = 0;
-  for (size_t row = rows.first; row < (size_t)a.T; row += rows.step) {
+  for (uint32_t row = rows.first; row < (uint32_t)a.T; row += rows.step) {
     tg = tg_next, s1 = s1_next, s2 = s2_next;
     scalars(row + rows.step);
     const RowSource src = rows.wait(row);
