@@ -54,6 +54,17 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// Two values of a 16-bit type that share a word.
+template <typename T>
+__device__ __forceinline__ void pair(float* f, uint32_t word) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    f[0] = __uint_as_float(word << 16);
+    f[1] = __uint_as_float(word & 0xffff0000u);
+  } else {
+    const float2 v = __half22float2(*(const __half2*)&word);
+    f[0] = v.x, f[1] = v.y;
+  }
+}
 // Element i of a parameter of type W.
 template <typename W>
 __device__ __forceinline__ float load1(const void* p, size_t i) {
@@ -242,11 +253,14 @@ struct Rows {
       }
     } else {
       const int at = col(c, 0);
-      alignas(16) T raw[4];
-      if constexpr (sizeof(T) == 4) *(uint4*)raw = EVEN || at < cols ? *(const uint4*)((const T*)row + at) : make_uint4(0u, 0u, 0u, 0u);
-      else *(uint2*)raw = EVEN || at < cols ? *(const uint2*)((const T*)row + at) : make_uint2(0u, 0u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = to_f<T>(raw[i]);
+      if constexpr (sizeof(T) == 4) {
+        const float4 raw = EVEN || at < cols ? *(const float4*)((const T*)row + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        f[0] = raw.x, f[1] = raw.y, f[2] = raw.z, f[3] = raw.w;
+      } else {
+        const uint2 raw = EVEN || at < cols ? *(const uint2*)((const T*)row + at) : make_uint2(0u, 0u);
+        pair<T>(f, raw.x);
+        pair<T>(f + 2, raw.y);
+      }
     }
   }
   template <typename T>
@@ -535,10 +549,12 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
     tg = tg_next, s1 = s1_next, s2 = s2_next;
     scalars(row + rows.step);
     const RowSource src = rows.wait(row);
-    // h, ge = the row's gate, q = gate u hhat, r, dy, g = dr + s2 dy pre of four columns
-    // (products with an absent part are left out where that is known: 0 * x is not 0 for every x)
-    auto values = [&](int c, float* h, float* ge, float* q, float* r, float* dy, float* g) {
-      if (KIND != OUT) rows.template load4<R>(r, src.residual, c);
+    // Of four columns: h, ge = the row's gate, uh = u h (with the row's gate), rh = rhat, dy, g = dr + s2 dy pre.  s1 and s2 stay out of what
+    // they need not be in: q = s1 uh, and rhat = s2 residual_scale residual + s1 s2 uh.
+    // (Products with an absent part are left out where that is known: 0 * x is not 0 for every x.)
+    const float s12 = s1 * s2, s2r = s2 * a.residual_scale;
+    auto values = [&](int c, float* h, float* ge, float* uh, float* rh, float* dy, float* g) {
+      if (KIND != OUT) rows.template load4<R>(rh, src.residual, c);
       if (KIND != IN) rows.template load4<T>(h, src.h, c);
       if (KIND != IN) rows.template load4<R>(g, src.dr, c);
       if (KIND != OUT) rows.template load4<T>(dy, src.dy, c);
@@ -550,62 +566,61 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
         if (!has_dr) g[i] = 0.f;
         if (!has_dy) dy[i] = 0.f;
         if constexpr (KIND != IN) {
-          q[i] = s1 * (u[c][i] * h[i]);
-          if (full || token) q[i] *= ge[i];
+          uh[i] = u[c][i] * h[i];
+          if (full || token) uh[i] *= ge[i];
         }
         if constexpr (KIND == IN) {
-          r[i] *= a.residual_scale;
+          rh[i] *= s2r;
           g[i] = s2 * (dy[i] * wp[c][i]);
         } else if constexpr (KIND != OUT) {
-          r[i] = a.residual_scale * r[i] + q[i];
+          rh[i] = s2r * rh[i] + s12 * uh[i];
           g[i] += s2 * (dy[i] * wp[c][i]);
+          if (!has_dy) rh[i] = 0.f;
         }
       }
     };
     float v[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < ROW_CH; ++c) {
-      float h[4], ge[4], q[4], r[4], dy[4], g[4];
-      values(c, h, ge, q, r, dy, g);
+      float h[4], ge[4], uh[4], rh[4], dy[4], g[4];
+      values(c, h, ge, uh, rh, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (KIND != OUT) v[0] += dy[i] * wp[c][i] * r[i];
+        if constexpr (KIND != OUT) v[0] += dy[i] * wp[c][i] * rh[i];
         if constexpr (KIND != IN) {
-          if (token) q[i] = s1 * (u[c][i] * h[i]);   // without the gate: see c2
-          v[1] += q[i] * g[i];
-          if constexpr (KIND != OUT) v[2] += q[i] * r[i];
+          if (token) uh[i] = u[c][i] * h[i];   // without the gate: see c2
+          v[1] += uh[i] * g[i];
+          if constexpr (KIND != OUT) v[2] += uh[i] * rh[i];
         }
       }
     }
     rows.sum(v, sums[buf]);
     buf ^= 1;
     if (row != rows.first) rows.refill(row - rows.step, rows.stage ? rows.stage - 1 : p.stages - 1);  // the barrier of the sum: all are done with the row before
-    const float c1 = ((s2 * v[0]) * inv_h * s2) * s2;              // c1 s2^2, as rhat = s2 r; in this order it does not overflow
-    const float qg = v[1] - c1 * v[2], c2 = has_post ? s1 * qg * tg * inv_h : 0.f;
+    const float c1 = v[0] * inv_h * s2, qg = s1 * (v[1] - c1 * v[2]), c2 = qg * tg * inv_h * s1 * s1;   // times s2, a sum, and times s1^2
     if (token && a.dgate && rows.tid == 0) store1<W>(a.dgate, row, qg);
 #pragma unroll
     for (int c = 0; c < ROW_CH; ++c) {
-      float h[4], ge[4], q[4], r[4], dy[4], g[4];
-      values(c, h, ge, q, r, dy, g);
+      float h[4], ge[4], uh[4], rh[4], dy[4], g[4];
+      values(c, h, ge, uh, rh, dy, g);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (KIND != OUT) {
-          g[i] -= c1 * r[i];
-          acc_p[c][i] += (s2 * dy[i]) * r[i];
+          g[i] -= c1 * rh[i];
+          acc_p[c][i] += dy[i] * rh[i];
         }
         dy[i] = a.residual_scale * g[i];
         if constexpr (KIND != IN) {
-          float gs = s1 * g[i];
-          if (full || token) gs *= ge[i];
-          acc_s[c][i] += gs * h[i];
-          q[i] = s1 * (g[i] * u[c][i]);
-          r[i] = (full || token ? ge[i] * q[i] : q[i]) - (s1 * c2) * h[i];
-          q[i] *= h[i];
+          g[i] *= s1;
+          if (full && a.dgate) uh[i] = u[c][i] * h[i] * g[i];
+          if (full || token) g[i] *= ge[i];
+          acc_s[c][i] += g[i] * h[i];
+          h[i] = has_post ? u[c][i] * g[i] - c2 * h[i] : u[c][i] * g[i];
         }
       }
       if (a.dresidual) rows.store4(rows.template out<R>(a.dresidual, row), c, dy);
-      if (KIND != IN && a.dh) rows.store4(rows.template out<T>(a.dh, row), c, r);
-      if (full && a.dgate) rows.store4(rows.template out<W>(a.dgate, row), c, q);
+      if (KIND != IN && a.dh) rows.store4(rows.template out<T>(a.dh, row), c, h);
+      if (full && a.dgate) rows.store4(rows.template out<W>(a.dgate, row), c, uh);
     }
     rows.next();
   }
