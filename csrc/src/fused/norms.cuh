@@ -6,6 +6,7 @@
 //   STAGED  one thread copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that the bytes in
 //           flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which spill:
 //           backward at 4096 x 8192 took 269 us with it, 119 without, before the steps that followed.)
+//   EARLY   the same, but a stage is filled again as soon as all warps have left it, not at the barrier of the next row (backward)
 //   VECTOR  rows are read where they lie, 8 or 16 bytes at a time: few rows, or rows too large for two stages
 //   SCALAR  the same one value at a time, for odd sizes and addresses
 //
@@ -75,7 +76,8 @@ __device__ __forceinline__ void store1(void* p, size_t i, float v) {
   ((W*)p)[i] = from_f<W>(v);
 }
 
-enum Mode { STAGED, VECTOR, SCALAR };
+enum Mode { STAGED, EARLY, VECTOR, SCALAR };
+__host__ __device__ constexpr bool staged(Mode m) { return m == STAGED || m == EARLY; }
 // What a kernel knows of its calls at compile time, besides a multiple of 512 columns (every warp has all of its own):
 //   BOTH  h, both norms, a gate per channel or none (backward: both gradients)
 //   IN    no h: the norm of a row alone      OUT  h, the norm after it, no norm that follows, any gate but [T][H]
@@ -132,7 +134,7 @@ struct Rows {
   static constexpr bool EVEN = KIND != ANY;  // whole warps of columns: nothing to guard
   const RowParams& p;
   uint8_t* data = nullptr;
-  uint64_t* full = nullptr;
+  uint64_t *full = nullptr, *empty = nullptr;
   volatile int* abort_flag = nullptr;
   StageRows at;
   int tid, threads, base, cols, stage = 0;  // base, cols: this CTA's columns
@@ -179,13 +181,17 @@ struct Rows {
     tid = threadIdx.x % threads;
     first = (blockIdx.x / pair) * groups + threadIdx.x / threads;
     step = (gridDim.x / pair) * groups;
-    if constexpr (MODE == STAGED) {
+    if constexpr (staged(MODE)) {
       data = smem;
       full = (uint64_t*)(smem + (size_t)p.stages * p.stage_bytes);
-      abort_flag = (volatile int*)(full + MAX_STAGES);
+      empty = full + MAX_STAGES;
+      abort_flag = (volatile int*)(empty + MAX_STAGES);
       if (threadIdx.x == 0) {
         *abort_flag = 0;
-        for (int i = 0; i < p.stages; ++i) sm100::mbar_init(&full[i], 1);
+        for (int i = 0; i < p.stages; ++i) {
+          sm100::mbar_init(&full[i], 1);
+          sm100::mbar_init(&empty[i], blockDim.x >> 5);
+        }
         sm100::mbar_fence_init();
         sm100::fence_proxy_async_smem();
       }
@@ -205,7 +211,7 @@ struct Rows {
     if (p.half) sm100::cluster_sync_all();  // the other CTA runs: its shared memory may be written
   }
   __device__ __forceinline__ RowSource wait(uint32_t row) const {
-    if constexpr (MODE == STAGED) {
+    if constexpr (staged(MODE)) {
       sm100::mbar_wait(&full[stage], phase, WAIT_NS, abort_flag);
       const uint8_t* s = data + (size_t)stage * p.stage_bytes;
       return {s + max(at.h, 0), s + max(at.residual, 0), s + max(at.dr, 0), s + max(at.dy, 0), s + at.gate};
@@ -215,13 +221,31 @@ struct Rows {
   }
   // All threads are past their last look at `row`, which was in `its_stage`: the stage takes the next row that falls to it.
   __device__ __forceinline__ void refill(uint32_t row, int its_stage) const {
-    if constexpr (MODE == STAGED) {
+    if constexpr (staged(MODE)) {
       const uint32_t next = row + p.stages * step;
       if (copies && next < (uint32_t)p.a.T) load(next, its_stage);
     }
   }
+  // The same without a barrier (EARLY): a warp says that it is past its last look at the current row, and the threads that copy wait
+  // for all to have said so of the row before this one a little later, when that is hardly a wait.
+  __device__ __forceinline__ void release() const {
+    if constexpr (MODE == EARLY) {
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) sm100::mbar_arrive(&empty[stage]);
+    }
+  }
+  __device__ __forceinline__ void refill_before(uint32_t row) const {
+    if constexpr (MODE == EARLY) {
+      const uint32_t next = row + (p.stages - 1) * step;
+      if (copies && row != first && next < (uint32_t)p.a.T) {
+        const int its_stage = stage ? stage - 1 : p.stages - 1;
+        sm100::mbar_wait(&empty[its_stage], stage ? phase : phase ^ 1, WAIT_NS, abort_flag);
+        load(next, its_stage);
+      }
+    }
+  }
   __device__ __forceinline__ void next() {
-    if constexpr (MODE == STAGED) {
+    if constexpr (staged(MODE)) {
       if (++stage == p.stages) {
         stage = 0;
         phase ^= 1;
@@ -229,7 +253,7 @@ struct Rows {
     }
   }
   __device__ __forceinline__ void end() const {
-    if constexpr (MODE == STAGED) {
+    if constexpr (staged(MODE)) {
       __syncthreads();
       if (!*abort_flag) return;
       const uint64_t t0 = sm100::timer_ns();  // copies still in flight land before the shared memory goes away
@@ -360,7 +384,7 @@ template <typename T, typename R, typename W, Mode MODE, Kind KIND>
 __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_kernel(const __grid_constant__ RowParams p) {
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int SUMS = MODE == STAGED && KIND == BOTH ? 2 : 1;
+  constexpr int SUMS = staged(MODE) && KIND == BOTH ? 2 : 1;
   __shared__ float sums[2][SUM_ROWS][SUMS];
   Rows<MODE, KIND> rows(p, smem, false);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
@@ -376,7 +400,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
       for (int i = 0; i < 4; ++i) wp[c][i] += a.weight_offset;
     }
   }
-  if constexpr (MODE == STAGED && KIND == BOTH) {
+  if constexpr (staged(MODE) && KIND == BOTH) {
     // One barrier a row: the sum of squares of the next row's h goes together with the one of this row's r.
     auto squares = [&](const RowSource& src) {
       float sum = 0.f;
@@ -439,12 +463,12 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
     const RowSource src = rows.wait(row);
     float r[ROW_CH][4], ss[SUMS] = {};
     if (has_h) {
-      float inv = 1.f, res[MODE == STAGED ? 1 : ROW_CH][4];
+      float inv = 1.f, res[staged(MODE) ? 1 : ROW_CH][4];
       ss[0] = 0.f;
 #pragma unroll
       for (int c = 0; c < ROW_CH; ++c) {
         rows.template load4<T>(r[c], src.h, c);
-        if constexpr (MODE != STAGED) rows.template load4<R>(res[c], src.residual, c);  // on the way during the sum
+        if constexpr (!staged(MODE)) rows.template load4<R>(res[c], src.residual, c);  // on the way during the sum
       }
 #pragma unroll
       for (int c = 0; c < ROW_CH; ++c)
@@ -467,9 +491,9 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
 #pragma unroll
           for (int i = 0; i < 4; ++i) r[c][i] *= x[i];
         }
-        if constexpr (MODE == STAGED) rows.template load4<R>(x, src.residual, c);
+        if constexpr (staged(MODE)) rows.template load4<R>(x, src.residual, c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[c][i] += a.residual_scale * (MODE == STAGED ? x[i] : res[MODE == STAGED ? 0 : c][i]);
+        for (int i = 0; i < 4; ++i) r[c][i] += a.residual_scale * (staged(MODE) ? x[i] : res[staged(MODE) ? 0 : c][i]);
       }
     } else {
 #pragma unroll
@@ -494,7 +518,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
       buf ^= 1;
       inv = rsqrtf(ss[0] * inv_h + a.eps);
       if (rows.tid == 0 && a.stat) a.stat[a.T + row] = inv;
-    } else if (MODE == STAGED) {
+    } else if (staged(MODE)) {
       __syncthreads();
     }
     rows.refill(row, rows.stage);  // after a barrier: every thread has taken the row out of its stage
@@ -593,10 +617,11 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
           if constexpr (KIND != OUT) v[2] += uh[i] * rh[i];
         }
       }
+      if (c == 0) rows.refill_before(row);
     }
     rows.sum(v, sums[buf]);
     buf ^= 1;
-    if (row != rows.first) rows.refill(row - rows.step, rows.stage ? rows.stage - 1 : p.stages - 1);  // the barrier of the sum: all are done with the row before
+    if (MODE != EARLY && row != rows.first) rows.refill(row - rows.step, rows.stage ? rows.stage - 1 : p.stages - 1);  // the barrier of the sum: all are done with the row before
     const float c1 = v[0] * inv_h * s2, qg = s1 * (v[1] - c1 * v[2]), c2 = qg * tg * inv_h * s1 * s1;   // times s2, a sum, and times s1^2
     if (token && a.dgate && rows.tid == 0) store1<W>(a.dgate, row, qg);
 #pragma unroll
@@ -622,11 +647,12 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
       if (KIND != IN && a.dh) rows.store4(rows.template out<T>(a.dh, row), c, h);
       if (full && a.dgate) rows.store4(rows.template out<W>(a.dgate, row), c, uh);
     }
+    rows.release();
     rows.next();
   }
   if (a.partials) {
     float* part = a.partials + (size_t)(p.half ? blockIdx.x / 2 : blockIdx.x) * 2 * a.H;
-    if (MODE == STAGED || blockDim.x == rows.threads) {
+    if (staged(MODE) || blockDim.x == rows.threads) {
 #pragma unroll
       for (int c = 0; c < ROW_CH; ++c) {
         rows.store4(part + rows.base, c, acc_s[c]);
@@ -729,14 +755,20 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
   int per_sm = ctas_per_sm(r.kind) * ROW_THREADS / r.block;
   if (per_sm > MAX_CTAS_PER_SM) per_sm = MAX_CTAS_PER_SM;
   if (vec && a->H > WARP_COLS && a->T > sms * per_sm / pair) {
-    // Two stages at least; rather fewer CTAs of an SM than none.
+    // Two stages at least; rather fewer CTAs of an SM than none.  Forward three at most where h is read too: more rows on their way favour some
+    // SMs over others, and the rows are dealt out beforehand (4096 x 8192 bf16 48.5 us with six, 46.5 with three; 8192 x 4096 48.4 and 45.2;
+    // fp32 residual 70 and 68).  A norm alone has half the bytes a row: 24.3 with six, 25.4 with three.
+    const int most_stages = backward || r.kind == IN ? MAX_STAGES : 3;
     r.stage_bytes = stage_rows(*a, cols, backward, r.kind).bytes;
     for (int n = per_sm; n > 0; --n) {
       const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
       if (fit < 2) continue;
       r.mode = STAGED;
-      r.stages = fit < MAX_STAGES ? fit : MAX_STAGES;
-      r.smem = r.stages * r.stage_bytes + MAX_STAGES * 8 + 16;
+      r.stages = fit < most_stages ? fit : most_stages;
+      r.smem = r.stages * r.stage_bytes + MAX_STAGES * 16 + 16;
+      // With two stages the copies would have half a row's time only (backward, fp32 residual, 4096 x 8192: 116 us, 101 early).  With three, or
+      // more CTAs, it costs instructions and gains nothing (bf16 74 us, 76 early; pairs 98 and 109), but for the short rows of a norm alone (49, 46).
+      if (backward && (r.kind == IN || (r.kind != OUT && r.stages == 2 && n == 1))) r.mode = EARLY;
       per_sm = n;
       break;
     }
@@ -791,17 +823,23 @@ constexpr auto kernel_of() {
 }
 template <typename T, typename R, typename W, bool BACKWARD, Mode MODE>
 static void (*by_kind(Kind kind))(RowParams) {
-  if constexpr (std::is_same<T, R>::value)
+  if constexpr (std::is_same<T, R>::value && !(BACKWARD && MODE == STAGED))   // backward, a row alone is EARLY
     if (kind == IN) return kernel_of<T, R, W, BACKWARD, MODE, IN>();
   return kind == BOTH ? kernel_of<T, R, W, BACKWARD, MODE, BOTH>() : kind == OUT ? kernel_of<T, R, W, BACKWARD, MODE, OUT>() : kernel_of<T, R, W, BACKWARD, MODE, ANY>();
+}
+template <typename T, typename R, typename W, bool BACKWARD>
+static void (*early_kernel(Kind kind))(RowParams) {
+  if constexpr (!BACKWARD) return nullptr;   // forward never is
+  else if constexpr (std::is_same<T, R>::value) return kind == IN ? kernel_of<T, R, W, true, EARLY, IN>() : kind == BOTH ? kernel_of<T, R, W, true, EARLY, BOTH>() : kernel_of<T, R, W, true, EARLY, ANY>();
+  else return kind == BOTH ? kernel_of<T, R, W, true, EARLY, BOTH>() : kernel_of<T, R, W, true, EARLY, ANY>();
 }
 template <typename T, typename R, typename W, bool BACKWARD>
 static int launch_rows(const bshmem_norm_args_t* a, cudaStream_t stream) {
   const RowPlan plan = row_plan(a, BACKWARD);
   const RowParams p = {*a, plan.threads, plan.half, plan.stages, plan.stage_bytes};
-  void (*const kernel)(RowParams) = plan.mode == STAGED ? by_kind<T, R, W, BACKWARD, STAGED>(plan.kind) : plan.mode == VECTOR ? by_kind<T, R, W, BACKWARD, VECTOR>(plan.kind)
+  void (*const kernel)(RowParams) = plan.mode == EARLY ? early_kernel<T, R, W, BACKWARD>(plan.kind) : plan.mode == STAGED ? by_kind<T, R, W, BACKWARD, STAGED>(plan.kind) : plan.mode == VECTOR ? by_kind<T, R, W, BACKWARD, VECTOR>(plan.kind)
                                                                                                         : kernel_of<T, R, W, BACKWARD, SCALAR, ANY>();
-  static std::atomic<uint64_t> ready[3][4];
+  static std::atomic<uint64_t> ready[4][4];
   const int st = launch(kernel, plan, p, ready[plan.mode][plan.kind], stream);
   return st || !BACKWARD || !a->partials ? st : launch_column_sums<W>(*a, plan.parts, stream);
 }

@@ -341,3 +341,24 @@ def test_a_weight_and_a_gate_in_one_unaligned_place(dt):
     want, mag = _reference({**d, "post": w, "pre": w, "gate": gate}, 1.0, 1.0, 1e-6, 0.0, backward=False)
     _compare(r, want["r"], mag["r"], "r")
     _compare(y, want["y"], mag["y"], "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,dt,rt,gate,post", [(1700, 8192, BF16, F32, "channel", True), (1333, 7000, BF16, F32, "full", True), (1700, 8192, BF16, F32, "token", False),
+                                                 (2900, 4096, F32, F32, "channel", True), (1024, 8192, F32, F32, "none", True)])
+def test_many_rows_a_cta(T, H, dt, rt, gate, post):
+    """The ring goes round several times."""
+    _check(_norm_inputs(T, H, dt, rt, F32, gate, post, True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H", [(40, 1000), (40, 1001), (400, 2048)])
+def test_infinities_without_norms(T, H):
+    """r = residual + gate h alone: the gradients of h and residual do not depend on either, infinite or not."""
+    from nvshmem_b200.ops import norms
+    d = _norm_inputs(T, H, BF16, F32, BF16, "token", False, False)
+    d["h"][1, 3], d["residual"][2, 5] = float("inf"), -float("inf")
+    h, res = d["h"].requires_grad_(True), d["residual"].requires_grad_(True)
+    dh, dres = torch.autograd.grad(norms.block_norms(h, res, gate=d["gate"])[0], [h, res], d["dr"])
+    assert torch.equal(dres, d["dr"])
+    _compare(dh, d["gate"].double() * d["dr"].double(), (d["gate"].double() * d["dr"].double()).abs(), "d_h")
