@@ -1,6 +1,6 @@
 // C interface of microscaled 4-bit floating point (libbshmem_fused.so): quantisation, reading back, and the product.
 //
-// A matrix [R][K] (K a multiple of 32, at most 2^26) is held as
+// A matrix [R][K] (K a multiple of 32, below 2^26) is held as
 //   data    [R][K/2] bytes: two E2M1 values each, the lower K in the low four bits
 //   scales  E8M0, one byte per 32 values along K, in blocks of 512 bytes that hold 128 rows by 4 scales the way the tensor
 //           core's scale operand wants them: row r, scale s of a block at (r % 32) * 16 + (r / 32) * 4 + s; block (rb, kb) of

@@ -26,7 +26,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f(__nv_bfloat16, float v) { return
 __device__ __forceinline__ __half from_f(__half, float v) { return __float2half_rn(v); }
 
 // ------------------------------------------------------------------ quantisation
-// Bound by memory: 2 or 4 bytes read and 17/32 written per value, and the reverse.  A warp takes 2048 values of a row, all its loads on
+// Bound by memory: 2 or 4 bytes read and 17/32 written per value, and the reverse.  A warp takes 1024 or 2048 values of a row, all its loads on
 // their way before the first is used, marked as read once; so are the values that are read back (8192 x 8192 to fp32 51.5 -> 44.5 us).  The eight rows of a CTA are those whose scales share a 32-byte sector: r, r + 1 and the same
 // 32, 64 and 96 rows on.
 constexpr int Q_THREADS = 256, Q_CHUNK = 2048;
@@ -39,7 +39,7 @@ __device__ __forceinline__ RowSlot row_slot() {
   const int warp = threadIdx.x >> 5, in32 = (blockIdx.x & 15) * 2 + (warp & 1), quarter = warp >> 1;
   return {(int64_t)(blockIdx.x >> 4) * 128 + quarter * 32 + in32, in32 * 16 + quarter * 4};
 }
-static dim3 row_grid(int64_t R, int64_t K) { return dim3((unsigned)(row_blocks(R) * 16), (unsigned)((k_blocks(K) * 128 + Q_CHUNK - 1) / Q_CHUNK)); }
+static dim3 row_grid(int64_t R, int64_t K, int chunk) { return dim3((unsigned)(row_blocks(R) * 16), (unsigned)((k_blocks(K) * 128 + chunk - 1) / chunk)); }
 
 // A lane takes a block of 32 values, so that their largest exponent needs no exchange (8192 x 8192 bf16 34.0 -> 29.9 us against eight values a
 // lane), and four lanes' scales go out as a word.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
@@ -65,63 +65,65 @@ __device__ __forceinline__ uint32_t exponent_bits(const uint4* raw, const float*
   }
 }
 
+// Values of a row that a warp takes, all its loads at once: one block a lane of fp32, two of 16-bit types (1001 x 1184 fp32 3.1 us; with
+// 2048 values in two steps 3.9).
+template <typename T>
+__host__ __device__ constexpr int quantize_chunk() { return sizeof(T) == 4 ? 1024 : 2048; }
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int K, int64_t stride, uint8_t* __restrict__ data,
                                                              uint8_t* __restrict__ scales) {
-  constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2, WORDS = sizeof(T) * 32 / 16;   // a lane takes blocks of 32 values, a warp 1024 values at a time
+  constexpr int UNROLL = quantize_chunk<T>() / 1024, WORDS = sizeof(T) * 32 / 16;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may set up, and fetch its weights, beside this kernel
   const RowSlot slot = row_slot();
   const int lane = threadIdx.x & 31;
-  const int KB = (int)k_blocks(K), first = (int)blockIdx.y * Q_CHUNK, last = first + Q_CHUNK < KB * 128 ? first + Q_CHUNK : KB * 128;
+  const int KB = (int)k_blocks(K), base = (int)blockIdx.y * quantize_chunk<T>() + lane * 32;
   const bool row_live = slot.row < R;
   const T* src = x + slot.row * stride;
   uint8_t* dst = data + slot.row * (K / 2);
   uint8_t* sdst = scales + (slot.row / 128) * KB * SCALE_BLOCK + slot.scale;
-#pragma unroll 1
-  for (int base = first + lane * 32; base < last + lane * 32; base += 1024 * UNROLL) {
-    uint4 raw[UNROLL][WORDS];
+  uint4 raw[UNROLL][WORDS];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const bool live = row_live && base + u * 1024 < K;
-      if constexpr (VEC) {
+  for (int u = 0; u < UNROLL; ++u) {
+    const bool live = row_live && base + u * 1024 < K;
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? __ldcs((const uint4*)(src + base + u * 1024) + i) : make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        T* v = (T*)raw[u];
+      for (int i = 0; i < WORDS; ++i) raw[u][i] = live ? __ldcs((const uint4*)(src + base + u * 1024) + i) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      T* v = (T*)raw[u];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = live ? src[base + u * 1024 + i] : T(0.f);
-      }
+      for (int i = 0; i < 32; ++i) v[i] = live ? src[base + u * 1024 + i] : T(0.f);
     }
+  }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int at = base + u * 1024;
-      uint32_t amax = 0;
+  for (int u = 0; u < UNROLL; ++u) {
+    const int at = base + u * 1024;
+    uint32_t amax = 0;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float f[8];
-        const T* v = (const T*)raw[u] + 8 * g;
+    for (int g = 0; g < 4; ++g) {
+      float f[8];
+      const T* v = (const T*)raw[u] + 8 * g;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
-        amax = max(amax, exponent_bits<T>(raw[u] + g * (WORDS / 4), f));
-      }
-      const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
-      const uint32_t code = biased == 255 ? 255 : max(biased, 2u) - 2;
-      const float inv = __uint_as_float((254u - min(code, 254u)) << 23);  // 2^(127 - code)
-      uint32_t packed[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float f[8];
-        const T* v = (const T*)raw[u] + 8 * g;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]) * inv;
-        packed[g] = pack_e2m1(f);
-      }
-      uint32_t word = code << (8 * (lane & 3));  // four lanes' scales as one word
-      word |= __shfl_xor_sync(0xffffffffu, word, 1);
-      word |= __shfl_xor_sync(0xffffffffu, word, 2);
-      if (row_live && at < K) *(uint4*)(dst + at / 2) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      if ((lane & 3) == 0 && at < KB * 128) *(uint32_t*)(sdst + at / 128 * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
+      for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]);
+      amax = max(amax, exponent_bits<T>(raw[u] + g * (WORDS / 4), f));
     }
+    const uint32_t biased = amax >> 23;  // floor(log2 amax) + 127; 0 for subnormals
+    const uint32_t code = biased == 255 ? 255 : max(biased, 2u) - 2;
+    const float inv = __uint_as_float((254u - min(code, 254u)) << 23);  // 2^(127 - code)
+    uint32_t packed[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float f[8];
+      const T* v = (const T*)raw[u] + 8 * g;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f(v[i]) * inv;
+      packed[g] = pack_e2m1(f);
+    }
+    uint32_t word = code << (8 * (lane & 3));  // four lanes' scales as one word
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    if (row_live && at < K) *(uint4*)(dst + at / 2) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    if ((lane & 3) == 0 && at < KB * 128) *(uint32_t*)(sdst + at / 128 * SCALE_BLOCK) = word;  // of rows and K past the end too: zeros
   }
 }
 
@@ -175,13 +177,13 @@ static int launched(const char* what) {
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
-  if (vec) quantize_kernel<T, true><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
-  else quantize_kernel<T, false><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
+  if (vec) quantize_kernel<T, true><<<row_grid(R, K, quantize_chunk<T>()), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
+  else quantize_kernel<T, false><<<row_grid(R, K, quantize_chunk<T>()), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
   return launched("bshmem_mxfp4_quantize");
 }
 template <typename T>
 static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
-  dequantize_kernel<T><<<row_grid(R, K), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out);
+  dequantize_kernel<T><<<row_grid(R, K, Q_CHUNK), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out);
   return launched("bshmem_mxfp4_dequantize");
 }
 
@@ -330,7 +332,7 @@ using namespace bshmem::mx;
 
 extern "C" size_t bshmem_mxfp4_scale_bytes(int64_t R, int64_t K) { return R > 0 && K > 0 ? (size_t)(row_blocks(R) * k_blocks(K)) * SCALE_BLOCK : 0; }
 
-static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K > 1 << 26 ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
+static int check_matrix(int64_t R, int64_t K) { return R < 0 || K < BLOCK || K % BLOCK || R > 0x7fffff00ll || K >= 1 << 26 ? BSHMEM_MX_ERR_SHAPE : BSHMEM_MX_OK; }
 
 extern "C" int bshmem_mxfp4_quantize(const void* x, int type, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const int st = check_matrix(R, K);

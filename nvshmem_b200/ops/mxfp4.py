@@ -19,7 +19,7 @@ from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
 
 BLOCK = 32
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32 and at most 2^26", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
+_ERRORS = {1: "bad arguments", 2: "shape: K must be a multiple of 32 and below 2^26", 3: "operands must be 16-byte aligned", 4: "CUDA driver/runtime error"}
 
 
 class _GemmArgs(C.Structure):

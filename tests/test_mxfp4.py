@@ -232,3 +232,16 @@ def test_refusals():
     for call in bad:
         with pytest.raises(FusedGemmError):
             call()
+
+
+def test_limits_of_the_entry_points():
+    """Sizes that a launch cannot take are refused before anything is launched (or looked at)."""
+    from nvshmem_b200.ops import mxfp4
+    lib = mxfp4._lib()
+    for R, K in ((1, 1 << 26), (1, (1 << 26) + 32), (1, 33), (1, 0), (-1, 32), (1 << 31, 32)):
+        assert lib.bshmem_mxfp4_quantize(None, 0, R, K, K, None, None, None) == 2
+        assert lib.bshmem_mxfp4_dequantize(None, None, R, K, 0, None, None) == 2
+        a = mxfp4._GemmArgs(M=R, N=8, K=K)
+        assert lib.bshmem_mxfp4_gemm(ctypes.byref(a), None) == 2
+    assert lib.bshmem_mxfp4_quantize(None, 0, 1, (1 << 26) - 32, 0, None, None, None) == 1   # the size would do
+    assert lib.bshmem_mxfp4_quantize(None, 0, 0, 32, 32, None, None, None) == 0
