@@ -236,6 +236,7 @@ def test_refusals():
 
 def test_limits_of_the_entry_points():
     """Sizes that a launch cannot take are refused before anything is launched (or looked at)."""
+    import ctypes
     from nvshmem_b200.ops import mxfp4
     lib = mxfp4._lib()
     for R, K in ((1, 1 << 26), (1, (1 << 26) + 32), (1, 33), (1, 0), (-1, 32), (1 << 31, 32)):
