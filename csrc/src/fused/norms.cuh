@@ -3,9 +3,9 @@
 // Every thread owns sixteen columns for the whole run, with their parameters and their sums over rows in registers; its CTA (up to 512
 // columns its warp, above 8192 its pair of CTAs, half a row each) walks rows with the stride of the grid.  512 threads of 128 registers
 // take 8192 columns.  Each input is read once from memory and each output written once.
-//   STAGED  one thread copies rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that the bytes in
-//           flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which spill:
-//           backward at 4096 x 8192 took 269 us with it, 119 without, before the steps that followed.)
+//   STAGED  threads of the first warps copy rows (cp.async.bulk, 16-byte aligned) into a ring in shared memory ahead of their use, so that
+//           the bytes in flight do not depend on the threads.  (A warp of its own for the copies would leave 96 registers a thread, which
+//           spill: backward at 4096 x 8192 took 269 us with it, 119 without, before the steps that followed.)
 //   EARLY   the same, but a stage is filled again as soon as all warps have left it, not at the barrier of the next row (backward)
 //   VECTOR  rows are read where they lie, 8 or 16 bytes at a time: few rows, or rows too large for two stages
 //   SCALAR  the same one value at a time, for odd sizes and addresses
@@ -21,8 +21,8 @@
 // in order.
 //
 // Bound by memory, and behind it by the instructions and the one barrier of a row.  4096 x 8192, kernel times (bytes over time): forward bf16 46 us
-// (5.8 TB/s), with an fp32 residual 65 (6.2); backward 89 (4.5) and 106 (5.7), the sums over rows 6 more.  Few rows: 8 x 7168 forward 3.4 us,
-// 777 x 1001 fp16 4.3 and 8.8 + 4.8.  Pairs: 2000 x 16384 bf16 66 and 107.
+// (5.8 TB/s), with an fp32 residual 67 (6.0); backward 70 (5.8) and 96 (6.3), the sums over rows 5 more.  Few rows: 8 x 7168 forward 3.2 us,
+// 777 x 1001 fp16 4.2 and 8.9 + 6.  Pairs: 2000 x 16384 bf16 63 and 98.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
