@@ -159,7 +159,7 @@ def test_many_rows_sizes(T, H, dt, rt, wt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,wt", [(BF16, BF16), (BF16, F32), (F16, F16), (F32, F32)])
-@pytest.mark.parametrize("T,H", [(1, 128), (77, 1000), (260, 7168), (400, 1024), (1000, 7168), (1400, 1024), (160, 16384)])
+@pytest.mark.parametrize("T,H", [(1, 128), (77, 1000), (260, 7168), (400, 1024), (1000, 7168), (1400, 1024), (160, 16384), (700, 16384), (3000, 2048)])
 def test_rms_norm(T, H, dt, wt):
     from nvshmem_b200.ops import norms
     d = _norm_inputs(T, H, dt, dt, wt, "none")
@@ -345,7 +345,8 @@ def test_a_weight_and_a_gate_in_one_unaligned_place(dt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,H,dt,rt,gate,post", [(1700, 8192, BF16, F32, "channel", True), (1333, 7000, BF16, F32, "full", True), (1700, 8192, BF16, F32, "token", False),
-                                                 (2900, 4096, F32, F32, "channel", True), (1024, 8192, F32, F32, "none", True)])
+                                                 (2900, 4096, F32, F32, "channel", True), (1024, 8192, F32, F32, "none", True),
+                                                 (500, 16384, BF16, F32, "channel", True), (400, 12296, F16, F32, "full", True)])
 def test_many_rows_a_cta(T, H, dt, rt, gate, post):
     """The ring goes round several times."""
     _check(_norm_inputs(T, H, dt, rt, F32, gate, post, True))
