@@ -8,6 +8,8 @@ Both are differentiable in every tensor argument.  Rows are ``[T, H]`` in bf16, 
 sums over rows are kept in fp32 and every result is rounded once.  The residual stream may be fp32 beside 16-bit blocks, and so may
 the parameters.  Gradients that are sums over rows are added in a fixed order.  Work is issued on the current stream; all tensors lie
 on the current device.
+A backward pass may be captured into a CUDA graph, on leaves of which no eager autograd graph is still alive (torch ties a leaf to the stream that
+used it first): drop the outputs of warm-up calls before the capture.
 """
 from __future__ import annotations
 

@@ -6,6 +6,8 @@
 
 Both are differentiable in the logits, which are ``[T, E]`` in fp32, bf16 or fp16 (rows may lie apart); up to 1024 experts, top-16.
 Everything is computed in fp32.  Work is issued on the current stream; all tensors lie on the current device.
+A backward pass may be captured into a CUDA graph, on leaves of which no eager autograd graph is still alive (torch ties a leaf to the stream that
+used it first): drop the outputs of warm-up calls before the capture.
 """
 from __future__ import annotations
 
