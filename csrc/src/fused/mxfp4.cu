@@ -255,7 +255,8 @@ static int launch_pair(const bshmem_mxfp4_gemm_args_t* a, uint64_t wait_limit_ns
   p.wait_limit_ns = wait_limit_ns;
   p.M = (int)a->M; p.N = (int)a->N; p.K = (int)a->K;
   p.tiles_m = (int)((a->M + 255) / 256);
-  const int64_t tiles = (int64_t)p.tiles_m * ((a->N + COLS - 1) / COLS);
+  p.tiles_n = (int)((a->N + COLS - 1) / COLS);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > 0x3fffffff) return BSHMEM_MX_ERR_SHAPE;
   p.tiles = (int)tiles;
   static std::atomic<uint64_t> ready;

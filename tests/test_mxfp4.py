@@ -169,7 +169,8 @@ def test_products_of_every_kernel(shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K", [(16, 8192, 8192), (3, 7168, 2048), (512, 4096, 7168), (1500, 2816, 1984), (2048, 2047, 1024), (4100, 1032, 512), (2600, 1, 320), (5000, 9, 64), (1, 50001, 64)])
+@pytest.mark.parametrize("M,N,K", [(16, 8192, 8192), (3, 7168, 2048), (512, 4096, 7168), (1500, 2816, 1984), (2048, 2047, 1024), (4100, 1032, 512), (2600, 1, 320), (5000, 9, 64), (1, 50001, 64),
+                                   (9000, 9500, 96), (12345, 8712, 64), (9100, 300, 544)])
 def test_larger_products(M, N, K):
     _check_product(torch.randn(M, K, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(torch.bfloat16),
                    torch.randn(N, K, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(torch.bfloat16) * 0.02)
