@@ -90,6 +90,7 @@ constexpr int MAX_CTAS_PER_SM = 8;
 constexpr int WARP_COLS = 32 * ROW_COLS, WARP_GROUPS = 8;   // rows of a warp each
 constexpr int STAGE_SMEM = 216 * 1024;  // of an SM, shared by its CTAs
 constexpr int SUM_ROWS = 17;            // 16 warps, and the other CTA of a pair
+constexpr int OWN_SMEM = 2 * SUM_ROWS * 4 * sizeof(float), DEFAULT_SMEM = 48 * 1024;  // a kernel's arrays for sums at most; what a launch gets of both without asking
 static_assert(BSHMEM_NORM_MAX_H == 2 * CTA_COLS, "a pair of CTAs takes the longest row");
 
 struct RowParams {
@@ -386,6 +387,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) forward_rows_k
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int SUMS = staged(MODE) && KIND == BOTH ? 2 : 1;
   __shared__ float sums[2][SUM_ROWS][SUMS];
+  static_assert(sizeof(sums) <= OWN_SMEM, "see launch");
   Rows<MODE, KIND> rows(p, smem, false);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
   const bool has_h = KIND == ANY ? a.h != nullptr : KIND != IN, has_post = KIND == ANY ? a.post != nullptr : KIND != IN, has_y = KIND == ANY ? a.y != nullptr : KIND != OUT;
@@ -541,6 +543,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ctas_per_sm(KIND)) backward_rows_
   const bshmem_norm_args_t& a = p.a;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sums[2][SUM_ROWS][4];   // room for three and an empty place
+  static_assert(sizeof(sums) <= OWN_SMEM, "see launch");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the kernel that adds the CTAs' sums waits for this one itself
   Rows<MODE, KIND> rows(p, smem, true);
   const bool token = (KIND == ANY || KIND == OUT) && a.gate_mode == BSHMEM_NORM_GATE_TOKEN, full = KIND == ANY && a.gate_mode == BSHMEM_NORM_GATE_FULL;
@@ -783,7 +786,7 @@ template <typename P>
 static int launch(void (*kernel)(P), const RowPlan& plan, const P& p, std::atomic<uint64_t>& ready, cudaStream_t stream) {
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return BSHMEM_NORM_ERR_DRIVER;
-  if (plan.smem > 48 * 1024 && (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1))) {
+  if (plan.smem + OWN_SMEM > DEFAULT_SMEM && (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1))) {
     if (cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STAGE_SMEM) != cudaSuccess) return BSHMEM_NORM_ERR_DRIVER;
     if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
   }

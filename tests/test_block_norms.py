@@ -363,3 +363,45 @@ def test_infinities_without_norms(T, H):
     dh, dres = torch.autograd.grad(norms.block_norms(h, res, gate=d["gate"])[0], [h, res], d["dr"])
     assert torch.equal(dres, d["dr"])
     _compare(dh, d["gate"].double() * d["dr"].double(), (d["gate"].double() * d["dr"].double()).abs(), "d_h")
+
+
+FRESH = """
+import sys
+import torch
+sys.path.insert(0, {root!r})
+from tests.test_block_norms import _check, _norm_inputs, BF16, F32
+torch.cuda.set_device(0)
+for T, H, dt, rt, wt, gate, pre in (
+        (400, 4080, BF16, BF16, BF16, "channel", True), (1000, 2040, BF16, BF16, F32, "none", True), (900, 2448, BF16, F32, F32, "channel", False),
+        (700, 2720, BF16, F32, BF16, "token", True), (1000, 1632, F32, F32, F32, "full", True), (900, 1528, F32, F32, F32, "channel", True)):
+    _check(_norm_inputs(T, H, dt, rt, wt, gate, True, pre))
+"""
+FRESH_NORM = """
+import torch
+from nvshmem_b200.ops import rms_norm
+torch.cuda.set_device(0)
+for T, H, dt in ((200, 8160, torch.bfloat16), (300, 4080, torch.float32), (900, 2040, torch.float16)):
+    x = torch.randn(T, H, device="cuda").to(dt).requires_grad_(True)
+    y = rms_norm(x, torch.ones(H, device="cuda", dtype=dt))
+    want = x.detach().double()
+    want = want * torch.rsqrt(want.square().mean(-1, keepdim=True) + 1e-6)
+    # half a step of the type (below its smallest normal value the steps stay smallest_normal * eps: a few of a million fp16 values lie
+    # there, where half a step is 2^-25 whatever the value is), and the statistics' part of 2^-18
+    half = torch.finfo(dt).eps / 2
+    assert ((y.detach().double() - want).abs() <= want.abs() * (half + 2.0 ** -18) + torch.finfo(dt).smallest_normal * half).all(), H
+    (g,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert g.isfinite().all()
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("script", [FRESH, FRESH_NORM], ids=["block_norms", "rms_norm"])
+def test_stages_that_just_fit_the_default_shared_memory(script):
+    """Rows whose stages take just under 48 KB: with the kernel's own arrays that is more than a launch gets unless the limit is raised.  In a
+    process of its own, as a limit stays raised once another size has asked for it."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", script.replace("{root!r}", repr(root))], cwd=root, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stderr[-2000:]
