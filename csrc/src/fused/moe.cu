@@ -35,6 +35,7 @@
 
 #include "../../include/bshmem/moe.h"
 #include "../../include/bshmem/tcgen05.cuh"
+#include "launch.cuh"
 
 namespace bshmem {
 namespace moe {
@@ -845,8 +846,7 @@ static int dispatch_local(DispatchParams& P, cudaStream_t stream) {
     auto kernel = fp8 ? dispatch_small_kernel<true> : dispatch_small_kernel<false>;
     st = coop_grid(kernel, 0, a.T * P.split, a.max_ctas, &grid);
     if (st) return st;
-    kernel<<<grid, THREADS, 0, stream>>>(P);
-    return launched("bshmem_moe_dispatch", cudaGetLastError());
+    return launched("bshmem_moe_dispatch", launch_kernel(kernel, grid, THREADS, stream, P));
   }
   // `max_ctas` holds for the call: a smaller cluster routes, and the rows wait for it instead of running beside it.
   int ctas = ROUTE_CTAS;
@@ -940,8 +940,7 @@ static int combine(const bshmem_moe_combine_args_t* a, bool general, cudaStream_
                             : (narrow ? combine_kernel<BSHMEM_MOE_MAX_TOPK, true, true> : combine_kernel<BSHMEM_MOE_MAX_TOPK, true, false>);
     st = coop_grid(kernel, 0, a->T * P.split, a->max_ctas, &grid);
     if (st) return st;
-    kernel<<<grid, THREADS, 0, stream>>>(P);
-    return launched("bshmem_moe_combine", cudaGetLastError());
+    return launched("bshmem_moe_combine", bshmem::launch_kernel(kernel, grid, THREADS, stream, P));
   }
   // Two builds of the kernel: up to 8 choices per token (62 registers, four CTAs per SM) and up to 16 (85, two).
   const void* kernel = a->K <= 8 ? (const void*)combine_kernel<8, false, false> : (const void*)combine_kernel<BSHMEM_MOE_MAX_TOPK, false, false>;

@@ -12,6 +12,7 @@
 #include "../../include/bshmem/mxfp4.h"
 #include "../../include/bshmem/tcgen05.cuh"
 #include "gemm_mxfp4.cuh"
+#include "launch.cuh"
 #include "tensor_map.cuh"
 
 namespace bshmem {
@@ -167,8 +168,7 @@ __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __
   }
 }
 
-static int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+static int launched(const char* what, cudaError_t e) {
   if (e == cudaSuccess) return BSHMEM_MX_OK;
   fprintf(stderr, "%s: launch failed: %s\n", what, cudaGetErrorString(e));
   return BSHMEM_MX_ERR_DRIVER;
@@ -177,14 +177,13 @@ static int launched(const char* what) {
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
-  if (vec) quantize_kernel<T, true><<<row_grid(R, K, quantize_chunk<T>()), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
-  else quantize_kernel<T, false><<<row_grid(R, K, quantize_chunk<T>()), Q_THREADS, 0, stream>>>((const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales);
-  return launched("bshmem_mxfp4_quantize");
+  return launched("bshmem_mxfp4_quantize", launch_kernel(vec ? quantize_kernel<T, true> : quantize_kernel<T, false>, row_grid(R, K, quantize_chunk<T>()), Q_THREADS, stream,
+                                                         (const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales));
 }
 template <typename T>
 static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
-  dequantize_kernel<T><<<row_grid(R, K, Q_CHUNK), Q_THREADS, 0, stream>>>((const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out);
-  return launched("bshmem_mxfp4_dequantize");
+  return launched("bshmem_mxfp4_dequantize",
+                  launch_kernel(dequantize_kernel<T>, row_grid(R, K, Q_CHUNK), Q_THREADS, stream, (const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out));
 }
 
 // Tensor map of scales: rows are row blocks, elements words; a box is 1 KB (256 values of K) of `blocks` row blocks.

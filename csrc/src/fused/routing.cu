@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "../../include/bshmem/routing.h"
+#include "launch.cuh"
 
 namespace bshmem {
 namespace routing {
@@ -597,7 +598,7 @@ static int dispatch(const bshmem_route_args_t* a, F&& f) {
   if (a->type == BSHMEM_ROUTE_BF16) return by_experts<__nv_bfloat16>(a->E, f);
   return by_experts<__half>(a->E, f);
 }
-static int launched() { return cudaGetLastError() == cudaSuccess ? BSHMEM_ROUTE_OK : BSHMEM_ROUTE_ERR_DRIVER; }
+static int launched(cudaError_t e) { return e == cudaSuccess ? BSHMEM_ROUTE_OK : BSHMEM_ROUTE_ERR_DRIVER; }
 
 struct Route {
   const Params& p;
@@ -605,9 +606,7 @@ struct Route {
   template <typename T, int VPL>
   int operator()() const {
     const unsigned grid = ((unsigned)p.a.T + WARPS - 1) / WARPS;
-    if (p.a.bias) route_kernel<T, VPL, true><<<grid, THREADS, 0, stream>>>(p);
-    else route_kernel<T, VPL, false><<<grid, THREADS, 0, stream>>>(p);
-    return launched();
+    return launched(launch_kernel(p.a.bias ? route_kernel<T, VPL, true> : route_kernel<T, VPL, false>, grid, THREADS, stream, p));
   }
 };
 struct RouteBackward {
@@ -615,8 +614,7 @@ struct RouteBackward {
   cudaStream_t stream;
   template <typename T, int VPL>
   int operator()() const {
-    route_backward_kernel<T, VPL><<<((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, 0, stream>>>(p);
-    return launched();
+    return launched(launch_kernel(route_backward_kernel<T, VPL>, ((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, stream, p));
   }
 };
 struct Balance {
@@ -625,8 +623,8 @@ struct Balance {
   template <typename T, int VPL>
   int operator()() const {
     const int grid = balance_ctas(p.a.T);
-    balance_kernel<T, VPL><<<grid, B_THREADS, 0, stream>>>(p);
-    if (grid == 1) return launched();
+    const int st = launched(launch_kernel(balance_kernel<T, VPL>, grid, B_THREADS, stream, p));
+    if (st || grid == 1) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(1);
     cfg.blockDim = dim3(1024);
@@ -636,7 +634,7 @@ struct Balance {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, balance_finish_kernel, p, grid) == cudaSuccess ? BSHMEM_ROUTE_OK : BSHMEM_ROUTE_ERR_DRIVER;
+    return launched(cudaLaunchKernelEx(&cfg, balance_finish_kernel, p, grid));
   }
 };
 struct BalanceBackward {
@@ -644,8 +642,7 @@ struct BalanceBackward {
   cudaStream_t stream;
   template <typename T, int VPL>
   int operator()() const {
-    balance_backward_kernel<T, VPL><<<((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, 0, stream>>>(p);
-    return launched();
+    return launched(launch_kernel(balance_backward_kernel<T, VPL>, ((unsigned)p.a.T + WARPS - 1) / WARPS, THREADS, stream, p));
   }
 };
 

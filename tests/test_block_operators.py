@@ -256,3 +256,49 @@ def test_moe_block_with_the_fused_router(nv, score):
     block.close()
     with pytest.raises(ValueError):
         ExpertParallelMoE(T, H, F, E, K, score="sigmoid")
+
+
+FAILED = """
+import torch
+from nvshmem_b200.ops import gemm_mxfp4, moe_route, norms, quantize_mxfp4
+torch.cuda.set_device(0)
+x, w, y = torch.randn(300, 512, device="cuda"), torch.ones(512, device="cuda"), torch.empty(300, 512, device="cuda")
+logits, q, out = torch.randn(4, 8, device="cuda"), quantize_mxfp4(x), torch.empty(300, 300, device="cuda", dtype=torch.bfloat16)
+plan = norms._settings(None, x, None, w, None, 300, 512, 0, 1.0, 1.0, 1e-6, 0.0)
+plan.device = 0
+def norm():
+    a = norms._Args(*plan.head, *plan.strides(None, x, None), 0, 0, *plan.scales, residual=x.data_ptr(), pre=w.data_ptr(), y=y.data_ptr(), error_flag=flag)
+    plan.launch(norms._lib().bshmem_block_norms, a, "bshmem_block_norms")
+flag = norms._error_flag(x.device).data_ptr()
+call = dict(norm=norm, gemm=lambda: gemm_mxfp4(q, q, out=out))[CALL]   # neither takes memory
+call()
+want = [t.clone() for t in moe_route(logits, 2)]
+torch.cuda.synchronize()
+refused = ""
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            torch.cuda.current_stream().synchronize()   # not allowed here: from now on every launch of this capture fails
+        except RuntimeError:
+            pass
+        try:
+            call()
+        except RuntimeError as e:
+            refused = str(e)
+except RuntimeError:
+    pass
+assert refused.startswith("bshmem"), refused
+for a, b in zip(moe_route(logits, 2), want):   # its own launch is fine
+    assert torch.equal(a, b)
+"""
+
+
+@pytest.mark.parametrize("call", ["norm", "gemm"])
+def test_a_launch_that_fails_is_not_blamed_on_the_next_call(call):
+    """In a process of its own: a capture that was made invalid on the host refuses launches."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", f"CALL = {call!r}\n" + FAILED], cwd=root, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stderr[-2000:]
