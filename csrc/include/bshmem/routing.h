@@ -3,9 +3,10 @@
 // route: the K experts of every token and their weights, from logits [T][E].
 //   choice   the K largest logits, or the K largest of score + bias where `bias` is given (computed in 64 bits, so that the
 //            order does not depend on roundings of the exponential); ties go to the lowest expert.  A logit (or score + bias)
-//            that is -inf or NaN is never chosen; places left over get expert -1 and weight 0.
+//            that is -inf or NaN is never chosen; places left over get expert -1 and weight 0.  The softmax of the biased choice is
+//            taken over the logits that are numbers, and those of +inf share it evenly.
 //   weight   the score of the chosen expert (softmax over all experts, or sigmoid), divided by the sum over the chosen ones
-//            where `renormalize` is set, times `scale`
+//            where `renormalize` is set, times `scale`; NaN for a softmax with a NaN or +inf among the token's logits
 // balance: loss = E * sum_e f_e P_e over the n valid tokens, f_e = counts_e / (n K), P_e = mean over them of the softmax of the
 //   logits (or of the sigmoids divided by their sum)
 // A token whose `valid` byte is 0 gets experts -1 and weights 0, counts nowhere and has a gradient of 0.

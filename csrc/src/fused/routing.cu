@@ -134,16 +134,20 @@ __device__ __forceinline__ void select_bounded(uint32_t (&key)[VPL], int rounds,
   select(key, rounds, lane, expert, its_key);
 }
 
+// Numerator of the softmax that the biased choice goes by, as 32 bits take it below: over the logits that are numbers, those of +inf sharing it
+// evenly, so that a row has an order whichever of the two decides.
+__device__ __forceinline__ double term64(double l, double top) { return l == top ? 1.0 : l > -CUDART_INF ? exp(l - top) : 0.0; }
+
 // Score + bias of one expert in 64 bits; `sum` is the softmax's.
 __device__ __forceinline__ uint64_t key_of(const bshmem_route_args_t& a, double l, double top, double sum, int e) {
-  const double s = a.score == BSHMEM_ROUTE_SOFTMAX ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l));
+  const double s = a.score == BSHMEM_ROUTE_SOFTMAX ? term64(l, top) / sum : 1.0 / (1.0 + exp(-l));
   return l > -CUDART_INF ? key64(s + (double)a.bias[e]) : 0ull;
 }
 template <typename T>
 __device__ __forceinline__ double sum_of(const bshmem_route_args_t& a, const T* row, float top, int lane) {
   double sum = 0.0;
 #pragma unroll 1
-  for (int e = lane; e < a.E; e += 32) sum += exp((double)to_f(row[e]) - (double)top);
+  for (int e = lane; e < a.E; e += 32) sum += term64((double)to_f(row[e]), (double)top);
   return warp_sum(sum);
 }
 
@@ -252,9 +256,14 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
     float s[VPL], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      if (a.score == BSHMEM_ROUTE_SOFTMAX) s[i] = l[i] > -CUDART_INF_F ? __expf(l[i] - top) : 0.f;
+      if (a.score == BSHMEM_ROUTE_SOFTMAX) s[i] = l[i] > -CUDART_INF_F ? __expf(l[i] - top) : 0.f;   // 0 for NaN
       else s[i] = __fdividef(1.f, 1.f + __expf(-l[i]));  // 0 from where the divisor passes 2^126 on
       sum += s[i];
+    }
+    if (a.score == BSHMEM_ROUTE_SOFTMAX && top == CUDART_INF_F) {
+      sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) sum += s[i] = l[i] == top ? 1.f : 0.f;
     }
     const float inv = a.score == BSHMEM_ROUTE_SOFTMAX ? 1.f / warp_sum(sum) : 1.f;
 #pragma unroll
@@ -288,7 +297,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
   } else if (mine >= 0) {
     w = sigmoid(to_f(row[mine]));
   }
-  if ((nan || top == CUDART_INF_F) && a.score == BSHMEM_ROUTE_SOFTMAX) w = CUDART_NAN_F;  // the sum over all experts is NaN
+  if (mine >= 0 && (nan || top == CUDART_INF_F) && a.score == BSHMEM_ROUTE_SOFTMAX) w = CUDART_NAN_F;  // the sum over all experts is NaN
   if (lane < K) {
     a.idx[t * K + lane] = mine;
     a.weight[t * K + lane] = w * a.scale;

@@ -145,7 +145,8 @@ def moe_route(logits: torch.Tensor, topk: int, score: str = "softmax", bias: tor
     sum where ``renormalize`` is set, times ``scale``.  ``bias`` (fp32 ``[E]``) is added to the scores for the choice only: it changes
     neither weights nor gradients.  Ties go to the lowest expert.  An expert whose logit (or score + bias) is -inf or NaN is
     never chosen; a place that is left over gets expert -1, which dispatch and combine skip, and weight 0.  ``valid`` (bool ``[T]``): tokens where it is False
-    get -1 and 0 everywhere and a gradient of 0.  A NaN or +inf among a token's logits makes all its softmax weights NaN."""
+    get -1 and 0 everywhere and a gradient of 0.  A NaN or +inf among a token's logits makes the softmax weights of all its chosen experts NaN; the choice
+    (with a bias: by the softmax over the logits that are numbers, which those of +inf share evenly) is made all the same."""
     _check(logits, topk, score, valid)
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (logits.shape[1],)):
         raise RoutingError(f"bias must be float32 of shape {(logits.shape[1],)}")

@@ -305,3 +305,49 @@ def test_where_the_largest_lie(E, K, dt):
     logits = torch.stack(rows).to(dt).cuda()
     for bias in (None, torch.zeros(E, device="cuda")):   # a bias orders by the sigmoids, where logits from 37 on are equal
         _check_route(logits, K, score="sigmoid", bias=bias)
+
+
+def _bad_rows(E, spread):
+    """Rows with a NaN or +inf among logits that lie `spread` apart, in shuffled order, and a last row without."""
+    g = torch.Generator().manual_seed(E)
+    l = torch.stack([torch.randperm(E, generator=g) * spread for _ in range(6)]).float()
+    l[0, 3], l[1, E - 1], l[1, 0] = float("nan"), float("nan"), float("nan")
+    l[2, 5] = math.inf
+    l[3, 7], l[3, 2], l[3, 4] = math.inf, math.inf, float("nan")
+    l[4, 6], l[4, ::2] = float("nan"), -math.inf
+    return l
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread", [1e-7, 1e-5, 1e-2, 0.5])   # in 64 bits throughout, in 32 bits throughout, and between
+@pytest.mark.parametrize("E,K", [(20, 3), (40, 16), (300, 8), (1000, 16)])
+@pytest.mark.parametrize("bias", [0.0, 1e-6, 0.1])
+def test_biased_choice_beside_bad_logits(E, K, spread, bias):
+    """Softmax + bias orders the logits that are numbers, whatever decides between them: NaN are left out, +inf share the softmax."""
+    from nvshmem_b200.ops import routing
+    l = _bad_rows(E, spread)
+    b = torch.randn(E, generator=torch.Generator().manual_seed(1)) * bias
+    d = l.double()
+    top = torch.where(d.isnan(), -math.inf, d).amax(-1, keepdim=True)
+    e = torch.where(d == top, 1.0, torch.exp(d - top))
+    p = torch.where(d.isnan(), 0.0, e)
+    p = p / p.sum(-1, keepdim=True)
+    order = torch.where(d.isnan() | (d == -math.inf), -math.inf, p + b.double())
+    bad = (d.isnan() | (d == math.inf)).any(-1)   # not the last two: the NaN of the fifth row is among those it then sets to -inf
+    for renormalize in (True, False):
+        idx, w = routing.moe_route(l.cuda(), K, bias=b.cuda(), renormalize=renormalize)
+        want = _choice(order, K)
+        assert torch.equal(idx.cpu().long(), want)
+        w = w.cpu()
+        assert w[bad][want[bad] >= 0].isnan().all() and not w[want < 0].any() and w[~bad].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_places_left_over_beside_bad_logits():
+    from nvshmem_b200.ops import routing
+    l = torch.full((2, 40), -math.inf, device="cuda")
+    l[0, 3], l[0, 9], l[1, 2], l[1, 4] = 1.0, float("nan"), math.inf, 0.0
+    for renormalize in (True, False):
+        idx, w = routing.moe_route(l, 4, renormalize=renormalize)
+        assert idx.tolist() == [[3, -1, -1, -1], [2, 4, -1, -1]]
+        assert w[0, 0].isnan() and w[1, :2].isnan().all() and not w[idx < 0].any()
