@@ -250,9 +250,13 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
     for (int i = 0; i < VPL; ++i) key[i] = key32(l[i]);
     choose(K);
   } else {
-    // Score + bias in 32 bits with the fast exponential and division first.  They and the sum of up to 37 terms are off by less than 4e-6
-    // of a score, which is at most 1, and the sum with the bias by half a step.  Where two neighbours in the order are closer than twice
-    // that (two tokens in a hundred), the choice is made in 64 bits.  8192 x 256, top-8: 12.5 us, 7.1 without a bias.  (All in 64 bits took 20 us where this took 16.6.)
+    // Score + bias in 32 bits with the fast exponential and division first.  An exponential of -x is off by (2 + 1.2 x) ulp and x half steps, the sum of
+    // up to 37 terms by as many half steps: together less than 5e-6 of a score down to 2^-10 of the largest, and less than that share of 2^-10 of
+    // it below; the sum with the bias is off by half a step.  No expert at or below a value v of score + bias has a score above v less the
+    // smallest bias, so that bounds what all of them are off by.  Where two neighbours in the order are closer than twice that for the upper one,
+    // the choice is made in 64 bits.  256 experts, top-8: 0.04 tokens in a hundred for a softmax of logits of deviation 1.5, 1 and 4 for 0.1 and
+    // 0.02, 6 for 10, 1 for sigmoids; sigmoids that round to 1 side by side need it always.  (A bound of 1e-5 for all sent 2, 83, 100 and 46.)
+    // 8192 x 256, top-8, us: 13.1, 14.5, 16.0 and 20.2 for these four, 13.0 for sigmoids, 7.5 to 8.1 without a bias.
     float s[VPL], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -266,16 +270,25 @@ __global__ void __launch_bounds__(THREADS) route_kernel(const __grid_constant__ 
       for (int i = 0; i < VPL; ++i) sum += s[i] = l[i] == top ? 1.f : 0.f;
     }
     const float inv = a.score == BSHMEM_ROUTE_SOFTMAX ? 1.f / warp_sum(sum) : 1.f;
+    // the largest score; a sigmoid below 2^-10, whose exponential is of a larger x, counts as that
+    const float most = a.score == BSHMEM_ROUTE_SOFTMAX ? inv : fmaxf(__fdividef(1.f, 1.f + __expf(-top)), 0x1p-10f);
+    float least_bias = CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = lane + 32 * i;
-      key[i] = e < E && l[i] > -CUDART_INF_F ? key32(s[i] * inv + a.bias[e]) : 0u;
+      key[i] = 0u;
+      if (e < E && l[i] > -CUDART_INF_F) {
+        const float b = a.bias[e];
+        key[i] = key32(s[i] * inv + b);
+        least_bias = fminf(least_bias, b);
+      }
     }
+    least_bias = -value32(__reduce_max_sync(0xffffffffu, key32(-least_bias)));
     const int rounds = K + 2;
     choose(rounds);
     const uint32_t next = __shfl_down_sync(0xffffffffu, mine_key, 1);
-    const float v = value32(mine_key);
-    const unsigned unclear = __ballot_sync(0xffffffffu, lane <= K && mine_key && next && !(v - value32(next) > 1e-5f + 5e-7f * fabsf(v)));
+    const float v = value32(mine_key), score = fminf(most, fmaxf(v - least_bias, most * 0x1p-10f));
+    const unsigned unclear = __ballot_sync(0xffffffffu, lane <= K && mine_key && next && !(v - value32(next) > 1e-5f * score + 5e-7f * fabsf(v)));
     if ((unclear >> (K - 1) & 3) == 3) mine = select64<T, VPL>(a, row, top, lane);  // what was not picked may belong to the K, too
     else if (unclear & ((1u << K) - 1)) mine = order64(a, row, top, lane, mine, rounds);
     if (lane >= K) mine = -1;
