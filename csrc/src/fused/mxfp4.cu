@@ -40,7 +40,9 @@ __device__ __forceinline__ RowSlot row_slot() {
   const int warp = threadIdx.x >> 5, in32 = (blockIdx.x & 15) * 2 + (warp & 1), quarter = warp >> 1;
   return {(int64_t)(blockIdx.x >> 4) * 128 + quarter * 32 + in32, in32 * 16 + quarter * 4};
 }
-static dim3 row_grid(int64_t R, int64_t K, int chunk) { return dim3((unsigned)(row_blocks(R) * 16), (unsigned)((k_blocks(K) * 128 + chunk - 1) / chunk)); }
+constexpr int MAX_GRID_Y = 65535;
+static int64_t chunks_of(int64_t K, int chunk) { return (k_blocks(K) * 128 + chunk - 1) / chunk; }
+static dim3 row_grid(int64_t R, int64_t chunks) { return dim3((unsigned)(row_blocks(R) * 16), (unsigned)chunks); }
 
 // A lane takes a block of 32 values, so that their largest exponent needs no exchange (8192 x 8192 bf16 34.0 -> 29.9 us against eight values a
 // lane), and four lanes' scales go out as a word.  A scale is a power of two, so x / scale is exact and the only rounding is the one to E2M1.
@@ -73,12 +75,12 @@ __host__ __device__ constexpr int quantize_chunk() { return sizeof(T) == 4 ? 102
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict__ x, int64_t R, int K, int64_t stride, uint8_t* __restrict__ data,
-                                                             uint8_t* __restrict__ scales) {
+                                                             uint8_t* __restrict__ scales, int first_chunk) {
   constexpr int UNROLL = quantize_chunk<T>() / 1024, WORDS = sizeof(T) * 32 / 16;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product may set up, and fetch its weights, beside this kernel
   const RowSlot slot = row_slot();
   const int lane = threadIdx.x & 31;
-  const int KB = (int)k_blocks(K), base = (int)blockIdx.y * quantize_chunk<T>() + lane * 32;
+  const int KB = (int)k_blocks(K), base = (first_chunk + (int)blockIdx.y) * quantize_chunk<T>() + lane * 32;
   const bool row_live = slot.row < R;
   const T* src = x + slot.row * stride;
   uint8_t* dst = data + slot.row * (K / 2);
@@ -128,6 +130,7 @@ __global__ void __launch_bounds__(Q_THREADS) quantize_kernel(const T* __restrict
   }
 }
 
+static_assert((1 << 26) / Q_CHUNK <= MAX_GRID_Y, "the longest row in one launch");
 // The reverse; a lane's values fill one 16-byte store: four fp32 or eight 16-bit ones.
 template <typename T>
 __global__ void __launch_bounds__(Q_THREADS) dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, int64_t R, int K, T* __restrict__ out) {
@@ -177,13 +180,20 @@ static int launched(const char* what, cudaError_t e) {
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int64_t K, int64_t stride, void* data, void* scales, cudaStream_t stream) {
   const bool vec = ((uintptr_t)x & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
-  return launched("bshmem_mxfp4_quantize", launch_kernel(vec ? quantize_kernel<T, true> : quantize_kernel<T, false>, row_grid(R, K, quantize_chunk<T>()), Q_THREADS, stream,
-                                                         (const T*)x, R, (int)K, stride, (uint8_t*)data, (uint8_t*)scales));
+  // The longest rows of fp32 have one chunk more than a grid's second dimension takes.
+  const int64_t chunks = chunks_of(K, quantize_chunk<T>());
+  for (int64_t first = 0; first < chunks; first += MAX_GRID_Y) {
+    const int64_t n = chunks - first < MAX_GRID_Y ? chunks - first : MAX_GRID_Y;
+    const int st = launched("bshmem_mxfp4_quantize", launch_kernel(vec ? quantize_kernel<T, true> : quantize_kernel<T, false>, row_grid(R, n), Q_THREADS, stream, (const T*)x, R,
+                                                                   (int)K, stride, (uint8_t*)data, (uint8_t*)scales, (int)first));
+    if (st) return st;
+  }
+  return BSHMEM_MX_OK;
 }
 template <typename T>
 static int launch_dequantize(const void* data, const void* scales, int64_t R, int64_t K, void* out, cudaStream_t stream) {
   return launched("bshmem_mxfp4_dequantize",
-                  launch_kernel(dequantize_kernel<T>, row_grid(R, K, Q_CHUNK), Q_THREADS, stream, (const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out));
+                  launch_kernel(dequantize_kernel<T>, row_grid(R, chunks_of(K, Q_CHUNK)), Q_THREADS, stream, (const uint8_t*)data, (const uint8_t*)scales, R, (int)K, (T*)out));
 }
 
 // Tensor map of scales: rows are row blocks, elements words; a box is 1 KB (256 values of K) of `blocks` row blocks.

@@ -247,3 +247,23 @@ def test_limits_of_the_entry_points():
         assert lib.bshmem_mxfp4_gemm(ctypes.byref(a), None) == 2
     assert lib.bshmem_mxfp4_quantize(None, 0, 1, (1 << 26) - 32, 0, None, None, None) == 1   # the size would do
     assert lib.bshmem_mxfp4_quantize(None, 0, 0, 32, 32, None, None, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_the_longest_rows(dt):
+    """K up to the limit: a row gives the bytes of the same blocks laid out as shorter rows."""
+    from nvshmem_b200.ops import mxfp4
+    for K, rows in (((1 << 26) - 32, 337), ((1 << 26) - 1024, 340), (65535 * 1024 + 32, 169)):   # divisors of K / 32
+        assert K % (rows * 32) == 0
+        x = torch.randn(1, K, device="cuda", generator=torch.Generator("cuda").manual_seed(rows)).to(dt)
+        q, short = mxfp4.quantize_mxfp4(x), mxfp4.quantize_mxfp4(x.view(rows, K // rows))
+        assert torch.equal(q.data.view(-1), short.data.view(-1)) and torch.equal(q.codes.view(-1), short.codes.view(-1))
+        assert not q.scales.view(-1, 32, 4, 4)[:, 1:].any() and not q.scales.view(-1, 32, 4, 4)[:, :, 1:].any()   # rows past the end
+        assert torch.equal(q.dequantize().view(-1), short.dequantize().view(-1))
+        # a product that picks values of both ends: exact
+        pick = torch.zeros(2, K, device="cuda", dtype=dt)
+        pick[0, 5], pick[1, K - 3] = 1.0, 2.0
+        got = mxfp4.gemm_mxfp4(pick, q)
+        values = q.dequantize(torch.float32)
+        assert torch.equal(got.float(), torch.stack([values[:, 5], 2 * values[:, K - 3]]).to(torch.bfloat16).float())
