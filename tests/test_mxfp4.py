@@ -267,3 +267,23 @@ def test_the_longest_rows(dt):
         got = mxfp4.gemm_mxfp4(pick, q)
         values = q.dequantize(torch.float32)
         assert torch.equal(got.float(), torch.stack([values[:, 5], 2 * values[:, K - 3]]).to(torch.bfloat16).float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(1, 256, 8192), (16, 1000, 8192), (33, 520, 4096), (64, 8192, 8192), (130, 260, 12288), (300, 512, 8192), (512, 4096, 7168), (777, 1040, 5024),
+                                   (1024, 4096, 4096), (2048, 2047, 8192)])
+def test_long_sums_are_exact_where_fp32_is(M, N, K):
+    """Elements of the grid with one scale per row: every product is a multiple of 1/4 of the rows' scales and every sum of them below 36 K / 4 <= 2^21
+    multiples, so that fp32 holds all of them and the result is the exact sum, rounded once."""
+    from nvshmem_b200.ops import mxfp4
+    g = torch.Generator(device="cuda").manual_seed(M)
+
+    def operand(R):
+        v = GRID.to("cuda")[torch.randint(0, 8, (R, K), generator=g, device="cuda")] * (torch.randint(0, 2, (R, K), generator=g, device="cuda") * 2 - 1)
+        v[:, ::32] = 6.0   # every block has the same scale before the row's own
+        return v.float() * torch.exp2(torch.randint(-3, 4, (R, 1), generator=g, device="cuda").float())
+
+    x, w = operand(M), operand(N)
+    xq, wq = mxfp4.quantize_mxfp4(x), mxfp4.quantize_mxfp4(w)
+    assert torch.equal(xq.dequantize(torch.float32), x) and torch.equal(wq.dequantize(torch.float32), w)
+    assert torch.equal(mxfp4.gemm_mxfp4(xq, wq), (x.double() @ w.double().t()).to(torch.bfloat16))
