@@ -24,14 +24,15 @@ from ..ops.routing import moe_route
 class ExpertParallelMoE(torch.nn.Module):
     """``router``: "torch" (softmax and topk of torch; ties in torch's order) or "fused" (:func:`~nvshmem_b200.ops.routing.moe_route`: ties
     go to the lowest expert).  The fused router also takes sigmoid scores (``score``) and a bias per expert for the choice
-    (:attr:`router_bias`, fp32 ``[experts]``, None at first)."""
+    (:attr:`router_bias`, fp32 ``[experts]``, None at first; a buffer that is saved, loaded and moved with the block and stays fp32)."""
 
     def __init__(self, tokens: int, hidden: int, ffn: int, experts: int, topk: int, payload: str = "bf16", seed: int = 0, wait_limit_ms: int = 0,
                  router: str = "torch", score: str = "softmax"):
         super().__init__()
         if router not in ("torch", "fused") or (router == "torch" and score != "softmax"):
             raise ValueError("router is 'torch' (softmax scores) or 'fused'")
-        self.fused_router, self.score, self.router_bias = router == "fused", score, None
+        self.fused_router, self.score = router == "fused", score
+        self.register_buffer("router_bias", None)
         from .. import core
         self.rank, self.npes = core.my_pe(), core.n_pes()
         self.T, self.H, self.F, self.E, self.K = tokens, hidden, ffn, experts, topk
@@ -51,6 +52,19 @@ class ExpertParallelMoE(torch.nn.Module):
         if self.grouped:
             self.w_in_gated = fg.interleave_gate_up(self.w_in.data)   # rows reordered for the fused gated activation
             self.act_buf = torch.empty(self.exchange.cap_rows, ffn, dtype=torch.bfloat16, device=dev)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        saved = state_dict.get(prefix + "router_bias")
+        if saved is not None and self.router_bias is None:   # a block without a bias takes the saved one
+            self.router_bias = torch.zeros(self.E, dtype=torch.float32, device=self.router.device)
+        super()._load_from_state_dict(state_dict, prefix, *args)
+
+    def _apply(self, fn, *args, **kwargs):
+        bias = self.router_bias
+        super()._apply(fn, *args, **kwargs)
+        if bias is not None and self.router_bias.dtype != torch.float32:   # the choice is made in fp32 or more, whatever the block's type
+            self.router_bias = bias.to(self.router_bias.device)
+        return self
 
     @staticmethod
     def fp8_payload(payload: str) -> bool:

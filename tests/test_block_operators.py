@@ -302,3 +302,32 @@ def test_a_launch_that_fails_is_not_blamed_on_the_next_call(call):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", f"CALL = {call!r}\n" + FAILED], cwd=root, capture_output=True, text=True, timeout=600)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_the_routers_bias_is_part_of_the_block(nv):
+    """It is saved and loaded with the block, moves with it and stays in 32 bits."""
+    from nvshmem_b200.models import ExpertParallelMoE
+    T, H, F, E, K = 128, 256, 128, 8, 2
+    make = lambda: ExpertParallelMoE(T, H, F, E, K, seed=3, router="fused", score="sigmoid")
+    block = make()
+    assert block.router_bias is None and "router_bias" not in block.state_dict()
+    plain = {k: v.clone() for k, v in block.state_dict().items()}
+    bias = torch.randn(E, device="cuda")
+    block.router_bias = bias.clone()
+    state = {k: v.clone() for k, v in block.state_dict().items()}
+    assert torch.equal(state["router_bias"], bias)
+    other = make()
+    other.load_state_dict(state)
+    x = torch.randn(T, H, device="cuda").to(BF16)
+    assert torch.equal(other.router_bias, bias) and other.router_bias.is_cuda and torch.equal(other.route(x)[0], block.route(x)[0])
+    other.to(BF16)
+    assert other.router_bias.dtype == F32 and torch.equal(other.router_bias, bias)
+    other.load_state_dict({**state, "router_bias": (bias + 1).cpu()})
+    assert torch.equal(other.router_bias, bias + 1) and other.router_bias.is_cuda
+    with pytest.raises(RuntimeError):       # a block with a bias, a checkpoint without
+        other.load_state_dict(plain)
+    fresh = make()
+    fresh.load_state_dict(plain)
+    assert fresh.router_bias is None
+    for b in (block, other, fresh):
+        b.close()
