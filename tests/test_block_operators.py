@@ -331,3 +331,34 @@ def test_the_routers_bias_is_part_of_the_block(nv):
     assert fresh.router_bias is None
     for b in (block, other, fresh):
         b.close()
+
+
+def test_sigmoid_scores_and_a_bias_in_the_moe_block(nv):
+    """The block's weights are the chosen experts' sigmoids over their sum, whatever bias chose them, and its output is that of the plain form:
+    three roundings to bf16 on the way (activation, experts' output, result), 2^-8 each of the largest value."""
+    from nvshmem_b200.models import ExpertParallelMoE
+    from nvshmem_b200.ops import fused_gemm as fg
+    T, H, F, E, K = 192, 256, 384, 8, 2
+    block = ExpertParallelMoE(T, H, F, E, K, seed=3, router="fused", score="sigmoid")
+    torch.manual_seed(18)
+    x = torch.randn(T, H, device="cuda").to(BF16)
+    s = torch.sigmoid((x @ block.router.t()).double())
+    for bias in (None, torch.linspace(-0.4, 0.4, E, device="cuda")):
+        block.router_bias = bias
+        idx, weight = block.route(x)
+        order = s if bias is None else s + bias.double()
+        top = order.sort(dim=-1, descending=True, stable=True)
+        assert torch.equal(idx.long(), top.indices[:, :K])
+        want = s.gather(-1, idx.long())
+        want = want / want.sum(-1, keepdim=True)
+        assert ((weight.double() - want).abs() <= 2.0 ** -18 * want).all()
+        out = torch.zeros(T, H, device="cuda")
+        for e in range(E):
+            tok, slot = (idx == e).nonzero(as_tuple=True)
+            a = x[tok].float() @ block.w_in[e].float().t()
+            a = torch.nn.functional.silu(a[:, :F]) * a[:, F:]
+            out.index_add_(0, tok, (a @ block.w_out[e].float().t()) * weight[tok, slot].unsqueeze(-1))
+        assert (block(x).float() - out).abs().max() <= 3 * 2.0 ** -8 * out.abs().max()
+    torch.cuda.synchronize()
+    fg.check_errors()
+    block.close()
