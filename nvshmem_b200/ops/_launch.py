@@ -24,6 +24,11 @@ def stream_of(device: int) -> int:
     return _current_stream(device)
 
 
+def wants_gradient(t: torch.Tensor) -> bool:
+    """Whether a derivative with respect to `t` is being asked for."""
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 def first_order(backward):
     """`backward` of an autograd function whose kernels record no graph.  A graph of the gradients (create_graph) may be asked for; going
     through it raises, as with ``once_differentiable``, whose wrapper takes 5 us a call and is entered only then."""

@@ -5,7 +5,8 @@
 * :func:`gemm_mxfp4` – ``x @ w.T`` of two such matrices on the tensor cores' block-scaled form, accumulated in fp32; a bf16,
   fp16 or fp32 ``x`` is quantised in the call.
 
-For serving: weights are quantised once, activations in every call, and nothing here records gradients.  K is a multiple of 32; rows and columns of the product may be
+For serving: weights are quantised once, activations in every call, and nothing here records gradients: a tensor that requires one is refused unless the
+call is under ``torch.no_grad()`` (or ``inference_mode``).  K is a multiple of 32; rows and columns of the product may be
 any number.  Work is issued on the current stream; all tensors lie on the current device.
 """
 from __future__ import annotations
@@ -14,7 +15,7 @@ import ctypes as C
 
 import torch
 
-from ._launch import device_of, stream_of
+from ._launch import device_of, stream_of, wants_gradient
 from .fused_gemm import _check_out, _error_flag, fused_lib, FusedGemmError
 
 BLOCK = 32
@@ -114,10 +115,16 @@ def quantize_mxfp4(x: torch.Tensor) -> MxFp4:
     return q
 
 
+def _no_gradient(name: str, t: torch.Tensor | None) -> None:
+    if t is not None and wants_gradient(t):
+        raise FusedGemmError(f"{name} requires a gradient, which 4-bit floats do not have: detach it or call under torch.no_grad()")
+
+
 def _checked(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """`x` as a matrix that can be quantised, and its device."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _TYPES:
         raise FusedGemmError("x must be a [R, K] tensor of bfloat16, float16 or float32")
+    _no_gradient("x", x)
     K = x.shape[1]
     if K < BLOCK or K % BLOCK:
         raise FusedGemmError(f"K must be a multiple of {BLOCK}, not {K}")
@@ -151,6 +158,7 @@ def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = Non
     if out is None:
         out = w.data.new_empty((M, N), dtype=torch.bfloat16)
     else:
+        _no_gradient("out", out)
         _check_out(out, M, N)
     a = _GemmArgs(*operand, w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), M, N, K, 0, _error_flag(dev).data_ptr(), *source)
     _raise(_lib().bshmem_mxfp4_gemm(C.byref(a), stream_of(device)), "bshmem_mxfp4_gemm")

@@ -362,3 +362,20 @@ def test_sigmoid_scores_and_a_bias_in_the_moe_block(nv):
     torch.cuda.synchronize()
     fg.check_errors()
     block.close()
+
+
+def test_gradients_that_would_be_lost_are_refused():
+    """The 4-bit floats record no gradients, and say so where one is asked for."""
+    from nvshmem_b200.ops import gemm_mxfp4, quantize_mxfp4
+    from nvshmem_b200.ops.fused_gemm import FusedGemmError
+    x = torch.randn(5, 64, device="cuda", requires_grad=True)
+    with torch.no_grad():
+        q = quantize_mxfp4(x)
+        want = gemm_mxfp4(x, q)
+    for call in (lambda: quantize_mxfp4(x), lambda: quantize_mxfp4(x * 2), lambda: gemm_mxfp4(x, q), lambda: gemm_mxfp4(x * 2, q)):
+        with pytest.raises(FusedGemmError, match="no_grad"):
+            call()
+    out = torch.zeros(5, 5, device="cuda", dtype=BF16, requires_grad=True)
+    with pytest.raises(FusedGemmError, match="no_grad"):
+        gemm_mxfp4(x.detach(), q, out=out)
+    assert torch.equal(gemm_mxfp4(x.detach(), quantize_mxfp4(x.detach())), want)
