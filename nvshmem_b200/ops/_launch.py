@@ -4,6 +4,7 @@ The calls take a few microseconds on the GPU, so the host's share counts: each h
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -24,9 +25,14 @@ def stream_of(device: int) -> int:
     return _current_stream(device)
 
 
+def forward_mode() -> bool:
+    """Whether tangents may be about (``torch.autograd.forward_ad``): a call then goes by its autograd function, which refuses them."""
+    return _forward_ad._current_level >= 0
+
+
 def wants_gradient(t: torch.Tensor) -> bool:
-    """Whether a derivative with respect to `t` is being asked for."""
-    return t.requires_grad and torch.is_grad_enabled()
+    """Whether a derivative with respect to `t` is being asked for, in reverse or forward mode."""
+    return (t.requires_grad and torch.is_grad_enabled()) or (forward_mode() and _forward_ad.unpack_dual(t).tangent is not None)
 
 
 def first_order(backward):

@@ -17,7 +17,7 @@ import ctypes as C
 
 import torch
 
-from ._launch import device_of, first_order, stream_of
+from ._launch import device_of, first_order, forward_mode, stream_of
 from .fused_gemm import _error_flag, fused_lib
 
 MAX_H = 16384
@@ -168,7 +168,7 @@ def _run(plan: _Plan, want_r: bool, h, residual, post, pre, gate):
         pre = pre.contiguous()
     if gate is not None:
         gate = _rows(gate) if plan.gate_mode == _FULL else gate.contiguous()
-    if torch.is_grad_enabled() and (residual.requires_grad or any([t is not None and t.requires_grad for t in tensors])):
+    if (torch.is_grad_enabled() and (residual.requires_grad or any([t is not None and t.requires_grad for t in tensors]))) or forward_mode():
         out = _BlockNorms.apply(plan, want_r, h, residual, post, pre, gate)
         if want_r and pre is not None:
             return out

@@ -15,7 +15,7 @@ import ctypes as C
 
 import torch
 
-from ._launch import device_of, first_order, stream_of
+from ._launch import device_of, first_order, forward_mode, stream_of
 from .fused_gemm import fused_lib
 
 MAX_EXPERTS, MAX_TOPK = 1024, 16
@@ -154,7 +154,7 @@ def moe_route(logits: torch.Tensor, topk: int, score: str = "softmax", bias: tor
     logits = _rows(logits)
     bias = None if bias is None else bias.detach().contiguous()
     valid = None if valid is None else valid.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if (torch.is_grad_enabled() and logits.requires_grad) or forward_mode():
         return _Route.apply(logits, topk, SCORES[score], bias, int(renormalize), float(scale), valid)
     return _route(logits, topk, SCORES[score], bias, int(renormalize), float(scale), valid)
 
@@ -176,6 +176,6 @@ def balance_loss(logits: torch.Tensor, idx: torch.Tensor, score: str = "softmax"
     device_of(RoutingError, logits, idx, valid)
     logits, idx = _rows(logits), idx.contiguous()
     valid = None if valid is None else valid.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if (torch.is_grad_enabled() and logits.requires_grad) or forward_mode():
         return _Balance.apply(logits, idx, SCORES[score], valid)
     return _balance(logits, idx, SCORES[score], valid)[:2]

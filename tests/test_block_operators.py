@@ -379,3 +379,21 @@ def test_gradients_that_would_be_lost_are_refused():
     with pytest.raises(FusedGemmError, match="no_grad"):
         gemm_mxfp4(x.detach(), q, out=out)
     assert torch.equal(gemm_mxfp4(x.detach(), quantize_mxfp4(x.detach())), want)
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives are not computed: a call with a tangent on an input raises, with and without a gradient asked for."""
+    import torch.autograd.forward_ad as fwd
+    from nvshmem_b200.ops import balance_loss, block_norms, gemm_mxfp4, moe_route, quantize_mxfp4, rms_norm
+    x, w = torch.randn(6, 64, device="cuda"), torch.ones(64, device="cuda")
+    idx, q = moe_route(x, 2)[0], quantize_mxfp4(x)
+    calls = [lambda t: rms_norm(t, w), lambda t: rms_norm(x, t[0]), lambda t: block_norms(t, x, w)[0], lambda t: block_norms(x, t)[0], lambda t: block_norms(x, x, gate=t)[0],
+             lambda t: moe_route(t, 2)[1], lambda t: balance_loss(t, idx)[0], lambda t: quantize_mxfp4(t), lambda t: gemm_mxfp4(t, q)]
+    with fwd.dual_level():
+        for call in calls:
+            call(x)      # no tangent: as outside
+            dual = fwd.make_dual(x, torch.ones_like(x))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call(dual)
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                call(dual)
