@@ -397,3 +397,62 @@ def test_tangents_are_refused():
                 call(dual)
             with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
                 call(dual)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values a tensor: the last rows give what they give alone (the sums over rows aside)."""
+    from nvshmem_b200.ops import balance_loss, block_norms, fused_gemm, gemm_mxfp4, moe_route, quantize_mxfp4, rms_norm
+    T, H, tail = 263000, 8192, 200
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(T, H, device="cuda", generator=g, dtype=BF16)
+    w, gate = (torch.rand(H, device="cuda", generator=g) + 0.5).to(BF16), torch.rand(T, 1, device="cuda", generator=g).to(BF16)
+    assert x.numel() > 2 ** 31
+
+    def norms(x, gate):
+        x = x.detach().requires_grad_(True)
+        y = rms_norm(x, w)
+        (dy,) = torch.autograd.grad(y, x, x.detach())
+        r, z = block_norms(x, x, w, w, gate)
+        (dr,) = torch.autograd.grad([r, z], x, [x.detach(), x.detach()])
+        return y.detach(), dy, r.detach(), z.detach(), dr
+
+    whole = [t[-tail:].clone() for t in norms(x, gate)]
+    alone = norms(x[-tail:], gate[-tail:])
+    for a, b in zip(whole, alone):   # other kernels take few rows: the same sums in another order, so a rounding may fall the other way
+        assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 2.0 ** -14 * b.float().abs().max()).all()
+    torch.cuda.empty_cache()
+    q, wq = quantize_mxfp4(x), quantize_mxfp4(torch.randn(H, H, device="cuda", generator=g))
+    tq = quantize_mxfp4(x[-tail:])
+    assert torch.equal(q.data[-tail:], tq.data) and torch.equal(q.codes[-tail:], tq.codes)
+    assert torch.equal(q.dequantize()[-tail:], tq.dequantize())
+    out = gemm_mxfp4(x, wq)     # 2^31 values come out as well
+    want = tq.dequantize(F32).double() @ wq.dequantize(F32).double().t()
+    mag = tq.dequantize(F32).double().abs() @ wq.dequantize(F32).double().abs().t()
+    assert ((out[-tail:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * mag).all()
+    assert torch.equal(out[:tail], gemm_mxfp4(x[:2 * 8192], wq)[:tail])
+    del out, q, whole, alone
+    torch.cuda.empty_cache()
+    logits = x.view(-1, 256)[:8400000]
+    assert logits.numel() > 2 ** 31
+
+    def route(l):
+        l = l.detach().requires_grad_(True)
+        idx, weight = moe_route(l, 8, renormalize=False)
+        (dl,) = torch.autograd.grad(weight, l, torch.ones_like(weight) * torch.arange(8, device="cuda"))
+        return idx, weight.detach(), dl
+
+    whole, alone = route(logits), route(logits[-tail:])
+    for a, b in zip(whole, alone):
+        assert torch.equal(a[-tail:], b)
+    idx = whole[0]
+    del whole
+    l = logits.detach().requires_grad_(True)
+    loss, counts = balance_loss(l, idx)
+    assert torch.equal(counts.long(), torch.bincount(idx.view(-1), minlength=256))
+    (dl,) = torch.autograd.grad(loss, l)
+    p = torch.softmax(l.detach()[-tail:].double(), -1)
+    c = counts.double() * 256 / (8 * float(len(idx)) ** 2)
+    want = p * (c - (p * c).sum(-1, keepdim=True))
+    assert ((dl[-tail:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * p * c.max()).all()
+    torch.cuda.synchronize()
+    fused_gemm.check_errors()
