@@ -758,10 +758,10 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
   int per_sm = ctas_per_sm(r.kind) * ROW_THREADS / r.block;
   if (per_sm > MAX_CTAS_PER_SM) per_sm = MAX_CTAS_PER_SM;
   if (vec && a->H > WARP_COLS && a->T > sms * per_sm / pair) {
-    // Two stages at least; rather fewer CTAs of an SM than none.  Forward three at most where h is read too: more rows on their way favour some
-    // SMs over others, and the rows are dealt out beforehand (4096 x 8192 bf16 48.5 us with six, 46.5 with three; 8192 x 4096 48.4 and 45.2;
-    // fp32 residual 70 and 68).  A norm alone has half the bytes a row: 24.3 with six, 25.4 with three.
-    const int most_stages = backward || r.kind == IN ? MAX_STAGES : 3;
+    // Two stages at least; rather fewer CTAs of an SM than none.  Forward three at most: more rows on their way favour some SMs over others, and the
+    // rows are dealt out beforehand (4096 x 8192 bf16 48.5 us with six, 46.5 with three; 8192 x 4096 48.4 and 45.2; fp32 residual 70 and 68; a
+    // norm alone, bf16, 4096 x 8192 25.0 and 24.1, 4096 x 5120 19.2 and 16.4, 8192 x 2048 15.8 and 13.5, fp32 4096 x 8192 49.1 both).
+    const int most_stages = backward ? MAX_STAGES : 3;
     r.stage_bytes = stage_rows(*a, cols, backward, r.kind).bytes;
     for (int n = per_sm; n > 0; --n) {
       const int fit = (STAGE_SMEM / n - 2048) / r.stage_bytes;
@@ -770,7 +770,8 @@ static inline RowPlan row_plan(const bshmem_norm_args_t* a, bool backward) {
       r.stages = fit < most_stages ? fit : most_stages;
       r.smem = r.stages * r.stage_bytes + MAX_STAGES * 16 + 16;
       // With two stages the copies would have half a row's time only (backward, fp32 residual, 4096 x 8192: 116 us, 101 early).  With three, or
-      // more CTAs, it costs instructions and gains nothing (bf16 74 us, 76 early; pairs 98 and 109), but for the short rows of a norm alone (49, 46).
+      // more CTAs, it costs instructions and gains nothing (bf16 74 us, 76 early; pairs 98 and 109), but for the short rows of a norm alone (4096 x 8192
+      // bf16 47.0 us, 45.1 early; 8192 x 4096 48.1 and 46.4; 16384 x 2048 48.6 both).
       if (backward && (r.kind == IN || (r.kind != OUT && r.stages == 2 && n == 1))) r.mode = EARLY;
       per_sm = n;
       break;
