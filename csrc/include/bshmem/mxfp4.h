@@ -40,7 +40,7 @@ typedef struct {
   int64_t raw_stride;
 } bshmem_mxfp4_gemm_args_t;
 
-/* data pointers 16-byte aligned. */
+/* data pointers 16-byte aligned.  The sum over K is divided by a rule on M, N and K: a row's last bits may differ with the number of rows. */
 int bshmem_mxfp4_gemm(const bshmem_mxfp4_gemm_args_t* args, cudaStream_t stream);
 
 #ifdef __cplusplus

@@ -243,10 +243,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) gemm_pair_kernel(const __grid_co
 
 // ------------------------------------------------------------------ few rows of x
 // One tile of 128 rows of w by COLS rows of x per CTA, in steps of 256 values of K: the weights are the tensor core's first operand.  Here
-// reading the weights is what takes the time: an SM takes in some 60 bytes a clock, so all SMs have to read, and a cluster of CTAs
+// reading the weights is what takes the time beside a fixed part, so as many SMs as possible have to read, and a cluster of CTAs
 // divides K.  Each sends its sums to the shared memory of the CTA that owns the row of x (its number modulo the cluster's size), which
 // adds them in order.  (Owners that fetch the sums instead wait for a round trip per value: 64 x 1024 x 8192 took 19 us that way, 7.5 now.)
-// 16 x 8192 x 8192: 11.7 us with cold weights (36 MB), 8.9 with warm ones, of which 5.4 are what the smallest product takes.
+// 16 x 8192 x 8192: 11.7 us with cold weights, 8.9 to 9.2 with warm ones, of which 5.3 are what the smallest product takes (launch, tensor memory, the
+// first loads, the exchange, the stores): the other 6.4 read 36 MB at 5.6 TB/s, from L2 3.7 at 9.7.
 //   warp 0  TMA producer   warp 1  MMA issuer   warp 2  tensor memory   then all eight warps store
 constexpr int F_THREADS = 256, F_STAGE_W = 128 * 128;
 template <int COLS>

@@ -88,7 +88,8 @@ class MxFp4:
         return self.scales.view(rb, kb, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(rb * 128, kb * 4)[:R, :K // BLOCK].contiguous()
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values, ``[R, K]``.  Exact in bf16 and fp32; fp16 rounds where its range ends."""
+        """The values, ``[R, K]``.  Exact in bf16 and fp32 (of scales from 2 ** 126 on, which quantisation does not make, the largest
+        elements are infinite); fp16 rounds where its range ends."""
         if dtype not in _TYPES:
             raise FusedGemmError("dtype must be bfloat16, float16 or float32")
         device = device_of(FusedGemmError, self.data, self.scales)
@@ -134,7 +135,8 @@ def _checked(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 def gemm_mxfp4(x: torch.Tensor | MxFp4, w: MxFp4, out: torch.Tensor | None = None) -> torch.Tensor:
     """``x[M, K] @ w[N, K].T`` -> bf16 ``[M, N]`` on the block-scaled tensor-core path, accumulated in fp32 and rounded once.  An
-    ``x`` that is not quantised yet is quantised in the call (:func:`quantize_mxfp4`).  M and N may be any number."""
+    ``x`` that is not quantised yet is quantised in the call (:func:`quantize_mxfp4`).  M and N may be any number.  The sum over K is
+    divided by a rule on M, N and K, so the last bits of a row may differ with the number of rows in the call; the same call gives the same bits."""
     if not isinstance(w, MxFp4):
         raise FusedGemmError("w must be quantised (quantize_mxfp4)")
     raw = not isinstance(x, MxFp4)
