@@ -85,6 +85,9 @@ int bshmem_fused_gemm(const bshmem_fused_args_t* args, cudaStream_t stream);
 #define BSHMEM_FUSED_B_TRANSPOSED 2
 int bshmem_fused_gemm_layout(const bshmem_fused_args_t* args, int layout, cudaStream_t stream);
 int bshmem_fused_gemm_smem_bytes(void);
+/* A device int for the `error_flag` of any entry of this library on GPU `device`, zero at first and kept until the process ends; null if there is no such GPU (or no
+ * room).  May be called while a stream is being captured. */
+int* bshmem_fused_error_word(int device);
 
 #ifdef __cplusplus
 }

@@ -56,16 +56,28 @@ def fused_lib() -> C.CDLL:
         _lib.bshmem_fused_gemm.argtypes = [C.POINTER(_Args), C.c_void_p]
         _lib.bshmem_fused_gemm_layout.restype = C.c_int
         _lib.bshmem_fused_gemm_layout.argtypes = [C.POINTER(_Args), C.c_int, C.c_void_p]
+        _lib.bshmem_fused_error_word.restype, _lib.bshmem_fused_error_word.argtypes = C.c_void_p, [C.c_int]
     return _lib
 
 
 _err_flags: dict[int, torch.Tensor] = {}
 
 
+class _Word:
+    """One int32 in device memory, as torch takes it over."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def _error_flag(device) -> torch.Tensor:
+    """The device's error word.  It is no tensor of torch's own: the first call may be one that is captured, and a replay of the graph would zero it."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     if idx not in _err_flags:
-        _err_flags[idx] = torch.zeros(1, dtype=torch.int32, device=device)
+        address = fused_lib().bshmem_fused_error_word(idx)
+        if not address:
+            raise FusedGemmError(f"no memory for the error word of GPU {idx}")
+        _err_flags[idx] = torch.as_tensor(_Word(address), device=torch.device("cuda", idx))
     return _err_flags[idx]
 
 

@@ -456,3 +456,38 @@ def test_offsets_beyond_32_bits():
     assert ((dl[-tail:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * p * c.max()).all()
     torch.cuda.synchronize()
     fused_gemm.check_errors()
+
+
+FIRST_CALL = """
+import torch
+from nvshmem_b200.ops import fused_gemm as fg
+from nvshmem_b200.ops import gemm_mxfp4, quantize_mxfp4, rms_norm
+torch.cuda.set_device(0)
+x, w = torch.randn(300, 512, device="cuda"), torch.ones(512, device="cuda")
+if CALL == "norm":
+    call, want = lambda: rms_norm(x, w), x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+else:
+    q = quantize_mxfp4(x)
+    call, want = lambda: gemm_mxfp4(q, q).float(), q.dequantize(torch.float32) @ q.dequantize(torch.float32).t()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = call()
+fg.check_errors()
+fg._error_flag(x.device).fill_(1)      # as a kernel does that gave up on a wait
+graph.replay()
+assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -7).all()
+assert fg.take_error() == 1 and fg.take_error() == 0
+graph.replay()
+fg.check_errors()
+"""
+
+
+@pytest.mark.parametrize("call", ["norm", "gemm"])
+def test_a_first_call_that_is_captured_keeps_errors(call):
+    """In a process of its own: the error word is made by the first call; a replay must not take an error back that nobody has read."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", f"CALL = {call!r}\n" + FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0, run.stderr[-2000:]
